@@ -1,0 +1,359 @@
+// Rows of the 4-bit paged key/value cache: written, read back, chosen for eviction and moved (layout: include/kv4.cuh).
+//
+// Formulas.  A group of 64 columns x of one token and head is stored as lo = min x, step = (max x - min x) / 15 rounded up to
+// bf16 and codes = round((x - lo) / step) (to nearest, ties to even, 0 where step = 0); it stands for code * step + lo.  lo is one
+// of the bf16 inputs and therefore exact; the step is rounded up so that 15 steps always reach the maximum, and code * step + lo has
+// one rounding in fp32 (code * step has 12 bits).  A group with a NaN, an infinity or a range beyond fp32 is NaN as a whole.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../include/kv4.cuh"
+#include "../include/omni_ptx.cuh"
+
+namespace omni {
+
+constexpr int KV4_SITE_ROWS = 81, KV4_SITE_KEEP = 82, KV4_SITE_MOVE = 83;
+
+// ------------------------------------------------------------------------------------------------ write and read
+struct Kv4Rows {
+  const __nv_bfloat16 *k, *v;       // write: sources; element strides below
+  __nv_bfloat16 *k_out, *v_out;     // read: [n, Hkv, d] contiguous
+  long long k_row, v_row;
+  int k_head, v_head;
+  const long long* slots;           // [n]; negative: skipped (write), zeros (read)
+  long long n;
+  float* weights;                   // write: [blocks, Hkv, block] or null, set to zero
+  int* positions;                   // write: [blocks, Hkv, block] or null, set to token_positions[i]
+  const long long* token_positions;
+};
+
+// A thread holds one word (8 columns) of one row; the 8 threads of a group find its range with three shuffles.  Bound by memory:
+// reads 2 d bytes and writes 9 d / 16 a row.
+template <bool VEC>
+__global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows a, Kv4Cache c, int words_log2, OmniStatus* st) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int u = (int)(i & ((1 << words_log2) - 1));
+  const long long row = i >> words_log2;                            // (token, head, key or value)
+  const long long th = row >> 1;
+  const bool values = row & 1;
+  const long long tok = th / c.hkv;
+  const int h = (int)(th - tok * c.hkv);
+  if (tok >= a.n) return;                                           // whole rows, and rows are whole groups of 8 threads
+  const unsigned mask = 0xffu << (threadIdx.x & 24);
+  const __nv_bfloat16* src = values ? a.v + tok * a.v_row + (long long)h * a.v_head : a.k + tok * a.k_row + (long long)h * a.k_head;
+  src += u * 8;
+  __nv_bfloat162 x[4];
+  if (VEC) {
+    *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(src);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __halves2bfloat162(src[2 * j], src[2 * j + 1]);
+  }
+  __nv_bfloat162 lo2 = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3]));
+  __nv_bfloat162 hi2 = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
+  __nv_bfloat16 lo = __hmin_nan(__low2bfloat16(lo2), __high2bfloat16(lo2)), hi = __hmax_nan(__low2bfloat16(hi2), __high2bfloat16(hi2));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    lo = __hmin_nan(lo, __shfl_xor_sync(mask, lo, o));
+    hi = __hmax_nan(hi, __shfl_xor_sync(mask, hi, o));
+  }
+  const float low = __bfloat162float(lo), range = __fsub_rn(__bfloat162float(hi), low);
+  float step = __uint_as_float((__float_as_uint(__fdiv_rn(range, 15.f)) + 0xffffu) & 0xffff0000u);
+  if (!(range < INFINITY)) step = __uint_as_float(0x7fc00000u);     // NaN or infinite
+  uint32_t word = 0;
+  if (step > 0.f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __bfloat1622float2(x[j]);
+      const float c0 = fminf(rintf(__fdiv_rn(__fsub_rn(f.x, low), step)), 15.f), c1 = fminf(rintf(__fdiv_rn(__fsub_rn(f.y, low), step)), 15.f);
+      word |= ((uint32_t)c0 | (uint32_t)c1 << 4) << (8 * j);
+    }
+  }
+  const long long slot = a.slots[tok];
+  if (slot < 0) return;
+  const long long blk = slot / c.block;
+  if (blk >= c.blocks) {
+    if (u == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_ROWS, (int)tok);
+    return;
+  }
+  const int t = (int)(slot - blk * c.block);
+  uint8_t* piece = (values ? c.v : c.k) + c.at(blk, h);
+  *reinterpret_cast<uint32_t*>(piece + (values ? c.v_word(t, u) : c.k_word(t, u))) = word;
+  if ((u & 7) == 0)
+    *reinterpret_cast<uint32_t*>(piece + c.scale_word(t, u >> 3)) = (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
+  if (u == 0 && !values) {
+    const long long at = (blk * c.hkv + h) * c.block + t;
+    if (a.weights != nullptr) a.weights[at] = 0.f;
+    if (a.positions != nullptr) a.positions[at] = (int)a.token_positions[tok];
+  }
+}
+
+// The inverse: one word of codes and its group's word to 8 bf16 values.  Bound by memory: reads 9 d / 16 bytes and writes 2 d a row.
+__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Rows a, Kv4Cache c, int words_log2, OmniStatus* st) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int u = (int)(i & ((1 << words_log2) - 1));
+  const long long row = i >> words_log2;
+  const long long th = row >> 1;
+  const bool values = row & 1;
+  const long long tok = th / c.hkv;
+  const int h = (int)(th - tok * c.hkv);
+  if (tok >= a.n) return;
+  const long long slot = a.slots[tok], blk = slot < 0 ? -1 : slot / c.block;
+  uint4 out = make_uint4(0u, 0u, 0u, 0u);
+  if (blk >= c.blocks) {
+    if (u == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_ROWS, (int)tok);
+  } else if (blk >= 0) {
+    const int t = (int)(slot - blk * c.block);
+    const uint8_t* piece = (values ? c.v : c.k) + c.at(blk, h);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(piece + (values ? c.v_word(t, u) : c.k_word(t, u)));
+    const uint32_t s = *reinterpret_cast<const uint32_t*>(piece + c.scale_word(t, u >> 3));
+    const float step = kv4_step(s), low = kv4_low(s);
+    __nv_bfloat162 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[j] = __floats2bfloat162_rn(fmaf((float)((w >> (8 * j)) & 15u), step, low), fmaf((float)((w >> (8 * j + 4)) & 15u), step, low));
+    out = *reinterpret_cast<uint4*>(x);
+  }
+  *reinterpret_cast<uint4*>((values ? a.v_out : a.k_out) + (th << words_log2) * 8 + u * 8) = out;
+}
+
+// ------------------------------------------------------------------------------------------------ eviction
+// Order of eviction: larger keys stay.  Places of the first and last positions come before all weights, a NaN before the numbers.
+__device__ __forceinline__ uint32_t kv4_keep_key(float w, int pos, int first, int last_from) {
+  if (pos < first || pos >= last_from) return 0xffffffffu;
+  if (w != w) return 0xfffffffeu;
+  const uint32_t b = __float_as_uint(w + 0.f);                      // -0 counts as 0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// Exclusive sum over a block of 1024 threads; `total` gets the sum.
+__device__ __forceinline__ int kv4_block_scan(int x, int& total) {
+  __shared__ int part[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int v = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();
+  if (lane == 31) part[warp] = v;
+  __syncthreads();
+  int base = 0, sum = 0;
+  for (int i = 0; i < 32; ++i) {
+    if (i < warp) base += part[i];
+    sum += part[i];
+  }
+  total = sum;
+  return base + v - x;
+}
+
+struct Kv4Keep {
+  const float* weights;
+  const int *positions, *table, *seq_lens, *seen;
+  long long blocks;
+  int table_ld, table_w, block, hkv, budget, first, last;
+  int *keep, *lens, *holes;         // [B, Hkv, budget], [B], scratch as keep
+};
+
+// One block for a request and head: the key of the budget-th heaviest place by a radix selection of 8 bits a pass, then one pass
+// in the order of places that fills the places below the budget that are not kept with the kept places behind it.
+__global__ void __launch_bounds__(1024) kv4_keep_kernel(Kv4Keep a, OmniStatus* st) {
+  const int b = blockIdx.y, h = blockIdx.x;
+  __shared__ int hist[256];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_left;
+  int n = max(a.seq_lens[b], 0);
+  if (n > a.table_w * a.block) {
+    if (threadIdx.x == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
+    n = a.table_w * a.block;
+  }
+  int* keep = a.keep + ((long long)b * a.hkv + h) * a.budget;
+  if (h == 0 && threadIdx.x == 0) a.lens[b] = min(n, a.budget);
+  if (n <= a.budget) {
+    for (int j = threadIdx.x; j < a.budget; j += 1024) keep[j] = j < n ? j : -1;
+    return;
+  }
+  const int last_from = a.seen[b] - a.last;
+  auto key_of = [&](int j) -> uint32_t {
+    const int blk = a.table[(long long)b * a.table_ld + j / a.block];
+    if (blk < 0 || blk >= a.blocks) {
+      report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
+      return 0u;
+    }
+    const long long at = ((long long)blk * a.hkv + h) * a.block + j % a.block;
+    return kv4_keep_key(a.weights[at], a.positions[at], a.first, last_from);
+  };
+  uint32_t prefix = 0, mask = 0;
+  int left = a.budget;                                              // of the places whose key starts with the prefix, so many stay
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += 1024) {
+      const uint32_t key = key_of(j);
+      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int d = 255, rest = left;
+      while (d > 0 && hist[d] < rest) rest -= hist[d--];
+      s_left = rest;
+      s_prefix = prefix | (uint32_t)d << shift;
+    }
+    __syncthreads();
+    prefix = s_prefix;
+    left = s_left;
+    mask |= 255u << shift;
+    __syncthreads();
+  }
+  // `prefix` is the key of the last place that stays; `left` of the places with that key do, the lowest first
+  int* holes = a.holes + ((long long)b * a.hkv + h) * a.budget;
+  int equal = 0, hole = 0, source = 0;                              // found so far
+  for (int j0 = 0; j0 < n; j0 += 1024) {
+    const int j = j0 + threadIdx.x;
+    const uint32_t key = j < n ? key_of(j) : 0u;
+    const bool same = j < n && key == prefix;
+    int all;
+    const int rank = equal + kv4_block_scan(same, all);
+    equal += all;
+    const bool stays = j < n && (key > prefix || (same && rank < left));
+    const bool is_hole = j < a.budget && !stays, is_source = j >= a.budget && stays;
+    if (j < a.budget && stays) keep[j] = j;
+    const int hr = hole + kv4_block_scan(is_hole, all);
+    hole += all;
+    if (is_hole) holes[hr] = j;
+    __syncthreads();                                                // a source's hole may have been found in this chunk
+    const int sr = source + kv4_block_scan(is_source, all);
+    source += all;
+    if (is_source) keep[holes[sr]] = j;
+  }
+}
+
+struct Kv4Move {
+  const int *table, *keep;
+  int table_ld, table_w, budget;
+  float* weights;
+  int* positions;
+};
+
+// A warp looks at 32 places and copies the rows of those that are filled from elsewhere.  Sources lie behind the budget and places
+// below it, so no row is both and the order of the copies does not matter.
+__global__ void __launch_bounds__(256) kv4_move_kernel(Kv4Move a, Kv4Cache c, OmniStatus* st) {
+  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31;
+  const int j = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 32 + lane;
+  const int* table = a.table + (long long)b * a.table_ld;
+  int from = -1, fb = 0, tb = 0;
+  if (j < a.budget) {
+    const int s = a.keep[((long long)b * c.hkv + h) * a.budget + j];
+    if (s >= 0 && s != j) {
+      const int w0 = s / c.block, w1 = j / c.block;
+      bool ok = s >= a.budget && w0 < a.table_w && w1 < a.table_w;
+      if (ok) {
+        fb = table[w0];
+        tb = table[w1];
+        ok = fb >= 0 && fb < c.blocks && tb >= 0 && tb < c.blocks;
+      }
+      if (ok) from = s;
+      else report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_MOVE, b);
+    }
+  }
+  unsigned todo = __ballot_sync(0xffffffffu, from >= 0);
+  const int words = c.d / 8, groups = c.groups();
+  while (todo) {
+    const int l = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const int s = __shfl_sync(0xffffffffu, from, l), sb = __shfl_sync(0xffffffffu, fb, l), db = __shfl_sync(0xffffffffu, tb, l);
+    const int ft = s % c.block, tt = (j - lane + l) % c.block;
+    const long long fp = c.at(sb, h), tp = c.at(db, h);
+    for (int u = lane; u < words; u += 32) {
+      *reinterpret_cast<uint32_t*>(c.k + tp + c.k_word(tt, u)) = *reinterpret_cast<const uint32_t*>(c.k + fp + c.k_word(ft, u));
+      *reinterpret_cast<uint32_t*>(c.v + tp + c.v_word(tt, u)) = *reinterpret_cast<const uint32_t*>(c.v + fp + c.v_word(ft, u));
+    }
+    if (lane < groups) {
+      *reinterpret_cast<uint32_t*>(c.k + tp + c.scale_word(tt, lane)) = *reinterpret_cast<const uint32_t*>(c.k + fp + c.scale_word(ft, lane));
+      *reinterpret_cast<uint32_t*>(c.v + tp + c.scale_word(tt, lane)) = *reinterpret_cast<const uint32_t*>(c.v + fp + c.scale_word(ft, lane));
+    }
+    if (lane == 31) {
+      const long long x = ((long long)sb * c.hkv + h) * c.block + ft, y = ((long long)db * c.hkv + h) * c.block + tt;
+      if (a.weights != nullptr) a.weights[y] = a.weights[x];
+      if (a.positions != nullptr) a.positions[y] = a.positions[x];
+    }
+  }
+}
+
+static int kv4_log2(int x) {
+  int l = 0;
+  while ((1 << l) < x) ++l;
+  return l;
+}
+
+}  // namespace omni
+
+using namespace omni;
+
+extern "C" int omni_kv4_write(const void* k, long long k_row, int k_head, const void* v, long long v_row, int v_head, const long long* slots,
+                              long long n, void* k_cache, void* v_cache, long long blocks, int block, int hkv, int d, float* weights,
+                              int* positions, const long long* token_positions, void* status, cudaStream_t stream) {
+  const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
+  if (!kv4_shape_ok(c)) return -1;
+  if ((positions == nullptr) != (token_positions == nullptr)) return -2;
+  if (n <= 0) return 0;
+  Kv4Rows a = {};
+  a.k = (const __nv_bfloat16*)k;
+  a.v = (const __nv_bfloat16*)v;
+  a.k_row = k_row;
+  a.v_row = v_row;
+  a.k_head = k_head;
+  a.v_head = v_head;
+  a.slots = slots;
+  a.n = n;
+  a.weights = weights;
+  a.positions = positions;
+  a.token_positions = token_positions;
+  const int wl = kv4_log2(d / 8);
+  const long long grid = (((n * hkv * 2) << wl) + 255) / 256;
+  if (grid > 0x7fffffffll) return -3;
+  const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && (k_row | v_row) % 8 == 0 && (k_head | v_head) % 8 == 0;
+  if (vec) kv4_write_kernel<true><<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
+  else kv4_write_kernel<false><<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
+  return (int)cudaGetLastError();
+}
+
+extern "C" int omni_kv4_read(const void* k_cache, const void* v_cache, long long blocks, int block, int hkv, int d, const long long* slots,
+                             long long n, void* k_out, void* v_out, void* status, cudaStream_t stream) {
+  const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
+  if (!kv4_shape_ok(c)) return -1;
+  if (n <= 0) return 0;
+  Kv4Rows a = {};
+  a.k_out = (__nv_bfloat16*)k_out;
+  a.v_out = (__nv_bfloat16*)v_out;
+  a.slots = slots;
+  a.n = n;
+  const int wl = kv4_log2(d / 8);
+  const long long grid = (((n * hkv * 2) << wl) + 255) / 256;
+  if (grid > 0x7fffffffll) return -3;
+  kv4_read_kernel<<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
+  return (int)cudaGetLastError();
+}
+
+extern "C" int omni_kv4_keep(const float* weights, const int* positions, long long blocks, int block, int hkv, const int* table, int table_ld,
+                             int table_w, const int* seq_lens, const int* seen, int B, int budget, int first, int last, int* keep, int* lens,
+                             int* scratch, void* status, cudaStream_t stream) {
+  if (blocks <= 0 || block < 1 || hkv < 1 || hkv > 65535 || B > 65535 || budget < 1 || first < 0 || last < 0 || first + last > budget) return -1;
+  if (B <= 0) return 0;
+  const Kv4Keep a = {weights, positions, table, seq_lens, seen, blocks, table_ld, table_w, block, hkv, budget, first, last, keep, lens, scratch};
+  kv4_keep_kernel<<<dim3(hkv, B), 1024, 0, stream>>>(a, (OmniStatus*)status);
+  return (int)cudaGetLastError();
+}
+
+extern "C" int omni_kv4_move(void* k_cache, void* v_cache, long long blocks, int block, int hkv, int d, const int* table, int table_ld, int table_w,
+                             const int* keep, int B, int budget, float* weights, int* positions, void* status, cudaStream_t stream) {
+  const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
+  if (!kv4_shape_ok(c) || hkv > 65535 || B > 65535 || budget < 1) return -1;
+  if (B <= 0) return 0;
+  const Kv4Move a = {table, keep, table_ld, table_w, budget, weights, positions};
+  kv4_move_kernel<<<dim3((budget + 255) / 256, hkv, B), 256, 0, stream>>>(a, c, (OmniStatus*)status);
+  return (int)cudaGetLastError();
+}

@@ -1,0 +1,353 @@
+"""The 4-bit paged key/value cache: rows written and read back, decode attention over it, and eviction by attention weight
+(``csrc/kernels/kv4_cache.cu``, ``csrc/kernels/kv4_decode.cu``), with fp32 PyTorch references.
+
+A cache (one for keys, one for values) is uint8 [blocks, Hkv, block_size, 9 d / 16]; ``kv4_cache`` makes a pair.  64 columns of a
+token's row share a bf16 step and a bf16 lowest value and stand for ``code * step + lowest``, so a row takes 4.5 bits an element.
+Inside the piece of a block and head the bytes lie as the kernels want them (``csrc/include/kv4.cuh``); ``kv4_read`` gives the
+values.  Whole blocks can be copied between caches like those of any paged cache.
+
+A request's tokens lie in the *places* 0, 1, ... of its block table.  Eviction (``kv4_keep``, ``kv4_move``) keeps ``budget`` tokens of
+every head, its own choice for each, in the places below the budget; ``positions`` says which token of the sequence a place holds,
+``weights`` how much attention it has had.  Keys carry their rotation with them, so attention does not ask for the order.
+
+Calls write to no memory but their outputs and what the allocator gives them for the call: they may run on several streams, and
+captured, as their arguments allow.  Block ids and slots outside the cache are skipped and reported by
+``ops._native.check_status``."""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+
+from . import _native as nat
+
+GROUP = 64
+DIMS = (64, 128, 256)
+
+
+def kv4_cache(num_blocks, block_size, hkv, d, device=None):
+    """(keys, values) of ``num_blocks`` blocks, all zero."""
+    assert d in DIMS and block_size % 16 == 0, f"head size {DIMS} and blocks of a multiple of 16 tokens: {d}, {block_size}"
+    return tuple(torch.zeros(num_blocks, hkv, block_size, d * 9 // 16, dtype=torch.uint8, device=device) for _ in range(2))
+
+
+# ----------------------------------------------------------------------------- layout and references
+def _code_places(block, d, values, device=None):
+    """(byte, shift) of the code of every [token, column] in the piece of one block and head."""
+    t = torch.arange(block, device=device)[:, None]
+    col = torch.arange(d, device=device)[None, :]
+    per = min(d // GROUP, 2)
+    g, i, j = col // GROUP, col % GROUP // 8, col % 8
+    if values:
+        pair = t // 2
+        chunk = i ^ (pair % 4 * 2) if per == 2 else i ^ (pair // 2 % 2 * 4)
+        byte = (g // per * block + pair * 2) * 32 * per + chunk * 8 * per + t % 2 * 4 * per + g % per * 4 + j // 2
+    else:
+        byte = (g // per * block + t) * 32 * per + (i // 2 * 2 * per + g % per * 2 + i % 2) * 4 + j // 2
+    return byte, (j % 2 * 4).expand(block, d)
+
+
+def kv4_quantise_ref(x):
+    """x [..., d] -> codes uint8 [..., d], (step, lowest) bf16 [..., d / 64]."""
+    v = x.float().unflatten(-1, (-1, GROUP))
+    lo, hi = v.amin(-1), v.amax(-1)
+    step = (((hi - lo) / torch.full_like(hi, 15.0)).contiguous().view(torch.int32) + 0xffff & -0x10000).view(torch.float32)
+    step = torch.where(torch.isfinite(hi - lo), step, torch.full_like(step, float("nan")))
+    code = torch.round((v - lo[..., None]) / step[..., None]).clamp(0, 15)
+    code = torch.where(step[..., None] > 0, code, torch.zeros_like(code))
+    return code.to(torch.uint8).flatten(-2), step.bfloat16(), lo.bfloat16()
+
+
+def _pieces(cache):
+    blocks, hkv, block, row = cache.shape
+    return cache.view(blocks, hkv, block * row), block, row * 16 // 9
+
+
+def _write_ref(x, slots, cache, values):
+    flat, block, d = _pieces(cache)
+    byte, shift = _code_places(block, d, values)
+    head = torch.arange(cache.shape[1])[:, None]
+    codes, step, lo = kv4_quantise_ref(x)
+    scales = torch.stack([step, lo], -1).flatten(2).contiguous().view(torch.uint8)
+    for i, slot in enumerate(slots.tolist()):
+        if slot < 0:
+            continue
+        at, t = flat[slot // block], slot % block
+        for half in (0, 4):
+            here = shift[t] == half
+            b = byte[t][here]
+            at[head, b] = at[head, b] & (0xf0 if half == 0 else 0x0f) | codes[i][:, here] << half
+        p = block * d // 2 + t * (d // 16)
+        at[:, p:p + d // 16] = scales[i]
+
+
+def _values_ref(cache, blk, t, values, head=None):
+    """fp32 values of the rows (blk, t): [..., Hkv, d], or [..., d] of the heads ``head``."""
+    flat, block, d = _pieces(cache)
+    byte, shift = _code_places(block, d, values, cache.device)
+    byte, shift = byte[t], shift[t].to(torch.uint8)
+    sc = block * d // 2 + t[..., None] * (d // 16) + torch.arange(d // 16, device=cache.device)
+    if head is None:
+        head = torch.arange(cache.shape[1], device=cache.device)
+        blk, byte, shift, sc = blk[..., None], byte[..., None, :], shift[..., None, :], sc[..., None, :]
+    blk, head = blk[..., None], head[..., None]
+    codes = (flat[blk, head, byte] >> shift & 15).float().unflatten(-1, (-1, GROUP))
+    scales = flat[blk, head, sc].contiguous().view(torch.bfloat16).float().unflatten(-1, (-1, 2))
+    return (codes * scales[..., :1] + scales[..., 1:]).flatten(-2)
+
+
+def kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights=None, decay=1.0):
+    T, hq, d = q.shape
+    hkv, block = k_cache.shape[1], k_cache.shape[2]
+    B = seq_lens.shape[0]
+    rows, rep = T // B if B else 0, hq // hkv
+    out = torch.zeros(T, hq, d, dtype=torch.float32, device=q.device)
+    for b, n in enumerate(seq_lens.tolist()):
+        if n <= 0:
+            continue
+        t = torch.arange(n, device=q.device)
+        blk = block_table[b].long()[t // block]
+        k, v = (_values_ref(c, blk, t % block, x).transpose(0, 1).repeat_interleave(rep, 0) for c, x in ((k_cache, False), (v_cache, True)))
+        s = torch.einsum("rhd,hnd->rhn", q[b * rows:(b + 1) * rows].float(), k) * scale
+        sees = n - rows + 1 + torch.arange(rows, device=q.device)
+        s = s.masked_fill(t >= sees[:, None, None], float("-inf"))
+        p = torch.where(sees[:, None, None] > 0, torch.softmax(s, -1), torch.zeros_like(s))
+        for i in range(rows):
+            m = max(0, int(sees[i]))
+            out[b * rows + i] = torch.einsum("hn,hnd->hd", p[i, :, :m], v[:, :m])
+        if weights is not None:
+            step = p.sum(0).view(hkv, rep, n).sum(1).transpose(0, 1)                  # [n, Hkv]
+            old = weights[blk, :, t % block]
+            weights[blk, :, t % block] = step if decay == 0 else old * decay + step
+    return out.to(q.dtype)
+
+
+def kv4_keep_ref(weights, positions, block_table, seq_lens, seen, budget, keep_first=0, keep_last=0):
+    hkv, block = weights.shape[1], weights.shape[2]
+    B = seq_lens.shape[0]
+    keep = torch.full((B, hkv, budget), -1, dtype=torch.int32)
+    lens = seq_lens.clamp(0, budget).to(torch.int32)
+    for b, n in enumerate(seq_lens.tolist()):
+        t = torch.arange(max(n, 0))
+        blk = block_table[b].long()[t // block]
+        for h in range(hkv):
+            place = list(range(min(n, budget)))
+            if n > budget:
+                w, pos = weights[blk, h, t % block].tolist(), positions[blk, h, t % block].tolist()
+                rank = []
+                for j in range(n):
+                    safe = pos[j] < keep_first or pos[j] >= int(seen[b]) - keep_last
+                    rank.append((2, 0.0) if safe else (1, 0.0) if w[j] != w[j] else (0, w[j]))
+                stay = set(sorted(range(n), key=lambda j: rank[j], reverse=True)[:budget])     # a stable sort: the lowest of equals
+                far = iter(sorted(j for j in stay if j >= budget))
+                place = [j if j in stay else next(far) for j in range(budget)]
+            keep[b, h, :len(place)] = torch.tensor(place, dtype=torch.int32)
+    return keep, lens
+
+
+def _move_ref(k_cache, v_cache, block_table, keep, weights, positions):
+    block = k_cache.shape[2]
+    to = torch.arange(keep.shape[2])
+    b, h, j = ((keep >= 0) & (keep != to)).nonzero(as_tuple=True)
+    s = keep[b, h, j].long()
+    fb, ft, tb, tt = block_table[b, s // block].long(), s % block, block_table[b, j // block].long(), j % block
+    for cache, values in ((k_cache, False), (v_cache, True)):
+        flat, _, d = _pieces(cache)
+        byte, shift = _code_places(block, d, values)
+        codes = flat[fb[:, None], h[:, None], byte[ft]] >> shift[ft].to(torch.uint8) & 15
+        for half in (0, 4):
+            here = shift[0] == half
+            at = (tb[:, None], h[:, None], byte[tt][:, here])
+            flat[at] = flat[at] & (0xf0 if half == 0 else 0x0f) | codes[:, here] << half
+        sc = block * d // 2 + torch.arange(d // 16)
+        flat[tb[:, None], h[:, None], sc + tt[:, None] * (d // 16)] = flat[fb[:, None], h[:, None], sc + ft[:, None] * (d // 16)]
+    for x in (weights, positions):
+        if x is not None:
+            x[tb, h, tt] = x[fb, h, ft]
+
+
+# ----------------------------------------------------------------------------- calls
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_ARGS = {
+    "omni_kv4_write": (_P, _L, _I, _P, _L, _I, _P, _L, _P, _P, _L, _I, _I, _I, _P, _P, _P, _P, _P),
+    "omni_kv4_read": (_P, _P, _L, _I, _I, _I, _P, _L, _P, _P, _P, _P),
+    "omni_kv4_keep": (_P, _P, _L, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P),
+    "omni_kv4_move": (_P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P),
+    "omni_kv4_decode": (_P, _L, _I, _P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _I, _I, _I, _F, _I, _P, _P, _P, _F, _P, _P),
+}
+_bound = {}
+
+
+def _call(name, device, *args):
+    """Launch on the current stream of the tensors' own device."""
+    fn = _bound.get(name)
+    if fn is None:
+        lib = nat.lib()
+        getattr(lib._cdll, name).argtypes = _ARGS[name]
+        fn = _bound[name] = getattr(lib, name)
+    here = contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    with here:
+        rc = fn(*args, nat.status_buffer(device).data_ptr(), torch.cuda.current_stream(device).cuda_stream)
+    nat.check_rc(rc, name)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _check_caches(k_cache, v_cache):
+    """(blocks, Hkv, block, d) of a pair of caches."""
+    assert k_cache.dtype == v_cache.dtype == torch.uint8 and k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "a pair of uint8 caches of one shape"
+    assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.device == v_cache.device, "contiguous caches on one device"
+    blocks, hkv, block, row = k_cache.shape
+    d = row * 16 // 9
+    assert d in DIMS and row * 16 == d * 9 and block > 0 and block % 16 == 0 and hkv > 0, \
+        f"rows of 9 d / 16 bytes with d in {DIMS} and blocks of a multiple of 16 tokens: {row}, {block}"
+    return blocks, hkv, block, d
+
+
+def _check_ints(device, dtype=torch.int32, **tensors):
+    for name, t in tensors.items():
+        assert t.dtype == dtype and t.device == device and (t.dim() == 0 or t.stride(-1) == 1), f"{name}: {dtype} on {device}, rows without gaps"
+
+
+def _check_per_place(device, shape, **tensors):
+    """``weights`` and ``positions``: a number for every place of the caches."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        dtype = torch.int32 if name == "positions" else torch.float32
+        assert t.dtype == dtype and t.device == device and t.is_contiguous() and tuple(t.shape) == shape, f"{name}: contiguous {dtype} {list(shape)}"
+
+
+def _check_table(table, device, B):
+    _check_ints(device, block_table=table)
+    assert table.dim() == 2 and table.shape[0] >= B, f"block_table: a row for each of the {B} requests"
+
+
+def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token_positions=None):
+    """Rows k, v [T, Hkv, d] (bf16; any row and head pitch) into the slots ``slots`` [T] int64 (block * block size + place in the
+    block; negative: not stored).  The slots of a call differ.  ``weights`` / ``positions`` [blocks, Hkv, block], where given, are
+    set to 0 and to ``token_positions`` [T] int64 in those slots."""
+    blocks, hkv, block, d = _check_caches(k_cache, v_cache)
+    for name, x in (("k", k), ("v", v)):
+        assert x.dim() == 3 and x.dtype == torch.bfloat16 and x.shape[1:] == (hkv, d) and x.device == k_cache.device, \
+            f"{name}: bf16 [T, {hkv}, {d}] on {k_cache.device}"
+        assert x.stride(2) == 1, f"{name}: columns without gaps"
+    T = k.shape[0]
+    _check_ints(k.device, torch.int64, slots=slots)
+    assert v.shape[0] == T and slots.shape == (T,), "a row of v and a slot for every row of k"
+    _check_per_place(k.device, (blocks, hkv, block), weights=weights, positions=positions)
+    assert (positions is None) == (token_positions is None), "positions and token_positions come together"
+    if token_positions is not None:
+        _check_ints(k.device, torch.int64, token_positions=token_positions)
+        assert token_positions.shape == (T,)
+    if not k.is_cuda:
+        _write_ref(k, slots, k_cache, False)
+        _write_ref(v, slots, v_cache, True)
+        ok = slots >= 0
+        blk, t = slots[ok] // block, slots[ok] % block
+        if weights is not None:
+            weights[blk, :, t] = 0.0
+        if positions is not None:
+            positions[blk, :, t] = token_positions[ok].to(torch.int32)[:, None]
+        return
+    if T == 0:
+        return
+    _call("omni_kv4_write", k.device, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _p(slots), T, _p(k_cache), _p(v_cache),
+          blocks, block, hkv, d, _p(weights), _p(positions), _p(token_positions))
+
+
+def kv4_read(k_cache, v_cache, slots):
+    """(k, v) [T, Hkv, d] bf16 of the slots ``slots`` [T] int64; zeros for negative ones.  A slot may be named more than once."""
+    blocks, hkv, block, d = _check_caches(k_cache, v_cache)
+    _check_ints(k_cache.device, torch.int64, slots=slots)
+    assert slots.dim() == 1
+    T = slots.shape[0]
+    if not k_cache.is_cuda:
+        s = slots.clamp_min(0)
+        ok = (slots >= 0)[:, None, None]
+        return tuple(torch.where(ok, _values_ref(c, s // block, s % block, x), torch.zeros(())).bfloat16() for c, x in ((k_cache, False), (v_cache, True)))
+    k, v = (torch.empty(T, hkv, d, dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
+    if T:
+        _call("omni_kv4_read", k_cache.device, _p(k_cache), _p(v_cache), blocks, block, hkv, d, _p(slots), T, _p(k), _p(v))
+    return k, v
+
+
+def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=None, weights=None, decay=1.0):
+    """Attention of the last tokens of every request over its cached ones: q [B n, Hq, d] bf16 (any row and head pitch), the ``n``
+    rows of a request one after the other; row i sees the first ``seq_lens[b] - n + 1 + i`` of the request's places (none: zeros).
+    ``block_table`` [B, blocks of a request] int32, ``seq_lens`` [B] int32, with the rows' own tokens.  Returns [B n, Hq, d].
+
+    ``weights`` [blocks, Hkv, block] fp32: of every place below seq_lens[b] becomes decay * weights + the softmax weights that the
+    rows and the query heads of its key/value head give it (decay 0: whatever was there is dropped).  Requests that share a block
+    would write the same numbers: give ``weights`` only where blocks belong to one request.  ``max_seq_len`` (a bound of
+    ``seq_lens``) shapes the launch; without it the width of the block table does."""
+    blocks, hkv, block, d = _check_caches(k_cache, v_cache)
+    assert q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == d and q.device == k_cache.device and q.stride(2) == 1, \
+        f"q: bf16 [rows, Hq, {d}] on {k_cache.device}, columns without gaps"
+    T, hq, B = q.shape[0], q.shape[1], seq_lens.shape[0]
+    assert hq > 0 and hq % hkv == 0, f"{hq} query heads do not divide over {hkv} key/value heads"
+    assert T == 0 if B == 0 else T > 0 and T % B == 0, f"{T} rows are not the same number for each of {B} requests"
+    _check_ints(q.device, seq_lens=seq_lens)
+    assert seq_lens.dim() == 1
+    _check_table(block_table, q.device, B)
+    _check_per_place(q.device, (blocks, hkv, block), weights=weights)
+    if not q.is_cuda:
+        return kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights, decay)
+    out = torch.empty(T, hq, d, dtype=q.dtype, device=q.device)
+    if T:
+        width = block_table.shape[1]
+        longest = width * block if max_seq_len is None else min(max_seq_len, width * block)
+        lse = torch.empty(T * hq, dtype=torch.float32, device=q.device) if weights is not None else None
+        _call("omni_kv4_decode", q.device, _p(q), q.stride(0), q.stride(1), _p(k_cache), _p(v_cache), blocks, block, hkv, d, _p(block_table),
+              block_table.stride(0), width, _p(seq_lens), B, T // B, hq, scale, longest, _p(out), _p(lse), _p(weights), decay)
+    return out
+
+
+def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first=0, keep_last=0, max_seq_len=None):
+    """Which tokens stay when every head of a request may keep ``budget`` of its first ``seq_lens[b]`` places: those of positions
+    below ``keep_first`` and from ``seen[b] - keep_last`` on (``seen`` [B] int32: tokens that the request has had), then the
+    heaviest by ``weights``, among equals the lowest place.  A NaN counts as heavier than any number.
+
+    Returns (keep [B, Hkv, budget] int32, lens [B] int32 = the smaller of seq_lens and budget).  keep[b, h, j] is the place whose token
+    is to be in place j: j itself where that stays, else one of the kept places from the budget on, in ascending order over the
+    places that become free; -1 from lens[b] on.  Nothing is moved: see ``kv4_move``."""
+    assert weights.dim() == 3, "weights: [blocks, Hkv, block]"
+    device = weights.device
+    blocks, hkv, block = weights.shape
+    _check_per_place(device, (blocks, hkv, block), weights=weights, positions=positions)
+    B = seq_lens.shape[0]
+    _check_ints(device, seq_lens=seq_lens, seen=seen)
+    assert seq_lens.shape == seen.shape == (B,)
+    _check_table(block_table, device, B)
+    assert budget >= 1 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, \
+        f"a budget of {budget} tokens holds at least the {keep_first} first and {keep_last} last ones"
+    if not weights.is_cuda:
+        return kv4_keep_ref(weights, positions, block_table, seq_lens, seen, budget, keep_first, keep_last)
+    keep = torch.empty(B, hkv, budget, dtype=torch.int32, device=device)
+    lens = torch.empty(B, dtype=torch.int32, device=device)
+    if B:
+        scratch = torch.empty_like(keep)
+        _call("omni_kv4_keep", device, _p(weights), _p(positions), blocks, block, hkv, _p(block_table), block_table.stride(0), block_table.shape[1],
+              _p(seq_lens), _p(seen), B, budget, keep_first, keep_last, _p(keep), _p(lens), _p(scratch))
+    return keep, lens
+
+
+def kv4_move(k_cache, v_cache, block_table, keep, weights=None, positions=None):
+    """Brings the tokens that ``keep`` [B, Hkv, budget] names (see ``kv4_keep``) to their places, in place, with their weights and
+    positions where given.  What other places hold is left.  Requests that share a block would lose tokens of one another: copy
+    such blocks first."""
+    blocks, hkv, block, d = _check_caches(k_cache, v_cache)
+    device = k_cache.device
+    assert keep.dim() == 3 and keep.shape[1] == hkv and keep.is_contiguous() and keep.dtype == torch.int32 and keep.device == device, \
+        f"keep: contiguous int32 [B, {hkv}, budget] on {device}"
+    B, _, budget = keep.shape
+    _check_table(block_table, device, B)
+    _check_per_place(device, (blocks, hkv, block), weights=weights, positions=positions)
+    if not k_cache.is_cuda:
+        _move_ref(k_cache, v_cache, block_table, keep, weights, positions)
+    elif B and budget:
+        _call("omni_kv4_move", device, _p(k_cache), _p(v_cache), blocks, block, hkv, d, _p(block_table), block_table.stride(0), block_table.shape[1],
+              _p(keep), B, budget, _p(weights), _p(positions))

@@ -1,0 +1,49 @@
+"""The 4-bit cache's formulas in 64 bits: what stored rows are worth, attention over them with its error bound, eviction."""
+import torch
+
+
+def stored(x):
+    """What bf16 rows x [..., d] are worth once stored: per 64 columns code * step + lowest, the step a bf16 number not below
+    (max - min) / 15."""
+    v = x.double().cpu().unflatten(-1, (-1, 64))
+    lo, hi = v.amin(-1, keepdim=True), v.amax(-1, keepdim=True)
+    rng = hi - lo
+    rng = torch.where(rng.float().isfinite(), rng, torch.full_like(rng, float("nan")))
+    step = rng / 15
+    e = torch.floor(torch.log2(step.clamp_min(1e-300))).clamp_min(-126)
+    unit = torch.exp2(e - 7)
+    step = torch.ceil(step / unit) * unit
+    code = torch.where(step > 0, torch.round((v - lo) / torch.where(step > 0, step, torch.ones_like(step))).clamp(0, 15), torch.zeros_like(v))
+    return (code * step + lo).flatten(-2), step.squeeze(-1), lo.squeeze(-1)
+
+
+def attention(q, k, v, scale, k_step, k_low):
+    """q [r, d], k, v [n, d] (64 bits) -> out, weights, and the bound of the error of each in fp32 arithmetic.
+
+    Scores.  A kernel may sum q (16 + code) step and q (lowest - 16 step) apart, so an fp32 sum of d products has an error of at
+    most (d + 16) 2^-24 sum_i |q_i| (32 step_i + |low_i| + 16 step_i) scale =: e.  A weight p = exp(s) / sum exp is then off by
+    a factor of at most exp(2 e), and by 2^-20 more for its own exponentials (2^-22 each) and sums.
+    Values.  Weights times steps may be carried in two bf16 parts (2^-16 of the value each), times codes plus 16 (up to 31) against
+    a value that is known up to half a step: at most 2^-16 * 31 * step sum p =: c on top, and the rounding of the result."""
+    s = q.double() @ k.T * scale
+    p = torch.softmax(s, -1)
+    d = q.shape[-1]
+    mag = (48 * k_step + k_low.abs()).repeat_interleave(64, -1)
+    e = ((d + 16) * 2.0 ** -24 * abs(scale) * (q.double().abs() @ mag.T)).amax(-1, keepdim=True)
+    rel = torch.expm1(2 * e) + 2.0 ** -20
+    return p @ v, p, rel, p @ v.abs()
+
+
+def keep(weights, positions, n, seen, budget, first, last):
+    """One request and head: lists of n weights and positions -> the place whose token each place below min(n, budget) holds."""
+    if n <= budget:
+        return list(range(n))
+
+    def rank(j):
+        if positions[j] < first or positions[j] >= seen - last:
+            return (0, 0.0, j)
+        return (1, 0.0, j) if weights[j] != weights[j] else (2, -weights[j], j)
+    stay = sorted(sorted(range(n), key=rank)[:budget])
+    inside = set(j for j in stay if j < budget)
+    outside = [j for j in stay if j >= budget]
+    return [j if j in inside else outside.pop(0) for j in range(budget)]
