@@ -3,6 +3,23 @@
 //   q    [B rows, Hq, d] bf16: the last `rows` tokens of every request; row i of a request of L cached tokens sees L - rows + 1 + i
 //   out  [B rows, Hq, d] bf16 = sum_t p_t v_t,  p = softmax_t(scale q k_t),  k_t and v_t = code * step + lowest
 //   weights[t] = decay * weights[t] + sum over the rows and the query heads of a key/value head of p_t
+//
+// Codes go to the tensor cores as they are.  The bits of a code placed at the top of the mantissa of 1.0 make the bf16 number
+// 1 + code / 16, one shift and one and-or for two codes, exactly; then
+//   q k_t = sum over groups  16 step (sum q (1 + code / 16)) + (lowest - 16 step) (sum q)
+//   out   = sum over groups  sum_t (16 step p_t) (1 + code / 16)  +  sum_t p_t (lowest - 16 step)
+// so keys and values are never rounded, the steps multiply fp32 scores and fp32 weights, and the terms without codes are a few
+// fp32 multiply-adds a token.  The weights of the second product, 16 step p_t, are carried as two bf16 numbers (16 bits of mantissa):
+// with one the rounding of the weights would be as large as that of the result.
+//
+// A row of keys takes 72 bytes at d = 128 and a tile of 16 tokens serves 8 query rows per product, so the op is bound by memory as
+// long as unpacking keeps up: 7 integer operations for 8 key codes, 17 for 16 value codes.
+//
+// The query rows of a key/value head (rows x heads of its group, in tiles of 8) are the columns of the products (mma.sync
+// m16n8k16), tokens and then columns of the head their rows: S = K Q^T, O^T = V^T P^T.  P^T wants tokens along its rows, which is what
+// movmatrix makes of S.  Each warp walks tiles of 64 tokens (32 at d = 256) by itself: one lane group starts bulk copies of the tile's
+// codes and scales, two tiles ahead, an mbarrier a stage says when they are there.  No block-wide wait stands in the loop.  The warps'
+// results meet in shared memory at the end, those of the parts of a long request in a second kernel.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -10,10 +27,12 @@
 
 #include "../include/kv4.cuh"
 #include "../include/omni_ptx.cuh"
+#include "../include/score_mod.cuh"
 
 namespace omni {
 
-constexpr int KV4_SITE_DECODE = 84;
+constexpr int KV4_SITE_DECODE = 84, KV4_SITE_TILE = 85, KV4_SITE_WEIGHTS = 86;
+constexpr int KV4_WARPS = 4, KV4_STAGES = 2;
 
 struct Kv4Decode {
   const __nv_bfloat16* q;
@@ -26,6 +45,10 @@ struct Kv4Decode {
   float* lse;                       // [B, Hq, rows] in units of log 2, or null
   float* weights;
   float decay;
+  int piece;                        // tokens of a copy: the largest of 64, 32, 16 that divides the block
+  int splits, min_tiles;            // parts of a request, and the fewest tiles of one
+  float* o_part;                    // [B, Hkv, chunks, splits, 8 NT, d]
+  float* lse_part;                  // [B, Hkv, chunks, splits, 8 NT]
 };
 
 __device__ __forceinline__ int kv4_length(const Kv4Decode& a, int block, int b, OmniStatus* st) {
@@ -34,111 +57,643 @@ __device__ __forceinline__ int kv4_length(const Kv4Decode& a, int block, int b, 
   if (threadIdx.x == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, b);
   return a.table_w * block;
 }
+// tiles of a part of `tiles`
+__device__ __forceinline__ int kv4_part(const Kv4Decode& a, int tiles) { return max(a.min_tiles, (tiles + a.splits - 1) / a.splits); }
 
-// q k of one token, or -inf for one in no valid block
-__device__ __forceinline__ float kv4_score(const Kv4Decode& a, const Kv4Cache& c, const float* q, int b, int h, int t, OmniStatus* st) {
-  const int blk = a.table[(long long)b * a.table_ld + t / c.block];
-  if (blk < 0 || blk >= c.blocks) {
-    report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, b);
-    return -INFINITY;
+// bf16 pair 1 + code / 16 of the codes at bits 4 I of both halves of w
+template <int I>
+__device__ __forceinline__ uint32_t kv4_ext(uint32_t w) {
+  const uint32_t s = I == 0 ? w << 3 : w >> (4 * I - 3);
+  return (s & 0x00780078u) | 0x3f803f80u;
+}
+__device__ __forceinline__ void kv4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t kv4_pack(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t kv4_rest(uint32_t packed, float lo, float hi) {
+  return kv4_pack(lo - __uint_as_float(packed << 16), hi - __uint_as_float(packed & 0xffff0000u));
+}
+__device__ __forceinline__ void kv4_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void kv4_lds(uint32_t (&w)[N], const uint8_t* p) {
+  if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+  if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
   }
-  const uint8_t* piece = c.k + c.at(blk, h);
-  float s = 0.f;
-  for (int u = 0; u < c.d / 8; ++u) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(piece + c.k_word(t % c.block, u));
-    const uint32_t p = *reinterpret_cast<const uint32_t*>(piece + c.scale_word(t % c.block, u >> 3));
-    for (int j = 0; j < 8; ++j) s = fmaf(q[u * 8 + j], fmaf((float)((w >> (4 * j)) & 15u), kv4_step(p), kv4_low(p)), s);
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   }
-  return s * a.scale_log2;
 }
 
-// One block for a query row: tiles of 128 tokens, a thread for each of them in the scores and for each column in the sums.
-__global__ void __launch_bounds__(128) kv4_decode_kernel(Kv4Decode a, Kv4Cache c, OmniStatus* st) {
-  const int b = blockIdx.z, row = blockIdx.y, hq = blockIdx.x, h = hq / (a.hq / c.hkv);
-  __shared__ float q[256], p[128], red[4];
-  const int sees = kv4_length(a, c.block, b, st) - a.rows + 1 + row;
-  const long long at = (long long)b * a.rows + row;
-  for (int i = threadIdx.x; i < c.d; i += 128) q[i] = __bfloat162float(a.q[at * a.q_row + (long long)hq * a.q_head + i]);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-  for (int t0 = 0; t0 < sees; t0 += 128) {
-    const int t = t0 + threadIdx.x;
-    const float s = t < sees ? kv4_score(a, c, q, b, h, t, st) : -INFINITY;
-    float top = warp_max(s);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float f = top == -INFINITY ? 1.f : exp2f(m - top), w = s == -INFINITY ? 0.f : exp2f(s - top);
-    m = top;
-    p[threadIdx.x] = w;
-    const float part = warp_sum(w);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = part;
-    __syncthreads();
-    l = l * f + red[0] + red[1] + red[2] + red[3];
-    for (int e = 0; e < 2; ++e) {
-      const int d = threadIdx.x + 128 * e;
-      if (d >= c.d) break;
-      o[e] *= f;
-      for (int i = 0; i < 128 && t0 + i < sees; ++i) {
-        const int blk = a.table[(long long)b * a.table_ld + (t0 + i) / c.block];
-        if (blk < 0 || blk >= c.blocks) continue;
-        const uint8_t* piece = c.v + c.at(blk, h);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(piece + c.v_word((t0 + i) % c.block, d >> 3));
-        const uint32_t g = *reinterpret_cast<const uint32_t*>(piece + c.scale_word((t0 + i) % c.block, d >> 6));
-        o[e] = fmaf(p[i], fmaf((float)((w >> (4 * (d & 7))) & 15u), kv4_step(g), kv4_low(g)), o[e]);
+template <int NG, bool VALUES>
+struct Kv4Tile {
+  static constexpr int PER = NG > 1 ? 2 : 1, PLANES = NG / PER;
+  static constexpr int TOKENS = NG == 4 ? 32 : 64, SUBS = TOKENS / 16;
+  static constexpr int CODES = TOKENS * 32 * NG, SCALES = TOKENS * 4 * NG;
+  static constexpr int V0 = CODES, KS0 = VALUES ? 2 * CODES : CODES, VS0 = KS0 + SCALES;
+  static constexpr int BYTES = VALUES ? 2 * (CODES + SCALES) : CODES + SCALES;
+  static constexpr int TOKEN_BYTES = BYTES / TOKENS;
+  static constexpr int KINDS = VALUES ? 2 * PLANES + 2 : PLANES + 1;      // copies of a run of tokens
+
+  // The block of the run of tokens that this lane copies of `tile`
+  static __device__ __forceinline__ int page(const Kv4Decode& a, const Kv4Cache& c, int b, int tile, int end, OmniStatus* st) {
+    const int t = tile * TOKENS + (int)(threadIdx.x & 31) / KINDS * a.piece;
+    if ((int)(threadIdx.x & 31) / KINDS * a.piece >= TOKENS || t >= end) return -1;
+    const int blk = a.table[(long long)b * a.table_ld + t / c.block];
+    if (blk >= 0 && blk < c.blocks) return blk;
+    report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, b);
+    return 0;                       // in bounds; the result is reported as wrong
+  }
+  // Start the copies of `tile`: whole 16 tokens below `end`
+  static __device__ __forceinline__ void start(const Kv4Decode& a, const Kv4Cache& c, int h, int tile, int end, int blk, uint8_t* stage, uint64_t* bar) {
+    const int lane = threadIdx.x & 31, kind = lane % KINDS, off = lane / KINDS * a.piece;
+    const int count = min(TOKENS, (end - tile * TOKENS + 15) & ~15);
+    if (lane == 0) mbar_expect_tx(bar, count * TOKEN_BYTES);
+    __syncwarp();
+    if (blk < 0) return;
+    const int n = min(a.piece, count - off), t = (tile * TOKENS + off) % c.block;
+    const bool values = VALUES && (kind >= PLANES && kind < 2 * PLANES || kind == 2 * PLANES + 1);
+    const bool scales = kind >= (VALUES ? 2 : 1) * PLANES;
+    const uint8_t* src = (values ? c.v : c.k) + c.at(blk, h);
+    uint32_t dst = smem_u32(stage);
+    if (scales) {
+      src += c.block * (32 * NG) + t * (4 * NG);
+      dst += (values ? VS0 : KS0) + off * (4 * NG);
+    } else {
+      const int plane = values ? kind - PLANES : kind;
+      src += (plane * c.block + t) * (32 * PER);
+      dst += (values ? V0 : 0) + (plane * TOKENS + off) * (32 * PER);
+    }
+    kv4_bulk(dst, src, n * (scales ? 4 * NG : 32 * PER), bar);
+  }
+};
+
+// Fragments of 8 query rows (row r: query token r / rep, head h rep + r % rep) and the sums of their groups for the rows 2 c, 2 c + 1
+template <int NG>
+struct Kv4Query {
+  uint32_t b[NG][4][2];
+  __device__ __forceinline__ void load(const Kv4Decode& a, int rep, int b0, int h, int r, int total) {
+    const int c = threadIdx.x & 3;
+    const __nv_bfloat16* q = a.q + ((long long)b0 * a.rows + r / rep) * a.q_row + (long long)(h * rep + r % rep) * a.q_head + c * 16;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = g * 64 + (s >> 1) * 8 + (s & 1) * 2 + e;
+          uint32_t v = 0u;
+          if (r < total) v = (uint32_t)__bfloat16_as_ushort(q[at]) | (uint32_t)__bfloat16_as_ushort(q[at + 4]) << 16;
+          b[g][s][e] = v;
+        }
+  }
+  __device__ __forceinline__ void sums(float (&qs)[NG][2]) const {
+    const int c = threadIdx.x & 3;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float x = 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) x += __uint_as_float(b[g][s][e] << 16) + __uint_as_float(b[g][s][e] & 0xffff0000u);
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      qs[g][0] = __shfl_sync(0xffffffffu, x, c * 8);
+      qs[g][1] = __shfl_sync(0xffffffffu, x, c * 8 + 4);
+    }
+  }
+};
+
+// Scores, in units of log 2, of 16 tokens of a staged tile and 8 query rows per tile of NT: tokens r and r + 8, rows 2 c and 2 c + 1
+template <int NG, int NT, bool VALUES>
+__device__ __forceinline__ void kv4_scores(const uint8_t* stage, int sub, float scale_log2, const Kv4Query<NG> (&q)[NT], const float (&qs)[NT][NG][2],
+                                           float (&s)[NT][4]) {
+  using T = Kv4Tile<NG, VALUES>;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  uint32_t sc[2][NG];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) kv4_lds<NG>(sc[e], stage + T::KS0 + (sub * 16 + r + 8 * e) * (4 * NG));
+#pragma unroll
+  for (int n = 0; n < NT; ++n) { s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f; }
+#pragma unroll
+  for (int p = 0; p < T::PLANES; ++p) {
+    uint32_t w[2][2 * T::PER];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) kv4_lds<2 * T::PER>(w[e], stage + (p * T::TOKENS + sub * 16 + r + 8 * e) * (32 * T::PER) + c * (8 * T::PER));
+#pragma unroll
+    for (int gp = 0; gp < T::PER; ++gp) {
+      const int g = p * T::PER + gp;
+      float acc[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) { acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f; }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t w0 = w[0][gp * 2 + x], w1 = w[1][gp * 2 + x];
+        const uint32_t a0 = kv4_ext<0>(w0), a1 = kv4_ext<0>(w1), a2 = kv4_ext<1>(w0), a3 = kv4_ext<1>(w1);
+        const uint32_t a4 = kv4_ext<2>(w0), a5 = kv4_ext<2>(w1), a6 = kv4_ext<3>(w0), a7 = kv4_ext<3>(w1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          kv4_mma(acc[n], a0, a1, a2, a3, q[n].b[g][2 * x][0], q[n].b[g][2 * x][1]);
+          kv4_mma(acc[n], a4, a5, a6, a7, q[n].b[g][2 * x + 1][0], q[n].b[g][2 * x + 1][1]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float up = kv4_step(sc[e][g]) * (16.f * scale_log2), low = fmaf(kv4_low(sc[e][g]), scale_log2, -up);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) s[n][2 * e + x] = fmaf(up, acc[n][2 * e + x], fmaf(low, qs[n][g][x], s[n][2 * e + x]));
       }
     }
-    __syncthreads();
   }
-  for (int e = 0; e < 2; ++e) {
-    const int d = threadIdx.x + 128 * e;
-    if (d < c.d) a.out[(at * a.hq + hq) * c.d + d] = __float2bfloat16(l == 0.f ? 0.f : o[e] / l);
-  }
-  if (a.lse != nullptr && threadIdx.x == 0) a.lse[((long long)b * a.hq + hq) * a.rows + row] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
-// A thread for a token and head: its scores once more, against the finished softmax denominators.
-__global__ void __launch_bounds__(128) kv4_weights_kernel(Kv4Decode a, Kv4Cache c, OmniStatus* st) {
-  const int b = blockIdx.z, h = blockIdx.y, rep = a.hq / c.hkv;
-  __shared__ float q[256];
-  const int n = kv4_length(a, c.block, b, st), tiles = (n + 127) / 128;
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int t = tile * 128 + threadIdx.x;
-    float sum = 0.f;
-    for (int r = 0; r < a.rows * rep; ++r) {
-      const int row = r / rep, hq = h * rep + r % rep;
-      const long long at = (long long)b * a.rows + row;
-      __syncthreads();
-      for (int i = threadIdx.x; i < c.d; i += 128) q[i] = __bfloat162float(a.q[at * a.q_row + (long long)hq * a.q_head + i]);
-      __syncthreads();
-      if (t < n - a.rows + 1 + row) sum += exp2f(kv4_score(a, c, q, b, h, t, st) - a.lse[((long long)b * a.hq + hq) * a.rows + row]);
-    }
-    if (t >= n) continue;
-    const int blk = a.table[(long long)b * a.table_ld + t / c.block];
-    if (blk < 0 || blk >= c.blocks) continue;
-    float* w = a.weights + ((long long)blk * c.hkv + h) * c.block + t % c.block;
-    *w = a.decay == 0.f ? sum : fmaf(a.decay, *w, sum);
+template <int NG, int NT>
+__global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decode_kernel(Kv4Decode a, Kv4Cache c, OmniStatus* st) {
+  using T = Kv4Tile<NG, true>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[KV4_WARPS * KV4_STAGES];
+  __shared__ int abort_flag;
+  constexpr int D = NG * 64, NQ = 8 * NT;
+  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ;
+  const int h = blockIdx.x / chunks, chunk = blockIdx.x - h * chunks, split = blockIdx.y, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
+  const int row0 = chunk * NQ;
+  const int len = kv4_length(a, c.block, b, st);
+  const int first_sees = len - a.rows + 1 + row0 / rep;                    // of the chunk's first and last rows
+  const int end = len - a.rows + 1 + (min(total, row0 + NQ) - 1) / rep;
+  const int tiles = end > 0 ? (end + T::TOKENS - 1) / T::TOKENS : 0;
+  const int part = kv4_part(a, tiles), begin_tile = split * part, end_tile = min(tiles, begin_tile + part);
+  if (begin_tile >= end_tile && split > 0) return;                         // the first part writes the zeros of rows that see nothing
+
+  uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
+  uint64_t* bar = bars + warp * KV4_STAGES;
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane == 0) {
+    for (int s = 0; s < KV4_STAGES; ++s) mbar_init(bar + s, 1);
+    mbar_fence_init();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  __syncthreads();
+  int tile = begin_tile + warp, next = tile, blk = T::page(a, c, b, next, next < end_tile ? end : 0, st);
+#pragma unroll
+  for (int s = 0; s < KV4_STAGES; ++s) {
+    if (next < end_tile) T::start(a, c, h, next, end, blk, stages + s * T::BYTES, bar + s);
+    next += KV4_WARPS;
+    blk = T::page(a, c, b, next, next < end_tile ? end : 0, st);
+  }
+
+  Kv4Query<NG> q[NT];
+  float qs[NT][NG][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    q[n].load(a, rep, b, h, row0 + n * 8 + r, total);
+    q[n].sums(qs[n]);
+  }
+  float m[NT][2], l[NT][2], o[NT][NG][4][4], z[NT][NG][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      m[n][x] = -INFINITY;
+      l[n][x] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        z[n][g][x] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][g][j][x] = o[n][g][j][x + 2] = 0.f;
+      }
+    }
+
+  int it = 0;
+  for (; tile < end_tile; tile += KV4_WARPS, ++it) {
+    const int st_i = it % KV4_STAGES;
+    uint8_t* stage = stages + st_i * T::BYTES;
+    if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (it / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_TILE, tile))) break;
+    const int t0 = tile * T::TOKENS;
+    const bool edge = t0 + T::TOKENS > first_sees;                         // some row does not see all of the tile
+    float s[T::SUBS][NT][4], top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < T::SUBS; ++u) {
+      kv4_scores<NG, NT, true>(stage, u, a.scale_log2, q, qs, s[u]);
+      if (edge) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int sees = len - a.rows + 1 + min(row0 + n * 8 + cc * 2 + x, total - 1) / rep;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (t0 + u * 16 + r + 8 * e >= sees) s[u][n][2 * e + x] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) top[n][x] = fmaxf(top[n][x], fmaxf(s[u][n][x], s[u][n][2 + x]));
+    }
+    // The maximum is followed only when a score exceeds it by 2^8, which weights in fp32 and bf16 bear easily.
+    bool more = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) more |= top[n][0] > m[n][0] + 8.f || top[n][1] > m[n][1] + 8.f;
+    if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float v = top[n][x];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+          v = fmaxf(v, m[n][x]);
+          const float f = v == -INFINITY ? 1.f : ex2_fast(m[n][x] - v);
+          m[n][x] = v;
+          l[n][x] *= f;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            z[n][g][x] *= f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[n][g][j][x] *= f;
+              o[n][g][j][x + 2] *= f;
+            }
+          }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < T::SUBS; ++u) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float sub = m[n][x] == -INFINITY ? 0.f : m[n][x];
+          s[u][n][x] = ex2_fast(s[u][n][x] - sub);
+          s[u][n][2 + x] = ex2_fast(s[u][n][2 + x] - sub);
+          l[n][x] += s[u][n][x] + s[u][n][2 + x];
+        }
+      uint32_t sc[2][NG];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        kv4_lds<NG>(sc[e], stage + T::VS0 + (u * 16 + r + 8 * e) * (4 * NG));
+        if (edge && t0 + u * 16 + r + 8 * e >= end) {                      // what lies there is not of this request
+#pragma unroll
+          for (int g = 0; g < NG; ++g) sc[e][g] = 0u;
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < T::PLANES; ++p) {
+        uint32_t w[2][2 * T::PER];                                         // pairs of tokens c and c + 4: even (groups), odd (groups)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int pair = u * 8 + cc + 4 * e;
+          const int ch = T::PER == 2 ? r ^ ((pair & 3) << 1) : r ^ (((pair >> 1) & 1) << 2);
+          kv4_lds<2 * T::PER>(w[e], stage + T::V0 + (p * T::TOKENS + pair * 2) * (32 * T::PER) + ch * (8 * T::PER));
+        }
+#pragma unroll
+        for (int gp = 0; gp < T::PER; ++gp) {
+          const int g = p * T::PER + gp;
+          uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float up = kv4_step(sc[e][g]) * 16.f, low = kv4_low(sc[e][g]) - up;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float p0 = s[u][n][2 * e], p1 = s[u][n][2 * e + 1];
+              float f0 = p0 * up, f1 = p1 * up, z0 = p0 * low, z1 = p1 * low;
+              if (edge) {                                                  // an unseen token adds nothing, whatever its value
+                if (p0 == 0.f) f0 = z0 = 0.f;
+                if (p1 == 0.f) f1 = z1 = 0.f;
+              }
+              z[n][g][0] += z0;
+              z[n][g][1] += z1;
+              hi[n][e] = kv4_pack(f0, f1);
+              lo[n][e] = kv4_transpose(kv4_rest(hi[n][e], f0, f1));
+              hi[n][e] = kv4_transpose(hi[n][e]);
+            }
+          }
+          const uint32_t x0 = __byte_perm(w[0][gp], w[0][T::PER + gp], 0x5410), y0 = __byte_perm(w[0][gp], w[0][T::PER + gp], 0x7632);
+          const uint32_t x1 = __byte_perm(w[1][gp], w[1][T::PER + gp], 0x5410), y1 = __byte_perm(w[1][gp], w[1][T::PER + gp], 0x7632);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t v0 = j < 2 ? x0 : y0, v1 = j < 2 ? x1 : y1;
+            const uint32_t a0 = j & 1 ? kv4_ext<2>(v0) : kv4_ext<0>(v0), a1 = j & 1 ? kv4_ext<3>(v0) : kv4_ext<1>(v0);
+            const uint32_t a2 = j & 1 ? kv4_ext<2>(v1) : kv4_ext<0>(v1), a3 = j & 1 ? kv4_ext<3>(v1) : kv4_ext<1>(v1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              kv4_mma(o[n][g][j], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+              kv4_mma(o[n][g][j], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();                                                          // every lane has read the stage
+    if (next < end_tile) T::start(a, c, h, next, end, blk, stage, bar + st_i);
+    next += KV4_WARPS;
+    blk = T::page(a, c, b, next, next < end_tile ? end : 0, st);
+  }
+
+  // ---- the sums over the lanes that share a query row, then over the warps
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], d);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) z[n][g][x] += __shfl_xor_sync(0xffffffffu, z[n][g][x], d);
+      }
+  __syncthreads();
+  if (abort_flag != 0) {                                                   // copies may still be under way: leave the memory alone
+    if (threadIdx.x == 0) report_abort(&abort_flag, st);
+    for (int s = 0; s < KV4_STAGES; ++s) {
+      const int left = it + s;                                             // what this warp has started and not seen: its phases
+      if (tile + s * KV4_WARPS < end_tile) {
+        for (int i = 0; i < 1 << 16 && !mbar_try_wait(bar + left % KV4_STAGES, (left / KV4_STAGES) & 1); ++i) {}
+      }
+    }
+    return;
+  }
+  float* s_o = reinterpret_cast<float*>(smem);                             // [warps][NQ][D]
+  float* s_m = s_o + KV4_WARPS * NQ * D;                                   // [warps][NQ], and the sums likewise
+  float* s_l = s_m + KV4_WARPS * NQ;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int i = warp * NQ + n * 8 + cc * 2 + x;
+      if (r == 0) {
+        s_m[i] = m[n][x];
+        s_l[i] = l[n][x];
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float2*>(s_o + (size_t)i * D + g * 64 + r * 8 + j * 2) = make_float2(o[n][g][j][x] + z[n][g][x], o[n][g][j][x + 2] + z[n][g][x]);
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < NQ * D; i += KV4_WARPS * 32) {
+    const int row = i / D, d = i - row * D;
+    if (row0 + row >= total) break;
+    float mm = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < KV4_WARPS; ++w) mm = fmaxf(mm, s_m[w * NQ + row]);
+#pragma unroll
+    for (int w = 0; w < KV4_WARPS; ++w) {
+      const float mw = s_m[w * NQ + row];
+      const float f = mw == -INFINITY ? (s_l[w * NQ + row] == 0.f ? 0.f : 1.f) : ex2_fast(mw - mm);      // a sum without a maximum is NaN
+      sum += s_l[w * NQ + row] * f;
+      acc += s_o[((size_t)w * NQ + row) * D + d] * f;
+    }
+    const float value = sum == 0.f ? 0.f : acc / sum, lse = sum == 0.f ? -INFINITY : mm + __log2f(sum);
+    const int head = h * rep + (row0 + row) % rep, tok = (row0 + row) / rep;
+    if (a.splits == 1) {
+      a.out[(((long long)b * a.rows + tok) * a.hq + head) * D + d] = __float2bfloat16(value);
+      if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = lse;
+    } else {
+      const long long at = (((long long)b * gridDim.x + blockIdx.x) * a.splits + split) * NQ + row;
+      a.o_part[at * D + d] = value;
+      if (d == 0) a.lse_part[at] = lse;
+    }
+  }
+}
+
+// The parts of a request, one block for a query row and head.
+template <int NT>
+__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, int tokens) {
+  constexpr int NQ = 8 * NT;
+  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ;
+  const int h = blockIdx.x / total, row = blockIdx.x - h * total, b = blockIdx.y, d = threadIdx.x;
+  const int chunk = row / NQ, len = min(max(a.seq_lens[b], 0), a.table_w * c.block);
+  const int end = len - a.rows + 1 + (min(total, chunk * NQ + NQ) - 1) / rep;
+  const int tiles = end > 0 ? (end + tokens - 1) / tokens : 0, part = kv4_part(a, tiles);
+  const int parts = max(1, (tiles + part - 1) / part);
+  const long long at = ((long long)b * c.hkv * chunks + h * chunks + chunk) * a.splits * NQ + row - chunk * NQ;
+  float mm = -INFINITY, sum = 0.f, acc = 0.f;
+  for (int s = 0; s < parts; ++s) mm = fmaxf(mm, a.lse_part[at + s * NQ]);
+  for (int s = 0; s < parts; ++s) {
+    const float v = a.lse_part[at + s * NQ];
+    const float f = v == -INFINITY ? 0.f : exp2f(v - mm);
+    sum += f;
+    acc += f == 0.f ? 0.f : f * a.o_part[(at + s * NQ) * c.d + d];
+  }
+  const int head = h * rep + row % rep, tok = row / rep;
+  a.out[(((long long)b * a.rows + tok) * a.hq + head) * c.d + d] = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
+  if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = sum == 0.f ? -INFINITY : mm + __log2f(sum);
+}
+
+// The weights that the rows give a request's tokens: the scores of the staged keys once more, against the finished sums.  Reading the
+// keys twice costs as much as keeping the scores of 8 query rows would, and nothing more for more rows.
+template <int NG>
+__global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decode a, Kv4Cache c, OmniStatus* st) {
+  using T = Kv4Tile<NG, false>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[KV4_WARPS * KV4_STAGES];
+  __shared__ int abort_flag;
+  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + 7) / 8;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
+  const int len = kv4_length(a, c.block, b, st), tiles = (len + T::TOKENS - 1) / T::TOKENS;
+  const int step = gridDim.x * KV4_WARPS;
+  if (blockIdx.x * KV4_WARPS >= tiles) return;
+  uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
+  uint2* s_q = reinterpret_cast<uint2*>(smem + KV4_WARPS * KV4_STAGES * T::BYTES);      // [chunks][NG * 4][32]
+  float* s_qs = reinterpret_cast<float*>(s_q + chunks * NG * 4 * 32);                    // [chunks][NG][8]
+  float* s_lse = s_qs + chunks * NG * 8;                                                 // [chunks][8]
+  uint64_t* bar = bars + warp * KV4_STAGES;
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane == 0) {
+    for (int s = 0; s < KV4_STAGES; ++s) mbar_init(bar + s, 1);
+    mbar_fence_init();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  int tile = blockIdx.x * KV4_WARPS + warp, next = tile, blk = T::page(a, c, b, next, next < tiles ? len : 0, st);
+#pragma unroll
+  for (int s = 0; s < KV4_STAGES; ++s) {
+    if (next < tiles) T::start(a, c, h, next, len, blk, stages + s * T::BYTES, bar + s);
+    next += step;
+    blk = T::page(a, c, b, next, next < tiles ? len : 0, st);
+  }
+  for (int ch = warp; ch < chunks; ch += KV4_WARPS) {
+    Kv4Query<NG> q;
+    float qs[NG][2];
+    q.load(a, rep, b, h, ch * 8 + r, total);
+    q.sums(qs);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) s_q[(ch * NG * 4 + g * 4 + s) * 32 + lane] = make_uint2(q.b[g][s][0], q.b[g][s][1]);
+      if (r == 0) {
+        s_qs[(ch * NG + g) * 8 + cc * 2] = qs[g][0];
+        s_qs[(ch * NG + g) * 8 + cc * 2 + 1] = qs[g][1];
+      }
+    }
+    if (lane < 8) {
+      const int row = ch * 8 + lane;
+      s_lse[row] = row < total ? a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep] : INFINITY;
+    }
+  }
+  __syncthreads();
+  int it = 0;
+  for (; tile < tiles; tile += step, ++it) {
+    const int st_i = it % KV4_STAGES;
+    uint8_t* stage = stages + st_i * T::BYTES;
+    if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (it / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_WEIGHTS, tile))) break;
+    const int t0 = tile * T::TOKENS;
+    const bool edge = t0 + T::TOKENS > len - a.rows + 1;
+    float w[T::SUBS][2];
+#pragma unroll
+    for (int u = 0; u < T::SUBS; ++u) w[u][0] = w[u][1] = 0.f;
+    for (int ch = 0; ch < chunks; ++ch) {
+      Kv4Query<NG> q[1];
+      float qs[1][NG][2];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const uint2 v = s_q[(ch * NG * 4 + g * 4 + s) * 32 + lane];
+          q[0].b[g][s][0] = v.x;
+          q[0].b[g][s][1] = v.y;
+        }
+        qs[0][g][0] = s_qs[(ch * NG + g) * 8 + cc * 2];
+        qs[0][g][1] = s_qs[(ch * NG + g) * 8 + cc * 2 + 1];
+      }
+      const float lse[2] = {s_lse[ch * 8 + cc * 2], s_lse[ch * 8 + cc * 2 + 1]};
+#pragma unroll
+      for (int u = 0; u < T::SUBS; ++u) {
+        float s[1][4];
+        kv4_scores<NG, 1, false>(stage, u, a.scale_log2, q, qs, s);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int row = ch * 8 + cc * 2 + x, sees = row < total ? len - a.rows + 1 + row / rep : 0;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float p = ex2_fast(s[0][2 * e + x] - lse[x]);
+            if (!edge || t0 + u * 16 + r + 8 * e < sees) w[u][e] += row < total ? p : 0.f;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < T::SUBS; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w[u][e] += __shfl_xor_sync(0xffffffffu, w[u][e], 1);
+        w[u][e] += __shfl_xor_sync(0xffffffffu, w[u][e], 2);
+        const int t = t0 + u * 16 + r + 8 * e;
+        if (cc == 0 && t < len) {
+          const int at = a.table[(long long)b * a.table_ld + t / c.block];
+          if (at >= 0 && at < c.blocks) {
+            float* to = a.weights + ((long long)at * c.hkv + h) * c.block + t % c.block;
+            *to = a.decay == 0.f ? w[u][e] : fmaf(a.decay, *to, w[u][e]);
+          }
+        }
+      }
+    __syncwarp();
+    if (next < tiles) T::start(a, c, h, next, len, blk, stage, bar + st_i);
+    next += step;
+    blk = T::page(a, c, b, next, next < tiles ? len : 0, st);
+  }
+  __syncthreads();
+  if (abort_flag != 0) {
+    if (threadIdx.x == 0) report_abort(&abort_flag, st);
+    for (int s = 0; s < KV4_STAGES; ++s) {
+      const int left = it + s;
+      if (tile + s * step < tiles) {
+        for (int i = 0; i < 1 << 16 && !mbar_try_wait(bar + left % KV4_STAGES, (left / KV4_STAGES) & 1); ++i) {}
+      }
+    }
+  }
+}
+
+// Shared memory beyond 48 KB is asked for once a device and kernel; `most` remembers how much.
+static cudaError_t kv4_smem(const void* kernel, int bytes, int (&most)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && most[dev] >= bytes)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) most[dev] = bytes;
+  return e;
+}
+
+template <int NG, int NT>
+static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, OmniStatus* st, cudaStream_t stream) {
+  using T = Kv4Tile<NG, true>;
+  constexpr int merge = KV4_WARPS * 8 * NT * (NG * 64 + 2) * 4, stages = KV4_WARPS * KV4_STAGES * T::BYTES, bytes = merge > stages ? merge : stages;
+  const int total = a.rows * (a.hq / c.hkv), chunks = (total + 8 * NT - 1) / (8 * NT);
+  static int most[64] = {0};
+  cudaError_t e = kv4_smem((const void*)kv4_decode_kernel<NG, NT>, bytes, most);
+  if (e != cudaSuccess) return e;
+  kv4_decode_kernel<NG, NT><<<dim3(c.hkv * chunks, a.splits, B), KV4_WARPS * 32, bytes, stream>>>(a, c, st);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || a.splits == 1) return e;
+  kv4_join_kernel<NT><<<dim3(c.hkv * total, B), c.d, 0, stream>>>(a, c, T::TOKENS);
+  return cudaGetLastError();
+}
+
+template <int NG>
+static cudaError_t kv4_launch_weights(const Kv4Decode& a, const Kv4Cache& c, int B, int max_len, OmniStatus* st, cudaStream_t stream) {
+  using T = Kv4Tile<NG, false>;
+  const int total = a.rows * (a.hq / c.hkv), chunks = (total + 7) / 8;
+  const int bytes = KV4_WARPS * KV4_STAGES * T::BYTES + chunks * (NG * 4 * 32 * 8 + NG * 8 * 4 + 8 * 4);
+  static int most[64] = {0};
+  cudaError_t e = kv4_smem((const void*)kv4_weights_kernel<NG>, bytes, most);
+  if (e != cudaSuccess) return e;
+  const long long tiles = (max_len + T::TOKENS - 1) / T::TOKENS, items = (long long)B * c.hkv;
+  long long parts = (148 * 3 * 2 + items - 1) / items;
+  if (parts > (tiles + KV4_WARPS - 1) / KV4_WARPS) parts = (tiles + KV4_WARPS - 1) / KV4_WARPS;
+  if (parts < 1) parts = 1;
+  kv4_weights_kernel<NG><<<dim3((unsigned)parts, c.hkv, B), KV4_WARPS * 32, bytes, stream>>>(a, c, st);
+  return cudaGetLastError();
 }
 
 }  // namespace omni
 
 using namespace omni;
 
+// row_tile: query rows that share a pass over the cache, 8, or 16 for d <= 128.  o_part and lse_part are sized by it.
 extern "C" int omni_kv4_decode(const void* q, long long q_row, int q_head, const void* k_cache, const void* v_cache, long long blocks, int block,
                                int hkv, int d, const int* table, int table_ld, int table_w, const int* seq_lens, int B, int rows, int hq,
-                               float scale, int max_len, void* out, float* lse, float* weights, float decay, void* status, cudaStream_t stream) {
+                               float scale, int max_len, int row_tile, int splits, int min_tiles, float* o_part, float* lse_part, void* out, float* lse,
+                               float* weights, float decay, void* status, cudaStream_t stream) {
   const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
-  if (!kv4_shape_ok(c) || hq % hkv != 0 || rows < 1 || hkv > 65535 || B > 65535 || rows > 65535) return -1;
-  if (weights != nullptr && lse == nullptr) return -2;
+  if (!kv4_shape_ok(c) || hq % hkv != 0 || rows < 1 || hkv > 65535 || B > 65535 || splits < 1 || splits > 65535 || min_tiles < 1 ||
+      (row_tile != 8 && (row_tile != 16 || d > 128)))
+    return -1;
+  if (weights != nullptr && (lse == nullptr || rows * (hq / hkv) > 256)) return -2;
+  if (splits > 1 && (o_part == nullptr || lse_part == nullptr)) return -3;
   if (B <= 0) return 0;
-  const Kv4Decode a = {(const __nv_bfloat16*)q, q_row, q_head, table, seq_lens, table_ld, table_w, rows, hq,
-                       scale * 1.4426950408889634f, (__nv_bfloat16*)out, lse, weights, decay};
-  kv4_decode_kernel<<<dim3(hq, rows, B), 128, 0, stream>>>(a, c, (OmniStatus*)status);
-  cudaError_t e = cudaGetLastError();
+  const Kv4Decode a = {(const __nv_bfloat16*)q, q_row, q_head, table, seq_lens, table_ld, table_w, rows, hq, scale * 1.4426950408889634f,
+                       (__nv_bfloat16*)out, lse, weights, decay, block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16, splits, min_tiles, o_part, lse_part};
+  OmniStatus* st = (OmniStatus*)status;
+  const bool wide = row_tile == 16;
+  cudaError_t e = d == 64    ? wide ? kv4_launch<1, 2>(a, c, B, st, stream) : kv4_launch<1, 1>(a, c, B, st, stream)
+                  : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, st, stream) : kv4_launch<2, 1>(a, c, B, st, stream)
+                             : kv4_launch<4, 1>(a, c, B, st, stream);
   if (e != cudaSuccess || weights == nullptr) return (int)e;
-  const int tiles = (max_len + 127) / 128;
-  kv4_weights_kernel<<<dim3(tiles < 1 ? 1 : tiles, hkv, B), 128, 0, stream>>>(a, c, (OmniStatus*)status);
-  return (int)cudaGetLastError();
+  e = d == 64 ? kv4_launch_weights<1>(a, c, B, max_len, st, stream) : d == 128 ? kv4_launch_weights<2>(a, c, B, max_len, st, stream)
+                                                                              : kv4_launch_weights<4>(a, c, B, max_len, st, stream);
+  return (int)e;
 }

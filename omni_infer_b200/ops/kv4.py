@@ -11,8 +11,8 @@ every head, its own choice for each, in the places below the budget; ``positions
 ``weights`` how much attention it has had.  Keys carry their rotation with them, so attention does not ask for the order.
 
 Calls write to no memory but their outputs and what the allocator gives them for the call: they may run on several streams, and
-captured, as their arguments allow.  Block ids and slots outside the cache are skipped and reported by
-``ops._native.check_status``."""
+captured, as their arguments allow.  Block ids and slots outside the cache are reported by ``ops._native.check_status``: rows there
+are neither written nor read, and the attention of a request with such a block is not to be used."""
 from __future__ import annotations
 
 import contextlib
@@ -174,7 +174,7 @@ _ARGS = {
     "omni_kv4_read": (_P, _P, _L, _I, _I, _I, _P, _L, _P, _P, _P, _P),
     "omni_kv4_keep": (_P, _P, _L, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P),
     "omni_kv4_move": (_P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P),
-    "omni_kv4_decode": (_P, _L, _I, _P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _I, _I, _I, _F, _I, _P, _P, _P, _F, _P, _P),
+    "omni_kv4_decode": (_P, _L, _I, _P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _P, _P, _P, _F, _P, _P),
 }
 _bound = {}
 
@@ -275,6 +275,12 @@ def kv4_read(k_cache, v_cache, slots):
     return k, v
 
 
+def _parts(items, tiles, resident):
+    """(most parts that a request is cut into, fewest tiles of one) for ``items`` passes over up to ``tiles`` tiles each, with
+    ``resident`` blocks on each of the 148 SMs."""
+    return max(1, min(-(-2 * 148 * resident // items), -(-tiles // 4))), 4
+
+
 def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=None, weights=None, decay=1.0):
     """Attention of the last tokens of every request over its cached ones: q [B n, Hq, d] bf16 (any row and head pitch), the ``n``
     rows of a request one after the other; row i sees the first ``seq_lens[b] - n + 1 + i`` of the request's places (none: zeros).
@@ -282,7 +288,8 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
 
     ``weights`` [blocks, Hkv, block] fp32: of every place below seq_lens[b] becomes decay * weights + the softmax weights that the
     rows and the query heads of its key/value head give it (decay 0: whatever was there is dropped).  Requests that share a block
-    would write the same numbers: give ``weights`` only where blocks belong to one request.  ``max_seq_len`` (a bound of
+    would write the same numbers: give ``weights`` only where blocks belong to one request.  At most 256 rows times query
+    heads of a key/value head then.  ``max_seq_len`` (a bound of
     ``seq_lens``) shapes the launch; without it the width of the block table does."""
     blocks, hkv, block, d = _check_caches(k_cache, v_cache)
     assert q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == d and q.device == k_cache.device and q.stride(2) == 1, \
@@ -298,11 +305,19 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
         return kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights, decay)
     out = torch.empty(T, hq, d, dtype=q.dtype, device=q.device)
     if T:
-        width = block_table.shape[1]
+        width, total = block_table.shape[1], T // B * (hq // hkv)
+        assert weights is None or total <= 256, f"weights of at most 256 query rows a key/value head at once: {total}"
         longest = width * block if max_seq_len is None else min(max_seq_len, width * block)
+        tile = 16 if d <= 128 and total > 8 else 8
+        items = B * hkv * -(-total // tile)
+        splits, min_tiles = _parts(items, -(-longest // (32 if d == 256 else 64)), 3 if tile * d <= 1024 else 2)
         lse = torch.empty(T * hq, dtype=torch.float32, device=q.device) if weights is not None else None
+        o_part = lse_part = None
+        if splits > 1:
+            part = torch.empty(items * splits * tile * (d + 1), dtype=torch.float32, device=q.device)
+            o_part, lse_part = part, part[items * splits * tile * d:]
         _call("omni_kv4_decode", q.device, _p(q), q.stride(0), q.stride(1), _p(k_cache), _p(v_cache), blocks, block, hkv, d, _p(block_table),
-              block_table.stride(0), width, _p(seq_lens), B, T // B, hq, scale, longest, _p(out), _p(lse), _p(weights), decay)
+              block_table.stride(0), width, _p(seq_lens), B, T // B, hq, scale, longest, tile, splits, min_tiles, _p(o_part), _p(lse_part), _p(out), _p(lse), _p(weights), decay)
     return out
 
 

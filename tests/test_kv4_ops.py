@@ -519,6 +519,15 @@ def test_refusals(what):
 
 
 @pytest.mark.gpu
+def test_weights_of_too_many_rows_are_refused():
+    a = _args("cuda")
+    q = torch.zeros(2 * 129, 4, 64, dtype=torch.bfloat16, device="cuda")
+    ops.kv4_decode(q, a["kc"], a["vc"], a["table"], a["lens"], 1.0)
+    with pytest.raises(AssertionError, match="256"):
+        ops.kv4_decode(q, a["kc"], a["vc"], a["table"], a["lens"], 1.0, weights=a["w"])
+
+
+@pytest.mark.gpu
 def test_blocks_and_slots_outside_the_cache_are_skipped_and_reported():
     def reported(f):
         f()
