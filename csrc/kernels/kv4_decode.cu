@@ -21,6 +21,7 @@
 // codes and scales, two tiles ahead, an mbarrier a stage says when they are there.  No block-wide wait stands in the loop.  The warps'
 // results meet in shared memory at the end, those of the parts of a long request in a second kernel.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -60,17 +61,28 @@ __device__ __forceinline__ int kv4_length(const Kv4Decode& a, int block, int b, 
 // tiles of a part of `tiles`
 __device__ __forceinline__ int kv4_part(const Kv4Decode& a, int tiles) { return max(a.min_tiles, (tiles + a.splits - 1) / a.splits); }
 
-// bf16 pair 1 + code / 16 of the codes at bits 4 I of both halves of w
+// The codes minus 8 of the nibbles I of both halves of a word, as an fp16 pair, exactly.  Behind the exponent of 1024 a code in bits
+// 0 .. 3 makes 1024 + code and one in bits 4 .. 7 makes 1024 + 16 code; the fp16 multiply-add that takes the offset off runs on
+// another pipe than the integer operations.
+__device__ __forceinline__ uint32_t kv4_bits(uint32_t x, uint32_t mask) { return (x & mask) | 0x64006400u; }
 template <int I>
-__device__ __forceinline__ uint32_t kv4_ext(uint32_t w) {
-  const uint32_t s = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (s & 0x00780078u) | 0x3f803f80u;
+__device__ __forceinline__ uint32_t kv4_code(uint32_t w) {
+  if (I >= 2) w >>= 8;
+  __half2 v;
+  if (I & 1) {
+    const uint32_t x = kv4_bits(w, 0x00f000f0u);
+    v = __hfma2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+  } else {
+    const uint32_t x = kv4_bits(w, 0x000f000fu);
+    v = __hadd2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(-1032.f));
+  }
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ void kv4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void kv4_mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
   uint32_t y;
@@ -78,11 +90,8 @@ __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
   return y;
 }
 __device__ __forceinline__ uint32_t kv4_pack(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t kv4_rest(uint32_t packed, float lo, float hi) {
-  return kv4_pack(lo - __uint_as_float(packed << 16), hi - __uint_as_float(packed & 0xffff0000u));
 }
 __device__ __forceinline__ void kv4_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
@@ -105,53 +114,82 @@ __device__ __forceinline__ void kv4_lds(uint32_t (&w)[N], const uint8_t* p) {
 template <int NG, bool VALUES>
 struct Kv4Tile {
   static constexpr int PER = NG > 1 ? 2 : 1, PLANES = NG / PER;
-  static constexpr int TOKENS = NG == 4 ? 32 : 64, SUBS = TOKENS / 16;
+  static constexpr int TOKENS = NG == 4 ? 32 : 64;
   static constexpr int CODES = TOKENS * 32 * NG, SCALES = TOKENS * 4 * NG;
   static constexpr int V0 = CODES, KS0 = VALUES ? 2 * CODES : CODES, VS0 = KS0 + SCALES;
   static constexpr int BYTES = VALUES ? 2 * (CODES + SCALES) : CODES + SCALES;
   static constexpr int TOKEN_BYTES = BYTES / TOKENS;
   static constexpr int KINDS = VALUES ? 2 * PLANES + 2 : PLANES + 1;      // copies of a run of tokens
+};
 
-  // The block of the run of tokens that this lane copies of `tile`
-  static __device__ __forceinline__ int page(const Kv4Decode& a, const Kv4Cache& c, int b, int tile, int end, OmniStatus* st) {
-    const int t = tile * TOKENS + (int)(threadIdx.x & 31) / KINDS * a.piece;
-    if ((int)(threadIdx.x & 31) / KINDS * a.piece >= TOKENS || t >= end) return -1;
-    const int blk = a.table[(long long)b * a.table_ld + t / c.block];
-    if (blk >= 0 && blk < c.blocks) return blk;
-    report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, b);
-    return 0;                       // in bounds; the result is reported as wrong
+// The copies of a warp's tiles: lane l copies one kind of data (a plane of codes, the scales) of one run of `piece` tokens of a tile,
+// which lies in one block.  Block ids are fetched a tile ahead of their use.
+template <int NG, bool VALUES>
+struct Kv4Feed {
+  using T = Kv4Tile<NG, VALUES>;
+  const uint8_t* base;              // of this lane's kind and head, in block 0
+  long long blk_bytes;
+  const int* table;
+  int tok_bytes, dst, run;          // bytes a token, place in the stage, first token of the run in the tile (TOKENS: no copy)
+  int t, page, off, step, step_page, step_off;
+  int blk;
+
+  __device__ __forceinline__ void init(const Kv4Decode& a, const Kv4Cache& c, int b, int h, int tile, int stride, int end, OmniStatus* st) {
+    const int lane = threadIdx.x & 31, kind = lane % T::KINDS;
+    run = min(lane / T::KINDS * a.piece, T::TOKENS);
+    const bool values = VALUES && ((kind >= T::PLANES && kind < 2 * T::PLANES) || kind == 2 * T::PLANES + 1);
+    const bool scales = kind >= (VALUES ? 2 : 1) * T::PLANES;
+    const int plane = values ? kind - T::PLANES : kind;
+    tok_bytes = scales ? 4 * NG : 32 * T::PER;
+    base = (values ? c.v : c.k) + c.at(0, h) + (scales ? c.block * (32 * NG) : plane * c.block * (32 * T::PER));
+    dst = scales ? (values ? T::VS0 : T::KS0) + run * (4 * NG) : (values ? T::V0 : 0) + (plane * T::TOKENS + run) * (32 * T::PER);
+    blk_bytes = c.hkv * c.piece();
+    table = a.table + (long long)b * a.table_ld;
+    step = stride * T::TOKENS;
+    step_page = step / c.block;
+    step_off = step - step_page * c.block;
+    t = tile * T::TOKENS + run;
+    page = t / c.block;
+    off = t - page * c.block;
+    fetch(c, end, st);
   }
-  // Start the copies of `tile`: whole 16 tokens below `end`
-  static __device__ __forceinline__ void start(const Kv4Decode& a, const Kv4Cache& c, int h, int tile, int end, int blk, uint8_t* stage, uint64_t* bar) {
-    const int lane = threadIdx.x & 31, kind = lane % KINDS, off = lane / KINDS * a.piece;
-    const int count = min(TOKENS, (end - tile * TOKENS + 15) & ~15);
-    if (lane == 0) mbar_expect_tx(bar, count * TOKEN_BYTES);
-    __syncwarp();
-    if (blk < 0) return;
-    const int n = min(a.piece, count - off), t = (tile * TOKENS + off) % c.block;
-    const bool values = VALUES && (kind >= PLANES && kind < 2 * PLANES || kind == 2 * PLANES + 1);
-    const bool scales = kind >= (VALUES ? 2 : 1) * PLANES;
-    const uint8_t* src = (values ? c.v : c.k) + c.at(blk, h);
-    uint32_t dst = smem_u32(stage);
-    if (scales) {
-      src += c.block * (32 * NG) + t * (4 * NG);
-      dst += (values ? VS0 : KS0) + off * (4 * NG);
-    } else {
-      const int plane = values ? kind - PLANES : kind;
-      src += (plane * c.block + t) * (32 * PER);
-      dst += (values ? V0 : 0) + (plane * TOKENS + off) * (32 * PER);
+  __device__ __forceinline__ void fetch(const Kv4Cache& c, int end, OmniStatus* st) {
+    blk = -1;
+    if (run < T::TOKENS && t < end) {
+      blk = table[page];
+      if (blk < 0 || blk >= c.blocks) {
+        report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, page);
+        blk = 0;                    // in bounds; the result is reported as wrong
+      }
     }
-    kv4_bulk(dst, src, n * (scales ? 4 * NG : 32 * PER), bar);
+  }
+  // Start the copies of the tile in turn, `tokens` of it (a multiple of 16), and go on to the next one
+  __device__ __forceinline__ void start(const Kv4Decode& a, const Kv4Cache& c, int tokens, int end, uint8_t* stage, uint64_t* bar, OmniStatus* st) {
+    if ((threadIdx.x & 31) == 0) mbar_expect_tx(bar, tokens * T::TOKEN_BYTES);
+    __syncwarp();
+    if (blk >= 0) kv4_bulk(smem_u32(stage) + dst, base + blk * blk_bytes + off * tok_bytes, min(a.piece, tokens - run) * tok_bytes, bar);
+    t += step;
+    page += step_page;
+    off += step_off;
+    if (off >= c.block) {
+      off -= c.block;
+      ++page;
+    }
+    fetch(c, end, st);
   }
 };
 
-// Fragments of 8 query rows (row r: query token r / rep, head h rep + r % rep) and the sums of their groups for the rows 2 c, 2 c + 1
+// Fragments of 8 query rows (row r: query token r / rep, head h rep + r % rep) as fp16 numbers times a power of two common to the 8 rows
+// that brings the largest to 2^13 .. 2^14: bf16 numbers keep all their bits down to 2^-28 of the largest.  `unit` is its inverse, qs the
+// sums of the groups for the rows 2 c and 2 c + 1.
 template <int NG>
 struct Kv4Query {
   uint32_t b[NG][4][2];
+  float qs[NG][2], unit;
   __device__ __forceinline__ void load(const Kv4Decode& a, int rep, int b0, int h, int r, int total) {
     const int c = threadIdx.x & 3;
     const __nv_bfloat16* q = a.q + ((long long)b0 * a.rows + r / rep) * a.q_row + (long long)(h * rep + r % rep) * a.q_head + c * 16;
+    float most = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -162,17 +200,24 @@ struct Kv4Query {
           uint32_t v = 0u;
           if (r < total) v = (uint32_t)__bfloat16_as_ushort(q[at]) | (uint32_t)__bfloat16_as_ushort(q[at + 4]) << 16;
           b[g][s][e] = v;
+          most = fmaxf(most, fmaxf(fabsf(__uint_as_float(v << 16)), fabsf(__uint_as_float(v & 0xffff0000u))));
         }
-  }
-  __device__ __forceinline__ void sums(float (&qs)[NG][2]) const {
-    const int c = threadIdx.x & 3;
+    most = warp_max(most);
+    // exponent of the factor: 13 - that of the largest, within what a factor and its inverse can be
+    const int e = min(max(13 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100);
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+    unit = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float x = 0.f;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) x += __uint_as_float(b[g][s][e] << 16) + __uint_as_float(b[g][s][e] & 0xffff0000u);
+        for (int e2 = 0; e2 < 2; ++e2) {
+          const float lo = __uint_as_float(b[g][s][e2] << 16) * up, hi = __uint_as_float(b[g][s][e2] & 0xffff0000u) * up;
+          b[g][s][e2] = kv4_pack(lo, hi);
+          x += lo + hi;
+        }
       x += __shfl_xor_sync(0xffffffffu, x, 1);
       x += __shfl_xor_sync(0xffffffffu, x, 2);
       qs[g][0] = __shfl_sync(0xffffffffu, x, c * 8);
@@ -181,50 +226,216 @@ struct Kv4Query {
   }
 };
 
-// Scores, in units of log 2, of 16 tokens of a staged tile and 8 query rows per tile of NT: tokens r and r + 8, rows 2 c and 2 c + 1
-template <int NG, int NT, bool VALUES>
-__device__ __forceinline__ void kv4_scores(const uint8_t* stage, int sub, float scale_log2, const Kv4Query<NG> (&q)[NT], const float (&qs)[NT][NG][2],
-                                           float (&s)[NT][4]) {
+// Key codes minus 8 of 16 tokens of a staged tile: the fragments of one group
+template <int NG, bool VALUES>
+struct Kv4Keys {
   using T = Kv4Tile<NG, VALUES>;
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  uint32_t sc[2][NG];
+  uint32_t w[T::PLANES][2][2 * T::PER], sc[2][NG];
+  __device__ __forceinline__ void load(const uint8_t* stage, int sub) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) kv4_lds<NG>(sc[e], stage + T::KS0 + (sub * 16 + r + 8 * e) * (4 * NG));
+    for (int e = 0; e < 2; ++e) {
+      kv4_lds<NG>(sc[e], stage + T::KS0 + (sub * 16 + r + 8 * e) * (4 * NG));
 #pragma unroll
-  for (int n = 0; n < NT; ++n) { s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f; }
+      for (int p = 0; p < T::PLANES; ++p)
+        kv4_lds<2 * T::PER>(w[p][e], stage + (p * T::TOKENS + sub * 16 + r + 8 * e) * (32 * T::PER) + c * (8 * T::PER));
+    }
+  }
+  __device__ __forceinline__ void fragment(int g, int s, uint32_t (&a)[4]) const {       // s: 16 columns of the group
+    const uint32_t w0 = w[g / T::PER][0][g % T::PER * 2 + (s >> 1)], w1 = w[g / T::PER][1][g % T::PER * 2 + (s >> 1)];
+    if (s & 1) {
+      a[0] = kv4_code<2>(w0); a[1] = kv4_code<2>(w1); a[2] = kv4_code<3>(w0); a[3] = kv4_code<3>(w1);
+    } else {
+      a[0] = kv4_code<0>(w0); a[1] = kv4_code<0>(w1); a[2] = kv4_code<1>(w0); a[3] = kv4_code<1>(w1);
+    }
+  }
+};
+
+// Adds a group's part to the scores of tokens r and r + 8 and rows 2 c and 2 c + 1
+__device__ __forceinline__ void kv4_score(float (&s)[4], const float (&acc)[4], const uint32_t (&word)[2], const float (&qs)[2], float unit) {
 #pragma unroll
-  for (int p = 0; p < T::PLANES; ++p) {
-    uint32_t w[2][2 * T::PER];
+  for (int e = 0; e < 2; ++e) {
+    const float step = kv4_step(word[e]) * unit, mid = fmaf(step, 8.f, kv4_low(word[e]) * unit);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) kv4_lds<2 * T::PER>(w[e], stage + (p * T::TOKENS + sub * 16 + r + 8 * e) * (32 * T::PER) + c * (8 * T::PER));
+    for (int x = 0; x < 2; ++x) s[2 * e + x] = fmaf(step, acc[2 * e + x], fmaf(mid, qs[x], s[2 * e + x]));
+  }
+}
+
+// What a warp carries along the cache for its query rows: running maxima, sums of weights, and the two parts of the result
+template <int NG, int NT>
+struct Kv4Sums {
+  using T = Kv4Tile<NG, true>;
+  static constexpr int HALF = 32, SUBS = HALF / 16;
+  float m[NT][2], l[NT][2], o[NT][NG][4][4], z[NT][NG][2];
+  float most, to_one;               // power of two not below the value steps so far, and 128 over it
+
+  __device__ __forceinline__ void clear() {
+    most = 0.f;
+    to_one = 0.f;
 #pragma unroll
-    for (int gp = 0; gp < T::PER; ++gp) {
-      const int g = p * T::PER + gp;
-      float acc[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) { acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f; }
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t w0 = w[0][gp * 2 + x], w1 = w[1][gp * 2 + x];
-        const uint32_t a0 = kv4_ext<0>(w0), a1 = kv4_ext<0>(w1), a2 = kv4_ext<1>(w0), a3 = kv4_ext<1>(w1);
-        const uint32_t a4 = kv4_ext<2>(w0), a5 = kv4_ext<2>(w1), a6 = kv4_ext<3>(w0), a7 = kv4_ext<3>(w1);
+        m[n][x] = -INFINITY;
+        l[n][x] = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          kv4_mma(acc[n], a0, a1, a2, a3, q[n].b[g][2 * x][0], q[n].b[g][2 * x][1]);
-          kv4_mma(acc[n], a4, a5, a6, a7, q[n].b[g][2 * x + 1][0], q[n].b[g][2 * x + 1][1]);
+        for (int g = 0; g < NG; ++g) {
+          z[n][g][x] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][g][j][x] = o[n][g][j][x + 2] = 0.f;
         }
+      }
+  }
+
+  // 32 tokens from `t0` on, from sub `sub0` of the stage.  EDGE: some row does not see all of them.
+  template <bool EDGE>
+  __device__ __forceinline__ void add(const uint8_t* stage, int sub0, int t0, int end, const int (&sees)[NT][2], const Kv4Query<NG> (&q)[NT], float scale_log2) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
+    float s[SUBS][NT][4], top[NT][2], steps = 0.f;
+    uint32_t vs[SUBS][2][NG];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      Kv4Keys<NG, true> k;
+      k.load(stage, sub0 + u);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float acc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t f[4];
+          k.fragment(g, x, f);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) kv4_mma(acc[n], f, q[n].b[g][x]);
+        }
+        const uint32_t word[2] = {k.sc[0][g], k.sc[1][g]};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) kv4_score(s[u][n], acc[n], word, q[n].qs[g], q[n].unit * scale_log2);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float up = kv4_step(sc[e][g]) * (16.f * scale_log2), low = fmaf(kv4_low(sc[e][g]), scale_log2, -up);
+        const int t = t0 + u * 16 + r + 8 * e;
+        kv4_lds<NG>(vs[u][e], stage + T::VS0 + ((sub0 + u) * 16 + r + 8 * e) * (4 * NG));
+        if (EDGE) {
+          if (t >= end) {                                                  // what lies there is not of this request
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int g = 0; g < NG; ++g) vs[u][e][g] = 0u;
+          }
 #pragma unroll
-          for (int x = 0; x < 2; ++x) s[n][2 * e + x] = fmaf(up, acc[n][2 * e + x], fmaf(low, qs[n][g][x], s[n][2 * e + x]));
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              if (t >= sees[n][x]) s[u][n][2 * e + x] = -INFINITY;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) steps = fmaxf(steps, kv4_step(vs[u][e][g]));
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) top[n][x] = fmaxf(top[n][x], fmaxf(s[u][n][x], s[u][n][2 + x]));
+    }
+    // The maximum is followed only when a score exceeds it by 2^8: weights in fp32, and in fp16 after to_one, bear that.
+    bool more = steps > most;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) more |= top[n][0] > m[n][0] + 8.f || top[n][1] > m[n][1] + 8.f;
+    if (__any_sync(0xffffffffu, more)) rescale(top, steps);
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float sub = EDGE && m[n][x] == -INFINITY ? 0.f : m[n][x];
+          s[u][n][x] = ex2_fast(s[u][n][x] - sub);
+          s[u][n][2 + x] = ex2_fast(s[u][n][2 + x] - sub);
+          l[n][x] += s[u][n][x] + s[u][n][2 + x];
+        }
+#pragma unroll
+      for (int p = 0; p < T::PLANES; ++p) {
+        uint32_t w[2][2 * T::PER];                                         // pairs of tokens c and c + 4: even (groups), odd (groups)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int pair = cc + 4 * e;
+          const int ch = T::PER == 2 ? r ^ ((pair & 3) << 1) : r ^ (((pair >> 1) & 1) << 2);
+          kv4_lds<2 * T::PER>(w[e], stage + T::V0 + (p * T::TOKENS + (sub0 + u) * 16 + pair * 2) * (32 * T::PER) + ch * (8 * T::PER));
+        }
+#pragma unroll
+        for (int gp = 0; gp < T::PER; ++gp) {
+          const int g = p * T::PER + gp;
+          uint32_t pt[NT][2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float step = kv4_step(vs[u][e][g]), mid = fmaf(step, 8.f, kv4_low(vs[u][e][g])), up = step * to_one;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float p0 = s[u][n][2 * e], p1 = s[u][n][2 * e + 1];
+              float f0 = p0 * up, f1 = p1 * up;
+              if (EDGE) {                                                  // an unseen token adds nothing, whatever its value
+                f0 = p0 == 0.f ? 0.f : f0;
+                f1 = p1 == 0.f ? 0.f : f1;
+                z[n][g][0] += p0 == 0.f ? 0.f : p0 * mid;
+                z[n][g][1] += p1 == 0.f ? 0.f : p1 * mid;
+              } else {
+                z[n][g][0] = fmaf(p0, mid, z[n][g][0]);
+                z[n][g][1] = fmaf(p1, mid, z[n][g][1]);
+              }
+              pt[n][e] = kv4_transpose(kv4_pack(f0, f1));
+            }
+          }
+          const uint32_t x0 = __byte_perm(w[0][gp], w[0][T::PER + gp], 0x5410), y0 = __byte_perm(w[0][gp], w[0][T::PER + gp], 0x7632);
+          const uint32_t x1 = __byte_perm(w[1][gp], w[1][T::PER + gp], 0x5410), y1 = __byte_perm(w[1][gp], w[1][T::PER + gp], 0x7632);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t v0 = j < 2 ? x0 : y0, v1 = j < 2 ? x1 : y1;
+            const uint32_t f[4] = {j & 1 ? kv4_code<2>(v0) : kv4_code<0>(v0), j & 1 ? kv4_code<3>(v0) : kv4_code<1>(v0),
+                                   j & 1 ? kv4_code<2>(v1) : kv4_code<0>(v1), j & 1 ? kv4_code<3>(v1) : kv4_code<1>(v1)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) kv4_mma(o[n][g][j], f, pt[n]);
+          }
+        }
       }
     }
   }
-}
+
+  __device__ __forceinline__ void rescale(const float (&top)[NT][2], float steps) {
+    steps = warp_max(steps);
+    float by = 1.f;
+    if (steps > most) {
+      const float next = fmaxf(__uint_as_float((__float_as_uint(steps) + 0x007fffffu) & 0x7f800000u), 0x1p-110f);
+      const float next_to_one = __uint_as_float(0x7f000000u - __float_as_uint(next)) * 128.f;
+      by = most * next_to_one * 0.0078125f;
+      most = next;
+      to_one = next_to_one;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float v = top[n][x];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+        v = fmaxf(v, m[n][x]);
+        const float f = v == -INFINITY ? 1.f : ex2_fast(m[n][x] - v);
+        m[n][x] = v;
+        l[n][x] *= f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          z[n][g][x] *= f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            o[n][g][j][x] *= f * by;
+            o[n][g][j][x + 2] *= f * by;
+          }
+        }
+      }
+  }
+};
 
 template <int NG, int NT>
 __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decode_kernel(Kv4Decode a, Kv4Cache c, OmniStatus* st) {
@@ -253,163 +464,37 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   __syncthreads();
-  int tile = begin_tile + warp, next = tile, blk = T::page(a, c, b, next, next < end_tile ? end : 0, st);
+  const int stop = min(end, end_tile * T::TOKENS);                         // first token behind this part
+  int tile = begin_tile + warp, next = tile;
+  Kv4Feed<NG, true> feed;
+  feed.init(a, c, b, h, tile, KV4_WARPS, stop, st);
 #pragma unroll
-  for (int s = 0; s < KV4_STAGES; ++s) {
-    if (next < end_tile) T::start(a, c, h, next, end, blk, stages + s * T::BYTES, bar + s);
-    next += KV4_WARPS;
-    blk = T::page(a, c, b, next, next < end_tile ? end : 0, st);
-  }
+  for (int s = 0; s < KV4_STAGES; ++s, next += KV4_WARPS)
+    if (next < end_tile) feed.start(a, c, min(T::TOKENS, (end - next * T::TOKENS + 15) & ~15), stop, stages + s * T::BYTES, bar + s, st);
 
   Kv4Query<NG> q[NT];
-  float qs[NT][NG][2];
+  int sees[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     q[n].load(a, rep, b, h, row0 + n * 8 + r, total);
-    q[n].sums(qs[n]);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) sees[n][x] = len - a.rows + 1 + min(row0 + n * 8 + cc * 2 + x, total - 1) / rep;
   }
-  float m[NT][2], l[NT][2], o[NT][NG][4][4], z[NT][NG][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      m[n][x] = -INFINITY;
-      l[n][x] = 0.f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        z[n][g][x] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[n][g][j][x] = o[n][g][j][x + 2] = 0.f;
-      }
-    }
-
+  Kv4Sums<NG, NT> sum;
+  sum.clear();
   int it = 0;
-  for (; tile < end_tile; tile += KV4_WARPS, ++it) {
+  for (; tile < end_tile; tile += KV4_WARPS, next += KV4_WARPS, ++it) {
     const int st_i = it % KV4_STAGES;
     uint8_t* stage = stages + st_i * T::BYTES;
     if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (it / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_TILE, tile))) break;
-    const int t0 = tile * T::TOKENS;
-    const bool edge = t0 + T::TOKENS > first_sees;                         // some row does not see all of the tile
-    float s[T::SUBS][NT][4], top[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < T::SUBS; ++u) {
-      kv4_scores<NG, NT, true>(stage, u, a.scale_log2, q, qs, s[u]);
-      if (edge) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int sees = len - a.rows + 1 + min(row0 + n * 8 + cc * 2 + x, total - 1) / rep;
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (t0 + u * 16 + r + 8 * e >= sees) s[u][n][2 * e + x] = -INFINITY;
-          }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) top[n][x] = fmaxf(top[n][x], fmaxf(s[u][n][x], s[u][n][2 + x]));
-    }
-    // The maximum is followed only when a score exceeds it by 2^8, which weights in fp32 and bf16 bear easily.
-    bool more = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) more |= top[n][0] > m[n][0] + 8.f || top[n][1] > m[n][1] + 8.f;
-    if (__any_sync(0xffffffffu, more)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float v = top[n][x];
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-          v = fmaxf(v, m[n][x]);
-          const float f = v == -INFINITY ? 1.f : ex2_fast(m[n][x] - v);
-          m[n][x] = v;
-          l[n][x] *= f;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            z[n][g][x] *= f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              o[n][g][j][x] *= f;
-              o[n][g][j][x + 2] *= f;
-            }
-          }
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < T::SUBS; ++u) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float sub = m[n][x] == -INFINITY ? 0.f : m[n][x];
-          s[u][n][x] = ex2_fast(s[u][n][x] - sub);
-          s[u][n][2 + x] = ex2_fast(s[u][n][2 + x] - sub);
-          l[n][x] += s[u][n][x] + s[u][n][2 + x];
-        }
-      uint32_t sc[2][NG];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        kv4_lds<NG>(sc[e], stage + T::VS0 + (u * 16 + r + 8 * e) * (4 * NG));
-        if (edge && t0 + u * 16 + r + 8 * e >= end) {                      // what lies there is not of this request
-#pragma unroll
-          for (int g = 0; g < NG; ++g) sc[e][g] = 0u;
-        }
-      }
-#pragma unroll
-      for (int p = 0; p < T::PLANES; ++p) {
-        uint32_t w[2][2 * T::PER];                                         // pairs of tokens c and c + 4: even (groups), odd (groups)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int pair = u * 8 + cc + 4 * e;
-          const int ch = T::PER == 2 ? r ^ ((pair & 3) << 1) : r ^ (((pair >> 1) & 1) << 2);
-          kv4_lds<2 * T::PER>(w[e], stage + T::V0 + (p * T::TOKENS + pair * 2) * (32 * T::PER) + ch * (8 * T::PER));
-        }
-#pragma unroll
-        for (int gp = 0; gp < T::PER; ++gp) {
-          const int g = p * T::PER + gp;
-          uint32_t hi[NT][2], lo[NT][2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float up = kv4_step(sc[e][g]) * 16.f, low = kv4_low(sc[e][g]) - up;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float p0 = s[u][n][2 * e], p1 = s[u][n][2 * e + 1];
-              float f0 = p0 * up, f1 = p1 * up, z0 = p0 * low, z1 = p1 * low;
-              if (edge) {                                                  // an unseen token adds nothing, whatever its value
-                if (p0 == 0.f) f0 = z0 = 0.f;
-                if (p1 == 0.f) f1 = z1 = 0.f;
-              }
-              z[n][g][0] += z0;
-              z[n][g][1] += z1;
-              hi[n][e] = kv4_pack(f0, f1);
-              lo[n][e] = kv4_transpose(kv4_rest(hi[n][e], f0, f1));
-              hi[n][e] = kv4_transpose(hi[n][e]);
-            }
-          }
-          const uint32_t x0 = __byte_perm(w[0][gp], w[0][T::PER + gp], 0x5410), y0 = __byte_perm(w[0][gp], w[0][T::PER + gp], 0x7632);
-          const uint32_t x1 = __byte_perm(w[1][gp], w[1][T::PER + gp], 0x5410), y1 = __byte_perm(w[1][gp], w[1][T::PER + gp], 0x7632);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t v0 = j < 2 ? x0 : y0, v1 = j < 2 ? x1 : y1;
-            const uint32_t a0 = j & 1 ? kv4_ext<2>(v0) : kv4_ext<0>(v0), a1 = j & 1 ? kv4_ext<3>(v0) : kv4_ext<1>(v0);
-            const uint32_t a2 = j & 1 ? kv4_ext<2>(v1) : kv4_ext<0>(v1), a3 = j & 1 ? kv4_ext<3>(v1) : kv4_ext<1>(v1);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              kv4_mma(o[n][g][j], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-              kv4_mma(o[n][g][j], a0, a1, a2, a3, lo[n][0], lo[n][1]);
-            }
-          }
-        }
-      }
+#pragma unroll 1
+    for (int sub = 0; sub < T::TOKENS / 16; sub += 2) {
+      const int t0 = tile * T::TOKENS + sub * 16;
+      if (t0 + 32 <= first_sees) sum.template add<false>(stage, sub, t0, end, sees, q, a.scale_log2);
+      else if (t0 < end) sum.template add<true>(stage, sub, t0, end, sees, q, a.scale_log2);
     }
     __syncwarp();                                                          // every lane has read the stage
-    if (next < end_tile) T::start(a, c, h, next, end, blk, stage, bar + st_i);
-    next += KV4_WARPS;
-    blk = T::page(a, c, b, next, next < end_tile ? end : 0, st);
+    if (next < end_tile) feed.start(a, c, min(T::TOKENS, (end - next * T::TOKENS + 15) & ~15), stop, stage, bar + st_i, st);
   }
 
   // ---- the sums over the lanes that share a query row, then over the warps
@@ -419,9 +504,9 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
-        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], d);
+        sum.l[n][x] += __shfl_xor_sync(0xffffffffu, sum.l[n][x], d);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) z[n][g][x] += __shfl_xor_sync(0xffffffffu, z[n][g][x], d);
+        for (int g = 0; g < NG; ++g) sum.z[n][g][x] += __shfl_xor_sync(0xffffffffu, sum.z[n][g][x], d);
       }
   __syncthreads();
   if (abort_flag != 0) {                                                   // copies may still be under way: leave the memory alone
@@ -434,6 +519,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     }
     return;
   }
+  const float unit = sum.most * 0.0078125f;
   float* s_o = reinterpret_cast<float*>(smem);                             // [warps][NQ][D]
   float* s_m = s_o + KV4_WARPS * NQ * D;                                   // [warps][NQ], and the sums likewise
   float* s_l = s_m + KV4_WARPS * NQ;
@@ -443,30 +529,31 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     for (int x = 0; x < 2; ++x) {
       const int i = warp * NQ + n * 8 + cc * 2 + x;
       if (r == 0) {
-        s_m[i] = m[n][x];
-        s_l[i] = l[n][x];
+        s_m[i] = sum.m[n][x];
+        s_l[i] = sum.l[n][x];
       }
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<float2*>(s_o + (size_t)i * D + g * 64 + r * 8 + j * 2) = make_float2(o[n][g][j][x] + z[n][g][x], o[n][g][j][x + 2] + z[n][g][x]);
+          *reinterpret_cast<float2*>(s_o + (size_t)i * D + g * 64 + r * 8 + j * 2) = 
+              make_float2(fmaf(sum.o[n][g][j][x], unit, sum.z[n][g][x]), fmaf(sum.o[n][g][j][x + 2], unit, sum.z[n][g][x]));
     }
   __syncthreads();
   for (int i = threadIdx.x; i < NQ * D; i += KV4_WARPS * 32) {
     const int row = i / D, d = i - row * D;
     if (row0 + row >= total) break;
-    float mm = -INFINITY, sum = 0.f, acc = 0.f;
+    float mm = -INFINITY, total_l = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < KV4_WARPS; ++w) mm = fmaxf(mm, s_m[w * NQ + row]);
 #pragma unroll
     for (int w = 0; w < KV4_WARPS; ++w) {
       const float mw = s_m[w * NQ + row];
       const float f = mw == -INFINITY ? (s_l[w * NQ + row] == 0.f ? 0.f : 1.f) : ex2_fast(mw - mm);      // a sum without a maximum is NaN
-      sum += s_l[w * NQ + row] * f;
+      total_l += s_l[w * NQ + row] * f;
       acc += s_o[((size_t)w * NQ + row) * D + d] * f;
     }
-    const float value = sum == 0.f ? 0.f : acc / sum, lse = sum == 0.f ? -INFINITY : mm + __log2f(sum);
+    const float value = total_l == 0.f ? 0.f : acc / total_l, lse = total_l == 0.f ? -INFINITY : mm + __log2f(total_l);
     const int head = h * rep + (row0 + row) % rep, tok = (row0 + row) / rep;
     if (a.splits == 1) {
       a.out[(((long long)b * a.rows + tok) * a.hq + head) * D + d] = __float2bfloat16(value);
@@ -504,7 +591,8 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, 
 }
 
 // The weights that the rows give a request's tokens: the scores of the staged keys once more, against the finished sums.  Reading the
-// keys twice costs as much as keeping the scores of 8 query rows would, and nothing more for more rows.
+// keys twice costs as much as keeping the scores of 8 query rows would, and nothing more for more rows; 16 tokens are unpacked once for
+// all rows, whose fragments stand in shared memory.
 template <int NG>
 __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decode a, Kv4Cache c, OmniStatus* st) {
   using T = Kv4Tile<NG, false>;
@@ -515,12 +603,12 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   const int h = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
   const int len = kv4_length(a, c.block, b, st), tiles = (len + T::TOKENS - 1) / T::TOKENS;
-  const int step = gridDim.x * KV4_WARPS;
+  const int stride = gridDim.x * KV4_WARPS;
   if (blockIdx.x * KV4_WARPS >= tiles) return;
   uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
   uint2* s_q = reinterpret_cast<uint2*>(smem + KV4_WARPS * KV4_STAGES * T::BYTES);      // [chunks][NG * 4][32]
-  float* s_qs = reinterpret_cast<float*>(s_q + chunks * NG * 4 * 32);                    // [chunks][NG][8]
-  float* s_lse = s_qs + chunks * NG * 8;                                                 // [chunks][8]
+  float4* s_row = reinterpret_cast<float4*>(s_q + chunks * NG * 4 * 32);                 // [chunks][1 + NG / 2][4]: see below
+  constexpr int ROW = 1 + (NG + 1) / 2;
   uint64_t* bar = bars + warp * KV4_STAGES;
   if (threadIdx.x == 0) abort_flag = 0;
   if (lane == 0) {
@@ -529,99 +617,104 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   __syncthreads();
-  int tile = blockIdx.x * KV4_WARPS + warp, next = tile, blk = T::page(a, c, b, next, next < tiles ? len : 0, st);
+  int tile = blockIdx.x * KV4_WARPS + warp, next = tile;
+  Kv4Feed<NG, false> feed;
+  feed.init(a, c, b, h, tile, stride, len, st);
 #pragma unroll
-  for (int s = 0; s < KV4_STAGES; ++s) {
-    if (next < tiles) T::start(a, c, h, next, len, blk, stages + s * T::BYTES, bar + s);
-    next += step;
-    blk = T::page(a, c, b, next, next < tiles ? len : 0, st);
-  }
+  for (int s = 0; s < KV4_STAGES; ++s, next += stride)
+    if (next < tiles) feed.start(a, c, min(T::TOKENS, (len - next * T::TOKENS + 15) & ~15), len, stages + s * T::BYTES, bar + s, st);
   for (int ch = warp; ch < chunks; ch += KV4_WARPS) {
     Kv4Query<NG> q;
-    float qs[NG][2];
     q.load(a, rep, b, h, ch * 8 + r, total);
-    q.sums(qs);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
+    for (int g = 0; g < NG; ++g)
 #pragma unroll
       for (int s = 0; s < 4; ++s) s_q[(ch * NG * 4 + g * 4 + s) * 32 + lane] = make_uint2(q.b[g][s][0], q.b[g][s][1]);
-      if (r == 0) {
-        s_qs[(ch * NG + g) * 8 + cc * 2] = qs[g][0];
-        s_qs[(ch * NG + g) * 8 + cc * 2 + 1] = qs[g][1];
+    if (r == 0) {                   // of the rows 2 c and 2 c + 1: their sums, the unit, and then pairs of qs
+      float lse[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int row = ch * 8 + cc * 2 + x;
+        lse[x] = row < total ? a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep] : INFINITY;
       }
-    }
-    if (lane < 8) {
-      const int row = ch * 8 + lane;
-      s_lse[row] = row < total ? a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep] : INFINITY;
+      s_row[(ch * ROW) * 4 + cc] = make_float4(lse[0], lse[1], q.unit * a.scale_log2, 0.f);
+#pragma unroll
+      for (int g = 0; g < NG; g += 2)
+        s_row[(ch * ROW + 1 + g / 2) * 4 + cc] = make_float4(q.qs[g][0], q.qs[g][1], g + 1 < NG ? q.qs[(g + 1) % NG][0] : 0.f, g + 1 < NG ? q.qs[(g + 1) % NG][1] : 0.f);
     }
   }
   __syncthreads();
   int it = 0;
-  for (; tile < tiles; tile += step, ++it) {
+  for (; tile < tiles; tile += stride, next += stride, ++it) {
     const int st_i = it % KV4_STAGES;
     uint8_t* stage = stages + st_i * T::BYTES;
     if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (it / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_WEIGHTS, tile))) break;
-    const int t0 = tile * T::TOKENS;
-    const bool edge = t0 + T::TOKENS > len - a.rows + 1;
-    float w[T::SUBS][2];
+#pragma unroll 1
+    for (int u = 0; u < T::TOKENS / 16; ++u) {
+      const int t0 = tile * T::TOKENS + u * 16;
+      if (t0 >= len) break;
+      const bool edge = t0 + 16 > len - a.rows + 1;
+      Kv4Keys<NG, false> k;
+      k.load(stage, u);
+      uint32_t f[NG][4][4];
 #pragma unroll
-    for (int u = 0; u < T::SUBS; ++u) w[u][0] = w[u][1] = 0.f;
-    for (int ch = 0; ch < chunks; ++ch) {
-      Kv4Query<NG> q[1];
-      float qs[1][NG][2];
+      for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
+        for (int x = 0; x < 4; ++x) k.fragment(g, x, f[g][x]);
+      float w[2] = {0.f, 0.f};
+#pragma unroll 1
+      for (int ch = 0; ch < chunks; ++ch) {
+        const float4 row = s_row[ch * ROW * 4 + cc];
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const uint2 v = s_q[(ch * NG * 4 + g * 4 + s) * 32 + lane];
-          q[0].b[g][s][0] = v.x;
-          q[0].b[g][s][1] = v.y;
+        for (int g = 0; g < NG; ++g) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint2 v = s_q[(ch * NG * 4 + g * 4 + x) * 32 + lane];
+            const uint32_t qb[2] = {v.x, v.y};
+            kv4_mma(acc, f[g][x], qb);
+          }
+          const float4 sums = s_row[(ch * ROW + 1 + g / 2) * 4 + cc];
+          const float qs[2] = {g & 1 ? sums.z : sums.x, g & 1 ? sums.w : sums.y};
+          const uint32_t word[2] = {k.sc[0][g], k.sc[1][g]};
+          kv4_score(s, acc, word, qs, row.z);
         }
-        qs[0][g][0] = s_qs[(ch * NG + g) * 8 + cc * 2];
-        qs[0][g][1] = s_qs[(ch * NG + g) * 8 + cc * 2 + 1];
-      }
-      const float lse[2] = {s_lse[ch * 8 + cc * 2], s_lse[ch * 8 + cc * 2 + 1]};
 #pragma unroll
-      for (int u = 0; u < T::SUBS; ++u) {
-        float s[1][4];
-        kv4_scores<NG, 1, false>(stage, u, a.scale_log2, q, qs, s);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int row = ch * 8 + cc * 2 + x, sees = row < total ? len - a.rows + 1 + row / rep : 0;
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float p = ex2_fast(s[0][2 * e + x] - lse[x]);
-            if (!edge || t0 + u * 16 + r + 8 * e < sees) w[u][e] += row < total ? p : 0.f;
+            float p = ex2_fast(s[2 * e + x] - (x ? row.y : row.x));
+            if (edge || ch == chunks - 1) {                                // rows beyond the last, tokens that the row does not see
+              const int i = ch * 8 + cc * 2 + x;
+              if (i >= total || t0 + r + 8 * e >= len - a.rows + 1 + i / rep) p = 0.f;
+            }
+            w[e] += p;
           }
-        }
       }
-    }
-#pragma unroll
-    for (int u = 0; u < T::SUBS; ++u)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        w[u][e] += __shfl_xor_sync(0xffffffffu, w[u][e], 1);
-        w[u][e] += __shfl_xor_sync(0xffffffffu, w[u][e], 2);
-        const int t = t0 + u * 16 + r + 8 * e;
+        w[e] += __shfl_xor_sync(0xffffffffu, w[e], 1);
+        w[e] += __shfl_xor_sync(0xffffffffu, w[e], 2);
+        const int t = t0 + r + 8 * e;
         if (cc == 0 && t < len) {
           const int at = a.table[(long long)b * a.table_ld + t / c.block];
           if (at >= 0 && at < c.blocks) {
             float* to = a.weights + ((long long)at * c.hkv + h) * c.block + t % c.block;
-            *to = a.decay == 0.f ? w[u][e] : fmaf(a.decay, *to, w[u][e]);
+            *to = a.decay == 0.f ? w[e] : fmaf(a.decay, *to, w[e]);
           }
         }
       }
+    }
     __syncwarp();
-    if (next < tiles) T::start(a, c, h, next, len, blk, stage, bar + st_i);
-    next += step;
-    blk = T::page(a, c, b, next, next < tiles ? len : 0, st);
+    if (next < tiles) feed.start(a, c, min(T::TOKENS, (len - next * T::TOKENS + 15) & ~15), len, stage, bar + st_i, st);
   }
   __syncthreads();
   if (abort_flag != 0) {
     if (threadIdx.x == 0) report_abort(&abort_flag, st);
     for (int s = 0; s < KV4_STAGES; ++s) {
       const int left = it + s;
-      if (tile + s * step < tiles) {
+      if (tile + s * stride < tiles) {
         for (int i = 0; i < 1 << 16 && !mbar_try_wait(bar + left % KV4_STAGES, (left / KV4_STAGES) & 1); ++i) {}
       }
     }
@@ -657,7 +750,7 @@ template <int NG>
 static cudaError_t kv4_launch_weights(const Kv4Decode& a, const Kv4Cache& c, int B, int max_len, OmniStatus* st, cudaStream_t stream) {
   using T = Kv4Tile<NG, false>;
   const int total = a.rows * (a.hq / c.hkv), chunks = (total + 7) / 8;
-  const int bytes = KV4_WARPS * KV4_STAGES * T::BYTES + chunks * (NG * 4 * 32 * 8 + NG * 8 * 4 + 8 * 4);
+  const int bytes = KV4_WARPS * KV4_STAGES * T::BYTES + chunks * (NG * 4 * 32 * 8 + (1 + (NG + 1) / 2) * 4 * 16);
   static int most[64] = {0};
   cudaError_t e = kv4_smem((const void*)kv4_weights_kernel<NG>, bytes, most);
   if (e != cudaSuccess) return e;
