@@ -33,7 +33,7 @@
 namespace omni {
 
 constexpr int KV4_SITE_DECODE = 84, KV4_SITE_TILE = 85, KV4_SITE_WEIGHTS = 86;
-constexpr int KV4_WARPS = 4, KV4_STAGES = 2;
+constexpr int KV4_WARPS = 4, KV4_STAGES = 2, KV4_MAX_PARTS = 512;
 
 struct Kv4Decode {
   const __nv_bfloat16* q;
@@ -64,16 +64,21 @@ __device__ __forceinline__ int kv4_part(const Kv4Decode& a, int tiles) { return 
 // The codes minus 8 of the nibbles I of both halves of a word, as an fp16 pair, exactly.  Behind the exponent of 1024 a code in bits
 // 0 .. 3 makes 1024 + code and one in bits 4 .. 7 makes 1024 + 16 code; the fp16 multiply-add that takes the offset off runs on
 // another pipe than the integer operations.
-__device__ __forceinline__ uint32_t kv4_bits(uint32_t x, uint32_t mask) { return (x & mask) | 0x64006400u; }
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t kv4_bits(uint32_t x) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, 0x64006400, 0xEA;" : "=r"(y) : "r"(x), "n"(MASK));      // (x & MASK) | 0x64006400
+  return y;
+}
 template <int I>
 __device__ __forceinline__ uint32_t kv4_code(uint32_t w) {
   if (I >= 2) w >>= 8;
   __half2 v;
   if (I & 1) {
-    const uint32_t x = kv4_bits(w, 0x00f000f0u);
+    const uint32_t x = kv4_bits<0x00f000f0u>(w);
     v = __hfma2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
   } else {
-    const uint32_t x = kv4_bits(w, 0x000f000fu);
+    const uint32_t x = kv4_bits<0x000f000fu>(w);
     v = __hadd2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(-1032.f));
   }
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -179,13 +184,13 @@ struct Kv4Feed {
   }
 };
 
-// Fragments of 8 query rows (row r: query token r / rep, head h rep + r % rep) as fp16 numbers times a power of two common to the 8 rows
-// that brings the largest to 2^13 .. 2^14: bf16 numbers keep all their bits down to 2^-28 of the largest.  `unit` is its inverse, qs the
-// sums of the groups for the rows 2 c and 2 c + 1.
+// Fragments of 8 query rows (row r: query token r / rep, head h rep + r % rep) as fp16 numbers, each row times a power of two that
+// brings its largest number to 2^13 .. 2^14: bf16 numbers keep all their bits down to 2^-28 of the largest.  qs are the sums of the
+// groups, unit what brings scores to units of log 2 (its sign is that of the query), for the rows 2 c and 2 c + 1.
 template <int NG>
 struct Kv4Query {
   uint32_t b[NG][4][2];
-  float qs[NG][2], unit;
+  float qs[NG][2], unit[2];
   __device__ __forceinline__ void load(const Kv4Decode& a, int rep, int b0, int h, int r, int total) {
     const int c = threadIdx.x & 3;
     const __nv_bfloat16* q = a.q + ((long long)b0 * a.rows + r / rep) * a.q_row + (long long)(h * rep + r % rep) * a.q_head + c * 16;
@@ -202,11 +207,14 @@ struct Kv4Query {
           b[g][s][e] = v;
           most = fmaxf(most, fmaxf(fabsf(__uint_as_float(v << 16)), fabsf(__uint_as_float(v & 0xffff0000u))));
         }
-    most = warp_max(most);
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     // exponent of the factor: 13 - that of the largest, within what a factor and its inverse can be
     const int e = min(max(13 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100);
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    unit = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float up = copysignf(__uint_as_float((uint32_t)(127 + e) << 23), a.scale_log2);
+    const float un = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23), 0x1p-120f);
+    unit[0] = __shfl_sync(0xffffffffu, un, c * 8);
+    unit[1] = __shfl_sync(0xffffffffu, un, c * 8 + 4);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float x = 0.f;
@@ -226,7 +234,7 @@ struct Kv4Query {
   }
 };
 
-// Key codes minus 8 of 16 tokens of a staged tile: the fragments of one group
+// Key codes minus 8 of 16 tokens of a staged tile
 template <int NG, bool VALUES>
 struct Kv4Keys {
   using T = Kv4Tile<NG, VALUES>;
@@ -252,10 +260,10 @@ struct Kv4Keys {
 };
 
 // Adds a group's part to the scores of tokens r and r + 8 and rows 2 c and 2 c + 1
-__device__ __forceinline__ void kv4_score(float (&s)[4], const float (&acc)[4], const uint32_t (&word)[2], const float (&qs)[2], float unit) {
+__device__ __forceinline__ void kv4_score(float (&s)[4], const float (&acc)[4], const uint32_t (&word)[2], const float (&qs)[2]) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const float step = kv4_step(word[e]) * unit, mid = fmaf(step, 8.f, kv4_low(word[e]) * unit);
+    const float step = kv4_step(word[e]), mid = fmaf(step, 8.f, kv4_low(word[e]));
 #pragma unroll
     for (int x = 0; x < 2; ++x) s[2 * e + x] = fmaf(step, acc[2 * e + x], fmaf(mid, qs[x], s[2 * e + x]));
   }
@@ -266,7 +274,7 @@ template <int NG, int NT>
 struct Kv4Sums {
   using T = Kv4Tile<NG, true>;
   static constexpr int HALF = 32, SUBS = HALF / 16;
-  float m[NT][2], l[NT][2], o[NT][NG][4][4], z[NT][NG][2];
+  float m[NT][2], l[NT][2], o[NT][NG][4][4], z[NT][NG][2];                 // m in the scores' own units
   float most, to_one;               // power of two not below the value steps so far, and 128 over it
 
   __device__ __forceinline__ void clear() {
@@ -289,7 +297,7 @@ struct Kv4Sums {
 
   // 32 tokens from `t0` on, from sub `sub0` of the stage.  EDGE: some row does not see all of them.
   template <bool EDGE>
-  __device__ __forceinline__ void add(const uint8_t* stage, int sub0, int t0, int end, const int (&sees)[NT][2], const Kv4Query<NG> (&q)[NT], float scale_log2) {
+  __device__ __forceinline__ void add(const uint8_t* stage, int sub0, int t0, int end, const int (&sees)[NT][2], const Kv4Query<NG> (&q)[NT]) {
     const int lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
     float s[SUBS][NT][4], top[NT][2], steps = 0.f;
     uint32_t vs[SUBS][2][NG];
@@ -315,7 +323,7 @@ struct Kv4Sums {
         }
         const uint32_t word[2] = {k.sc[0][g], k.sc[1][g]};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) kv4_score(s[u][n], acc[n], word, q[n].qs[g], q[n].unit * scale_log2);
+        for (int n = 0; n < NT; ++n) kv4_score(s[u][n], acc[n], word, q[n].qs[g]);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -343,17 +351,17 @@ struct Kv4Sums {
     // The maximum is followed only when a score exceeds it by 2^8: weights in fp32, and in fp16 after to_one, bear that.
     bool more = steps > most;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) more |= top[n][0] > m[n][0] + 8.f || top[n][1] > m[n][1] + 8.f;
-    if (__any_sync(0xffffffffu, more)) rescale(top, steps);
+    for (int n = 0; n < NT; ++n) more |= (top[n][0] - m[n][0]) * q[n].unit[0] > 8.f || (top[n][1] - m[n][1]) * q[n].unit[1] > 8.f;
+    if (__any_sync(0xffffffffu, more)) rescale(top, steps, q);
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float sub = EDGE && m[n][x] == -INFINITY ? 0.f : m[n][x];
-          s[u][n][x] = ex2_fast(s[u][n][x] - sub);
-          s[u][n][2 + x] = ex2_fast(s[u][n][2 + x] - sub);
+          const float sub = EDGE && m[n][x] == -INFINITY ? 0.f : m[n][x] * q[n].unit[x];
+          s[u][n][x] = ex2_fast(fmaf(s[u][n][x], q[n].unit[x], -sub));
+          s[u][n][2 + x] = ex2_fast(fmaf(s[u][n][2 + x], q[n].unit[x], -sub));
           l[n][x] += s[u][n][x] + s[u][n][2 + x];
         }
 #pragma unroll
@@ -403,7 +411,7 @@ struct Kv4Sums {
     }
   }
 
-  __device__ __forceinline__ void rescale(const float (&top)[NT][2], float steps) {
+  __device__ __forceinline__ void rescale(const float (&top)[NT][2], float steps, const Kv4Query<NG> (&q)[NT]) {
     steps = warp_max(steps);
     float by = 1.f;
     if (steps > most) {
@@ -421,7 +429,7 @@ struct Kv4Sums {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
         v = fmaxf(v, m[n][x]);
-        const float f = v == -INFINITY ? 1.f : ex2_fast(m[n][x] - v);
+        const float f = v == -INFINITY ? 1.f : ex2_fast((m[n][x] - v) * q[n].unit[x]);
         m[n][x] = v;
         l[n][x] *= f;
 #pragma unroll
@@ -490,8 +498,8 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
 #pragma unroll 1
     for (int sub = 0; sub < T::TOKENS / 16; sub += 2) {
       const int t0 = tile * T::TOKENS + sub * 16;
-      if (t0 + 32 <= first_sees) sum.template add<false>(stage, sub, t0, end, sees, q, a.scale_log2);
-      else if (t0 < end) sum.template add<true>(stage, sub, t0, end, sees, q, a.scale_log2);
+      if (t0 + 32 <= first_sees) sum.template add<false>(stage, sub, t0, end, sees, q);
+      else if (t0 < end) sum.template add<true>(stage, sub, t0, end, sees, q);
     }
     __syncwarp();                                                          // every lane has read the stage
     if (next < end_tile) feed.start(a, c, min(T::TOKENS, (end - next * T::TOKENS + 15) & ~15), stop, stage, bar + st_i, st);
@@ -529,7 +537,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     for (int x = 0; x < 2; ++x) {
       const int i = warp * NQ + n * 8 + cc * 2 + x;
       if (r == 0) {
-        s_m[i] = sum.m[n][x];
+        s_m[i] = sum.m[n][x] * q[n].unit[x];
         s_l[i] = sum.l[n][x];
       }
 #pragma unroll
@@ -566,10 +574,11 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
   }
 }
 
-// The parts of a request, one block for a query row and head.
+// The parts of a request, one block for a query row and head: a thread a column.
 template <int NT>
 __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, int tokens) {
   constexpr int NQ = 8 * NT;
+  __shared__ float s_f[KV4_MAX_PARTS];
   const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ;
   const int h = blockIdx.x / total, row = blockIdx.x - h * total, b = blockIdx.y, d = threadIdx.x;
   const int chunk = row / NQ, len = min(max(a.seq_lens[b], 0), a.table_w * c.block);
@@ -577,13 +586,23 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, 
   const int tiles = end > 0 ? (end + tokens - 1) / tokens : 0, part = kv4_part(a, tiles);
   const int parts = max(1, (tiles + part - 1) / part);
   const long long at = ((long long)b * c.hkv * chunks + h * chunks + chunk) * a.splits * NQ + row - chunk * NQ;
-  float mm = -INFINITY, sum = 0.f, acc = 0.f;
-  for (int s = 0; s < parts; ++s) mm = fmaxf(mm, a.lse_part[at + s * NQ]);
-  for (int s = 0; s < parts; ++s) {
-    const float v = a.lse_part[at + s * NQ];
-    const float f = v == -INFINITY ? 0.f : exp2f(v - mm);
+  // every warp finds the maximum and the sum of the parts by itself
+  float mm = -INFINITY, sum = 0.f;
+  for (int s = d & 31; s < parts; s += 32) mm = fmaxf(mm, a.lse_part[at + s * NQ]);
+  mm = warp_max(mm);
+  for (int s = d & 31; s < parts; s += 32) {
+    const float v = a.lse_part[at + s * NQ], f = v == -INFINITY ? 0.f : exp2f(v - mm);
     sum += f;
-    acc += f == 0.f ? 0.f : f * a.o_part[(at + s * NQ) * c.d + d];
+    if (d < 32) s_f[s] = f;
+  }
+  sum = warp_sum(sum);
+  __syncthreads();
+  float acc = 0.f;
+  const float* o = a.o_part + at * c.d + d;
+#pragma unroll 8
+  for (int s = 0; s < parts; ++s) {
+    const float f = s_f[s], v = o[(long long)s * NQ * c.d];
+    acc += f == 0.f ? 0.f : f * v;
   }
   const int head = h * rep + row % rep, tok = row / rep;
   a.out[(((long long)b * a.rows + tok) * a.hq + head) * c.d + d] = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
@@ -606,8 +625,8 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   const int stride = gridDim.x * KV4_WARPS;
   if (blockIdx.x * KV4_WARPS >= tiles) return;
   uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
-  uint2* s_q = reinterpret_cast<uint2*>(smem + KV4_WARPS * KV4_STAGES * T::BYTES);      // [chunks][NG * 4][32]
-  float4* s_row = reinterpret_cast<float4*>(s_q + chunks * NG * 4 * 32);                 // [chunks][1 + NG / 2][4]: see below
+  uint4* s_q = reinterpret_cast<uint4*>(smem + KV4_WARPS * KV4_STAGES * T::BYTES);      // [chunks][NG][2][32]
+  float4* s_row = reinterpret_cast<float4*>(s_q + chunks * NG * 64);                     // [chunks][1 + NG / 2][4]: see below
   constexpr int ROW = 1 + (NG + 1) / 2;
   uint64_t* bar = bars + warp * KV4_STAGES;
   if (threadIdx.x == 0) abort_flag = 0;
@@ -629,15 +648,16 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) s_q[(ch * NG * 4 + g * 4 + s) * 32 + lane] = make_uint2(q.b[g][s][0], q.b[g][s][1]);
-    if (r == 0) {                   // of the rows 2 c and 2 c + 1: their sums, the unit, and then pairs of qs
+      for (int x = 0; x < 2; ++x)
+        s_q[(ch * NG * 2 + g * 2 + x) * 32 + lane] = make_uint4(q.b[g][2 * x][0], q.b[g][2 * x][1], q.b[g][2 * x + 1][0], q.b[g][2 * x + 1][1]);
+    if (r == 0) {                   // of the rows 2 c and 2 c + 1: their sums and units, and then pairs of qs
       float lse[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int row = ch * 8 + cc * 2 + x;
         lse[x] = row < total ? a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep] : INFINITY;
       }
-      s_row[(ch * ROW) * 4 + cc] = make_float4(lse[0], lse[1], q.unit * a.scale_log2, 0.f);
+      s_row[(ch * ROW) * 4 + cc] = make_float4(lse[0], lse[1], q.unit[0], q.unit[1]);
 #pragma unroll
       for (int g = 0; g < NG; g += 2)
         s_row[(ch * ROW + 1 + g / 2) * 4 + cc] = make_float4(q.qs[g][0], q.qs[g][1], g + 1 < NG ? q.qs[(g + 1) % NG][0] : 0.f, g + 1 < NG ? q.qs[(g + 1) % NG][1] : 0.f);
@@ -670,22 +690,23 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
         for (int g = 0; g < NG; ++g) {
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint2 v = s_q[(ch * NG * 4 + g * 4 + x) * 32 + lane];
-            const uint32_t qb[2] = {v.x, v.y};
-            kv4_mma(acc, f[g][x], qb);
+          for (int x = 0; x < 2; ++x) {
+            const uint4 v = s_q[(ch * NG * 2 + g * 2 + x) * 32 + lane];
+            const uint32_t b0[2] = {v.x, v.y}, b1[2] = {v.z, v.w};
+            kv4_mma(acc, f[g][2 * x], b0);
+            kv4_mma(acc, f[g][2 * x + 1], b1);
           }
           const float4 sums = s_row[(ch * ROW + 1 + g / 2) * 4 + cc];
           const float qs[2] = {g & 1 ? sums.z : sums.x, g & 1 ? sums.w : sums.y};
           const uint32_t word[2] = {k.sc[0][g], k.sc[1][g]};
-          kv4_score(s, acc, word, qs, row.z);
+          kv4_score(s, acc, word, qs);
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float p = ex2_fast(s[2 * e + x] - (x ? row.y : row.x));
-            if (edge || ch == chunks - 1) {                                // rows beyond the last, tokens that the row does not see
+            float p = ex2_fast(fmaf(s[2 * e + x], x ? row.w : row.z, -(x ? row.y : row.x)));
+            if (edge || (ch + 1) * 8 > total) {                            // rows beyond the last, tokens that the row does not see
               const int i = ch * 8 + cc * 2 + x;
               if (i >= total || t0 + r + 8 * e >= len - a.rows + 1 + i / rep) p = 0.f;
             }
@@ -750,7 +771,7 @@ template <int NG>
 static cudaError_t kv4_launch_weights(const Kv4Decode& a, const Kv4Cache& c, int B, int max_len, OmniStatus* st, cudaStream_t stream) {
   using T = Kv4Tile<NG, false>;
   const int total = a.rows * (a.hq / c.hkv), chunks = (total + 7) / 8;
-  const int bytes = KV4_WARPS * KV4_STAGES * T::BYTES + chunks * (NG * 4 * 32 * 8 + (1 + (NG + 1) / 2) * 4 * 16);
+  const int bytes = KV4_WARPS * KV4_STAGES * T::BYTES + chunks * (NG * 64 * 16 + (1 + (NG + 1) / 2) * 4 * 16);
   static int most[64] = {0};
   cudaError_t e = kv4_smem((const void*)kv4_weights_kernel<NG>, bytes, most);
   if (e != cudaSuccess) return e;
@@ -772,7 +793,7 @@ extern "C" int omni_kv4_decode(const void* q, long long q_row, int q_head, const
                                float scale, int max_len, int row_tile, int splits, int min_tiles, float* o_part, float* lse_part, void* out, float* lse,
                                float* weights, float decay, void* status, cudaStream_t stream) {
   const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
-  if (!kv4_shape_ok(c) || hq % hkv != 0 || rows < 1 || hkv > 65535 || B > 65535 || splits < 1 || splits > 65535 || min_tiles < 1 ||
+  if (!kv4_shape_ok(c) || hq % hkv != 0 || rows < 1 || hkv > 65535 || B > 65535 || splits < 1 || splits > KV4_MAX_PARTS || min_tiles < 1 ||
       (row_tile != 8 && (row_tile != 16 || d > 128)))
     return -1;
   if (weights != nullptr && (lse == nullptr || rows * (hq / hkv) > 256)) return -2;

@@ -278,7 +278,7 @@ def kv4_read(k_cache, v_cache, slots):
 def _parts(items, tiles, resident):
     """(most parts that a request is cut into, fewest tiles of one) for ``items`` passes over up to ``tiles`` tiles each, with
     ``resident`` blocks on each of the 148 SMs."""
-    return max(1, min(-(-2 * 148 * resident // items), -(-tiles // 4))), 4
+    return max(1, min(-(-148 * resident // items), -(-tiles // 4))), 4
 
 
 def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=None, weights=None, decay=1.0):

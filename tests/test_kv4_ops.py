@@ -231,6 +231,29 @@ def test_attention_of_any_magnitude(dev, q_scale, k_scale, v_scale, scale):
 
 
 @BOTH
+@pytest.mark.parametrize("outlier", [300.0, 3000.0, 65536.0])
+def test_queries_with_one_large_column(dev, outlier):
+    """A column that outweighs the others by far, with keys that are all alike there: the softmax goes by the other columns, which have
+    to keep their bits.  The large product is 4 outlier scale in an fp32 sum of some 20 steps (16 columns a step and a few more):
+    an error of 20 * 2^-24 of it at most, twice that in the weights; an error of half a step in an 8th bit of the other columns would
+    be over 100 times that for the first two."""
+    d, n, scale = 128, 200, 0.09
+    f = Filled(31, [n], 2, d, 16, dev)
+    f.k[0][:, :, 9] = 4.0
+    ops.kv4_write(f.k[0].to(dev), f.v[0].to(dev), f.slots[0].to(dev), f.k_cache, f.v_cache)
+    q = torch.randn(1, 12, d, generator=_gen(1))
+    q[:, ::2, 9] = outlier
+    q = q.bfloat16().to(dev)
+    w = torch.zeros(f.k_cache.shape[:3], device=dev)
+    ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, scale, weights=w, decay=0.0)
+    k = O.stored(f.k[0])[0]
+    blk, t = f.table[0].long()[torch.arange(n) // 16], torch.arange(n) % 16
+    for h in range(2):
+        p = torch.softmax(q[0, 6 * h:6 * h + 6].double().cpu() @ k[:, h].T * scale, -1).sum(0)
+        assert ((w.cpu()[blk, h, t].double() - p).abs() <= p * (1e-5 + 2 * 20 * 2.0 ** -24 * 4 * outlier * scale)).all()
+
+
+@BOTH
 def test_rising_scores(dev):
     """Scores that rise, fall and stand still along the cache by far more than what an exponential holds: the running maximum has to
     follow them."""
