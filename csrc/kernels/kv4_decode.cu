@@ -33,7 +33,7 @@
 namespace omni {
 
 constexpr int KV4_SITE_DECODE = 84, KV4_SITE_TILE = 85, KV4_SITE_WEIGHTS = 86;
-constexpr int KV4_WARPS = 4, KV4_STAGES = 2, KV4_MAX_PARTS = 512;
+constexpr int KV4_WARPS = 4, KV4_STAGES = 2, KV4_MAX_BLOCKS = 4096;
 
 struct Kv4Decode {
   const __nv_bfloat16* q;
@@ -47,9 +47,9 @@ struct Kv4Decode {
   float* weights;
   float decay;
   int piece;                        // tokens of a copy: the largest of 64, 32, 16 that divides the block
-  int splits, min_tiles;            // parts of a request, and the fewest tiles of one
-  float* o_part;                    // [B, Hkv, chunks, splits, 8 NT, d]
-  float* lse_part;                  // [B, Hkv, chunks, splits, 8 NT]
+  int min_tiles;                    // fewest tiles of a block's share; 0: a block takes one item, whole
+  float* o_part;                    // [blocks, 2, 8 NT, d]: what a block has of the item that it starts with, and of the one it ends with
+  float* lse_part;                  // [blocks, 2, 8 NT]
 };
 
 __device__ __forceinline__ int kv4_length(const Kv4Decode& a, int block, int b, OmniStatus* st) {
@@ -58,8 +58,48 @@ __device__ __forceinline__ int kv4_length(const Kv4Decode& a, int block, int b, 
   if (threadIdx.x == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, b);
   return a.table_w * block;
 }
-// tiles of a part of `tiles`
-__device__ __forceinline__ int kv4_part(const Kv4Decode& a, int tiles) { return max(a.min_tiles, (tiles + a.splits - 1) / a.splits); }
+// Work is cut into equal shares.  An item is a tile of query rows of a key/value head of a request; the items of a request one after the
+// other, requests one after the other, their tiles are numbered through, and block i of the grid takes the tiles from i * share on.  A
+// warp finds the tiles ahead of request `b`, and their total, in one pass over the lengths.
+__device__ __forceinline__ int kv4_tiles(const Kv4Decode& a, int block, int tokens, int b) {
+  return (min(max(a.seq_lens[b], 0), a.table_w * block) + tokens - 1) / tokens;
+}
+__device__ __forceinline__ long long kv4_warp_sum(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ long long kv4_ahead(const Kv4Decode& a, int block, int tokens, int items, int from, int to) {
+  long long n = 0;
+  for (int b = from + (threadIdx.x & 31); b < to; b += 32) n += kv4_tiles(a, block, tokens, b);
+  return kv4_warp_sum(n) * items;
+}
+__device__ __forceinline__ long long kv4_share(const Kv4Decode& a, long long total, int blocks) {
+  const long long even = (total + blocks - 1) / blocks;
+  return even > a.min_tiles ? even : a.min_tiles;
+}
+// Request of tile g, and the tiles ahead of it; -1 behind the last
+__device__ __forceinline__ int kv4_find(const Kv4Decode& a, int block, int tokens, int items, int B, long long g, long long& ahead) {
+  const int lane = threadIdx.x & 31;
+  ahead = 0;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const long long mine = b0 + lane < B ? (long long)kv4_tiles(a, block, tokens, b0 + lane) * items : 0;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, ahead + upto > g);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      ahead += __shfl_sync(0xffffffffu, upto - mine, l);
+      return b0 + l;
+    }
+    ahead += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return -1;
+}
 
 // The codes minus 8 of the nibbles I of both halves of a word, as an fp16 pair, exactly.  Behind the exponent of 1024 a code in bits
 // 0 .. 3 makes 1024 + code and one in bits 4 .. 7 makes 1024 + 16 code; the fp16 multiply-add that takes the offset off runs on
@@ -446,152 +486,190 @@ struct Kv4Sums {
 };
 
 template <int NG, int NT>
-__global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decode_kernel(Kv4Decode a, Kv4Cache c, OmniStatus* st) {
+__global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decode_kernel(Kv4Decode a, Kv4Cache c, int B, OmniStatus* st) {
   using T = Kv4Tile<NG, true>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[KV4_WARPS * KV4_STAGES];
   __shared__ int abort_flag;
   constexpr int D = NG * 64, NQ = 8 * NT;
-  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ;
-  const int h = blockIdx.x / chunks, chunk = blockIdx.x - h * chunks, split = blockIdx.y, b = blockIdx.z;
+  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ, items = c.hkv * chunks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
-  const int row0 = chunk * NQ;
-  const int len = kv4_length(a, c.block, b, st);
-  const int first_sees = len - a.rows + 1 + row0 / rep;                    // of the chunk's first and last rows
-  const int end = len - a.rows + 1 + (min(total, row0 + NQ) - 1) / rep;
-  const int tiles = end > 0 ? (end + T::TOKENS - 1) / T::TOKENS : 0;
-  const int part = kv4_part(a, tiles), begin_tile = split * part, end_tile = min(tiles, begin_tile + part);
-  if (begin_tile >= end_tile && split > 0) return;                         // the first part writes the zeros of rows that see nothing
-
   uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
   uint64_t* bar = bars + warp * KV4_STAGES;
   if (threadIdx.x == 0) abort_flag = 0;
   if (lane == 0) {
     for (int s = 0; s < KV4_STAGES; ++s) mbar_init(bar + s, 1);
     mbar_fence_init();
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_proxy_async_smem();
   }
   __syncthreads();
-  const int stop = min(end, end_tile * T::TOKENS);                         // first token behind this part
-  int tile = begin_tile + warp, next = tile;
-  Kv4Feed<NG, true> feed;
-  feed.init(a, c, b, h, tile, KV4_WARPS, stop, st);
-#pragma unroll
-  for (int s = 0; s < KV4_STAGES; ++s, next += KV4_WARPS)
-    if (next < end_tile) feed.start(a, c, min(T::TOKENS, (end - next * T::TOKENS + 15) & ~15), stop, stages + s * T::BYTES, bar + s, st);
+  asm volatile("griddepcontrol.launch_dependents;");
 
-  Kv4Query<NG> q[NT];
-  int sees[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    q[n].load(a, rep, b, h, row0 + n * 8 + r, total);
-#pragma unroll
-    for (int x = 0; x < 2; ++x) sees[n][x] = len - a.rows + 1 + min(row0 + n * 8 + cc * 2 + x, total - 1) / rep;
+  // this block's tiles, from item `item` of request `b` on
+  int b, item, tile0, n_tiles;
+  long long left;
+  if (a.min_tiles == 0) {
+    b = blockIdx.x / items;
+    item = blockIdx.x - b * items;
+    tile0 = 0;
+    n_tiles = kv4_tiles(a, c.block, T::TOKENS, b);
+    left = n_tiles;
+  } else {
+    const long long all = kv4_ahead(a, c.block, T::TOKENS, items, 0, B), share = kv4_share(a, all, gridDim.x), g = blockIdx.x * share;
+    long long ahead;
+    if (g >= all) return;
+    b = kv4_find(a, c.block, T::TOKENS, items, B, g, ahead);
+    n_tiles = kv4_tiles(a, c.block, T::TOKENS, b);
+    item = (int)((g - ahead) / n_tiles);
+    tile0 = (int)(g - ahead - (long long)item * n_tiles);
+    left = min(share, all - g);
   }
-  Kv4Sums<NG, NT> sum;
-  sum.clear();
-  int it = 0;
-  for (; tile < end_tile; tile += KV4_WARPS, next += KV4_WARPS, ++it) {
-    const int st_i = it % KV4_STAGES;
-    uint8_t* stage = stages + st_i * T::BYTES;
-    if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (it / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_TILE, tile))) break;
+  int uses = 0;                                                            // of this warp's stages so far
+  for (bool first = true;; first = false) {
+    const int h = item / chunks, row0 = (item - h * chunks) * NQ;
+    const int len = kv4_length(a, c.block, b, st);
+    const int first_sees = len - a.rows + 1 + row0 / rep;                  // of the item's first and last rows
+    const int end = len - a.rows + 1 + (min(total, row0 + NQ) - 1) / rep;
+    const int end_tile = (int)min((long long)n_tiles, tile0 + left);
+    const int stop = min(end, end_tile * T::TOKENS);                       // first token behind this part
+    const int stop_tile = stop > 0 ? (stop + T::TOKENS - 1) / T::TOKENS : 0;
+    int tile = tile0 + warp, next = tile;
+    Kv4Feed<NG, true> feed;
+    feed.init(a, c, b, h, tile, KV4_WARPS, stop, st);
+#pragma unroll
+    for (int s = 0; s < KV4_STAGES; ++s, next += KV4_WARPS) {
+      const int i = (uses + s) % KV4_STAGES;
+      if (next < stop_tile) feed.start(a, c, min(T::TOKENS, (end - next * T::TOKENS + 15) & ~15), stop, stages + i * T::BYTES, bar + i, st);
+    }
+    Kv4Query<NG> q[NT];
+    int sees[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      q[n].load(a, rep, b, h, row0 + n * 8 + r, total);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) sees[n][x] = len - a.rows + 1 + min(row0 + n * 8 + cc * 2 + x, total - 1) / rep;
+    }
+    Kv4Sums<NG, NT> sum;
+    sum.clear();
+    for (; tile < stop_tile; tile += KV4_WARPS, next += KV4_WARPS, ++uses) {
+      const int i = uses % KV4_STAGES;
+      uint8_t* stage = stages + i * T::BYTES;
+      if (!__all_sync(0xffffffffu, mbar_wait(bar + i, (uses / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_TILE, tile))) break;
 #pragma unroll 1
-    for (int sub = 0; sub < T::TOKENS / 16; sub += 2) {
-      const int t0 = tile * T::TOKENS + sub * 16;
-      if (t0 + 32 <= first_sees) sum.template add<false>(stage, sub, t0, end, sees, q);
-      else if (t0 < end) sum.template add<true>(stage, sub, t0, end, sees, q);
+      for (int sub = 0; sub < T::TOKENS / 16; sub += 2) {
+        const int t0 = tile * T::TOKENS + sub * 16;
+        if (t0 + 32 <= first_sees) sum.template add<false>(stage, sub, t0, end, sees, q);
+        else if (t0 < end) sum.template add<true>(stage, sub, t0, end, sees, q);
+      }
+      __syncwarp();                                                        // every lane has read the stage
+      if (next < stop_tile) feed.start(a, c, min(T::TOKENS, (end - next * T::TOKENS + 15) & ~15), stop, stage, bar + i, st);
     }
-    __syncwarp();                                                          // every lane has read the stage
-    if (next < end_tile) feed.start(a, c, min(T::TOKENS, (end - next * T::TOKENS + 15) & ~15), stop, stage, bar + st_i, st);
-  }
 
-  // ---- the sums over the lanes that share a query row, then over the warps
+    // ---- the sums over the lanes that share a query row, then over the warps
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        sum.l[n][x] += __shfl_xor_sync(0xffffffffu, sum.l[n][x], d);
+        for (int d = 4; d < 32; d <<= 1) {
+          sum.l[n][x] += __shfl_xor_sync(0xffffffffu, sum.l[n][x], d);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) sum.z[n][g][x] += __shfl_xor_sync(0xffffffffu, sum.z[n][g][x], d);
+          for (int g = 0; g < NG; ++g) sum.z[n][g][x] += __shfl_xor_sync(0xffffffffu, sum.z[n][g][x], d);
+        }
+    __syncthreads();
+    if (abort_flag != 0) {                                                 // copies may still be under way: leave the memory alone
+      if (threadIdx.x == 0) report_abort(&abort_flag, st);
+      for (int s = 0; s < KV4_STAGES; ++s) {
+        const int i = uses + s;                                            // what this warp has started and not seen: its phases
+        if (tile + s * KV4_WARPS < stop_tile) {
+          for (int k = 0; k < 1 << 16 && !mbar_try_wait(bar + i % KV4_STAGES, (i / KV4_STAGES) & 1); ++k) {}
+        }
       }
-  __syncthreads();
-  if (abort_flag != 0) {                                                   // copies may still be under way: leave the memory alone
-    if (threadIdx.x == 0) report_abort(&abort_flag, st);
-    for (int s = 0; s < KV4_STAGES; ++s) {
-      const int left = it + s;                                             // what this warp has started and not seen: its phases
-      if (tile + s * KV4_WARPS < end_tile) {
-        for (int i = 0; i < 1 << 16 && !mbar_try_wait(bar + left % KV4_STAGES, (left / KV4_STAGES) & 1); ++i) {}
+      return;
+    }
+    const float unit = sum.most * 0.0078125f;
+    float* s_o = reinterpret_cast<float*>(smem);                           // [warps][NQ][D]
+    float* s_m = s_o + KV4_WARPS * NQ * D;                                 // [warps][NQ], and the sums likewise
+    float* s_l = s_m + KV4_WARPS * NQ;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int i = warp * NQ + n * 8 + cc * 2 + x;
+        if (r == 0) {
+          s_m[i] = sum.m[n][x] * q[n].unit[x];
+          s_l[i] = sum.l[n][x];
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float2*>(s_o + (size_t)i * D + g * 64 + r * 8 + j * 2) =
+                make_float2(fmaf(sum.o[n][g][j][x], unit, sum.z[n][g][x]), fmaf(sum.o[n][g][j][x + 2], unit, sum.z[n][g][x]));
+      }
+    __syncthreads();
+    const bool whole = tile0 == 0 && end_tile == n_tiles;
+    for (int i = threadIdx.x; i < NQ * D; i += KV4_WARPS * 32) {
+      const int row = i / D, d = i - row * D;
+      if (row0 + row >= total) break;
+      float mm = -INFINITY, total_l = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < KV4_WARPS; ++w) mm = fmaxf(mm, s_m[w * NQ + row]);
+#pragma unroll
+      for (int w = 0; w < KV4_WARPS; ++w) {
+        const float mw = s_m[w * NQ + row];
+        const float f = mw == -INFINITY ? (s_l[w * NQ + row] == 0.f ? 0.f : 1.f) : ex2_fast(mw - mm);    // a sum without a maximum is NaN
+        total_l += s_l[w * NQ + row] * f;
+        acc += s_o[((size_t)w * NQ + row) * D + d] * f;
+      }
+      const float value = total_l == 0.f ? 0.f : acc / total_l, lse = total_l == 0.f ? -INFINITY : mm + __log2f(total_l);
+      if (whole) {
+        const int head = h * rep + (row0 + row) % rep, tok = (row0 + row) / rep;
+        a.out[(((long long)b * a.rows + tok) * a.hq + head) * D + d] = __float2bfloat16(value);
+        if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = lse;
+      } else {
+        const long long at = ((long long)blockIdx.x * 2 + (first ? 0 : 1)) * NQ + row;
+        a.o_part[at * D + d] = value;
+        if (d == 0) a.lse_part[at] = lse;
       }
     }
-    return;
-  }
-  const float unit = sum.most * 0.0078125f;
-  float* s_o = reinterpret_cast<float*>(smem);                             // [warps][NQ][D]
-  float* s_m = s_o + KV4_WARPS * NQ * D;                                   // [warps][NQ], and the sums likewise
-  float* s_l = s_m + KV4_WARPS * NQ;
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int i = warp * NQ + n * 8 + cc * 2 + x;
-      if (r == 0) {
-        s_m[i] = sum.m[n][x] * q[n].unit[x];
-        s_l[i] = sum.l[n][x];
-      }
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<float2*>(s_o + (size_t)i * D + g * 64 + r * 8 + j * 2) = 
-              make_float2(fmaf(sum.o[n][g][j][x], unit, sum.z[n][g][x]), fmaf(sum.o[n][g][j][x + 2], unit, sum.z[n][g][x]));
+    // ---- the next item
+    left -= end_tile - tile0;
+    if (left <= 0) return;
+    tile0 = 0;
+    if (++item == items) {
+      item = 0;
+      do n_tiles = kv4_tiles(a, c.block, T::TOKENS, ++b);                  // tiles are left, so there is a request that has some
+      while (n_tiles == 0);
     }
-  __syncthreads();
-  for (int i = threadIdx.x; i < NQ * D; i += KV4_WARPS * 32) {
-    const int row = i / D, d = i - row * D;
-    if (row0 + row >= total) break;
-    float mm = -INFINITY, total_l = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < KV4_WARPS; ++w) mm = fmaxf(mm, s_m[w * NQ + row]);
-#pragma unroll
-    for (int w = 0; w < KV4_WARPS; ++w) {
-      const float mw = s_m[w * NQ + row];
-      const float f = mw == -INFINITY ? (s_l[w * NQ + row] == 0.f ? 0.f : 1.f) : ex2_fast(mw - mm);      // a sum without a maximum is NaN
-      total_l += s_l[w * NQ + row] * f;
-      acc += s_o[((size_t)w * NQ + row) * D + d] * f;
-    }
-    const float value = total_l == 0.f ? 0.f : acc / total_l, lse = total_l == 0.f ? -INFINITY : mm + __log2f(total_l);
-    const int head = h * rep + (row0 + row) % rep, tok = (row0 + row) / rep;
-    if (a.splits == 1) {
-      a.out[(((long long)b * a.rows + tok) * a.hq + head) * D + d] = __float2bfloat16(value);
-      if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = lse;
-    } else {
-      const long long at = (((long long)b * gridDim.x + blockIdx.x) * a.splits + split) * NQ + row;
-      a.o_part[at * D + d] = value;
-      if (d == 0) a.lse_part[at] = lse;
-    }
+    fence_proxy_async_smem();                                              // the sums in shared memory come before the next copies
+    __syncthreads();
   }
 }
 
-// The parts of a request, one block for a query row and head: a thread a column.
+// Items that several blocks have worked on, and requests of no tokens: one block for a query row and head, a thread a column.
 template <int NT>
-__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, int tokens) {
+__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, int B, int blocks, int tokens) {
   constexpr int NQ = 8 * NT;
-  __shared__ float s_f[KV4_MAX_PARTS];
-  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ;
-  const int h = blockIdx.x / total, row = blockIdx.x - h * total, b = blockIdx.y, d = threadIdx.x;
-  const int chunk = row / NQ, len = min(max(a.seq_lens[b], 0), a.table_w * c.block);
-  const int end = len - a.rows + 1 + (min(total, chunk * NQ + NQ) - 1) / rep;
-  const int tiles = end > 0 ? (end + tokens - 1) / tokens : 0, part = kv4_part(a, tiles);
-  const int parts = max(1, (tiles + part - 1) / part);
-  const long long at = ((long long)b * c.hkv * chunks + h * chunks + chunk) * a.splits * NQ + row - chunk * NQ;
+  extern __shared__ float s_f[];                                           // [blocks]
+  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ, items = c.hkv * chunks;
+  const int h = blockIdx.x / total, row = blockIdx.x - h * total, b = blockIdx.y, d = threadIdx.x, lane = d & 31;
+  const int item = h * chunks + row / NQ, tiles = kv4_tiles(a, c.block, tokens, b);
+  const long long before = kv4_ahead(a, c.block, tokens, items, 0, b);
+  const long long share = kv4_share(a, before + kv4_ahead(a, c.block, tokens, items, b, B), blocks);
+  const long long g0 = before + (long long)item * tiles, g1 = g0 + tiles;
+  const int i0 = (int)(g0 / share), parts = tiles == 0 ? 0 : (int)((g1 - 1) / share) - i0 + 1;
+  // Every block waits, those without work too: a kernel that follows this one may then count on the one ahead of it being done.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (parts == 1) return;                                                  // written by its only block
+  const int first = g0 == (long long)i0 * share ? 0 : 1;                   // where the first of the blocks has its part
+  const long long at = ((long long)i0 * 2) * NQ + row % NQ;
   // every warp finds the maximum and the sum of the parts by itself
   float mm = -INFINITY, sum = 0.f;
-  for (int s = d & 31; s < parts; s += 32) mm = fmaxf(mm, a.lse_part[at + s * NQ]);
+  for (int s = lane; s < parts; s += 32) mm = fmaxf(mm, a.lse_part[at + (s == 0 ? first : 2 * s) * NQ]);
   mm = warp_max(mm);
-  for (int s = d & 31; s < parts; s += 32) {
-    const float v = a.lse_part[at + s * NQ], f = v == -INFINITY ? 0.f : exp2f(v - mm);
+  for (int s = lane; s < parts; s += 32) {
+    const float v = a.lse_part[at + (s == 0 ? first : 2 * s) * NQ], f = v == -INFINITY ? 0.f : exp2f(v - mm);
     sum += f;
     if (d < 32) s_f[s] = f;
   }
@@ -601,7 +679,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, 
   const float* o = a.o_part + at * c.d + d;
 #pragma unroll 8
   for (int s = 0; s < parts; ++s) {
-    const float f = s_f[s], v = o[(long long)s * NQ * c.d];
+    const float f = s_f[s], v = o[(long long)(s == 0 ? first : 2 * s) * NQ * c.d];
     acc += f == 0.f ? 0.f : f * v;
   }
   const int head = h * rep + row % rep, tok = row / rep;
@@ -623,10 +701,14 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
   const int len = kv4_length(a, c.block, b, st), tiles = (len + T::TOKENS - 1) / T::TOKENS;
   const int stride = gridDim.x * KV4_WARPS;
-  if (blockIdx.x * KV4_WARPS >= tiles) return;
+  if (blockIdx.x * KV4_WARPS >= tiles) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");                    // as in the join
+    return;
+  }
   uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
   uint4* s_q = reinterpret_cast<uint4*>(smem + KV4_WARPS * KV4_STAGES * T::BYTES);      // [chunks][NG][2][32]
   float4* s_row = reinterpret_cast<float4*>(s_q + chunks * NG * 64);                     // [chunks][1 + NG / 2][4]: see below
+  __shared__ float s_w[KV4_WARPS][T::TOKENS];
   constexpr int ROW = 1 + (NG + 1) / 2;
   uint64_t* bar = bars + warp * KV4_STAGES;
   if (threadIdx.x == 0) abort_flag = 0;
@@ -642,6 +724,18 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
 #pragma unroll
   for (int s = 0; s < KV4_STAGES; ++s, next += stride)
     if (next < tiles) feed.start(a, c, min(T::TOKENS, (len - next * T::TOKENS + 15) & ~15), len, stages + s * T::BYTES, bar + s, st);
+  // the places of the weights of a lane's tokens of the next tile
+  constexpr int EACH = T::TOKENS / 32;
+  int place[EACH];
+  auto look = [&](int of) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int t = of * T::TOKENS + i * 32 + lane;
+      place[i] = of < tiles && t < len ? a.table[(long long)b * a.table_ld + t / c.block] : -1;
+    }
+  };
+  look(tile);
+  asm volatile("griddepcontrol.wait;" ::: "memory");                      // the sums are there
   for (int ch = warp; ch < chunks; ch += KV4_WARPS) {
     Kv4Query<NG> q;
     q.load(a, rep, b, h, ch * 8 + r, total);
@@ -668,6 +762,15 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   for (; tile < tiles; tile += stride, next += stride, ++it) {
     const int st_i = it % KV4_STAGES;
     uint8_t* stage = stages + st_i * T::BYTES;
+    float* to[EACH];
+    float old[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int t = tile * T::TOKENS + i * 32 + lane;
+      to[i] = place[i] >= 0 && place[i] < c.blocks ? a.weights + ((long long)place[i] * c.hkv + h) * c.block + t % c.block : nullptr;
+      old[i] = to[i] != nullptr && a.decay != 0.f ? *to[i] : 0.f;
+    }
+    look(tile + stride);
     if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (it / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_WEIGHTS, tile))) break;
 #pragma unroll 1
     for (int u = 0; u < T::TOKENS / 16; ++u) {
@@ -717,16 +820,13 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
       for (int e = 0; e < 2; ++e) {
         w[e] += __shfl_xor_sync(0xffffffffu, w[e], 1);
         w[e] += __shfl_xor_sync(0xffffffffu, w[e], 2);
-        const int t = t0 + r + 8 * e;
-        if (cc == 0 && t < len) {
-          const int at = a.table[(long long)b * a.table_ld + t / c.block];
-          if (at >= 0 && at < c.blocks) {
-            float* to = a.weights + ((long long)at * c.hkv + h) * c.block + t % c.block;
-            *to = a.decay == 0.f ? w[e] : fmaf(a.decay, *to, w[e]);
-          }
-        }
+        if (cc == 0) s_w[warp][u * 16 + r + 8 * e] = w[e];
       }
     }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (to[i] != nullptr) *to[i] = a.decay == 0.f ? s_w[warp][i * 32 + lane] : fmaf(a.decay, old[i], s_w[warp][i * 32 + lane]);
     __syncwarp();
     if (next < tiles) feed.start(a, c, min(T::TOKENS, (len - next * T::TOKENS + 15) & ~15), len, stage, bar + st_i, st);
   }
@@ -752,19 +852,36 @@ static cudaError_t kv4_smem(const void* kernel, int bytes, int (&most)[64]) {
   return e;
 }
 
+// A launch that may begin while the kernel ahead of it ends; it waits for that one's results itself.
+template <typename... Args>
+static cudaError_t kv4_follow(void (*kernel)(Args...), dim3 grid, int threads, int bytes, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 template <int NG, int NT>
-static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, OmniStatus* st, cudaStream_t stream) {
+static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int blocks, OmniStatus* st, cudaStream_t stream) {
   using T = Kv4Tile<NG, true>;
   constexpr int merge = KV4_WARPS * 8 * NT * (NG * 64 + 2) * 4, stages = KV4_WARPS * KV4_STAGES * T::BYTES, bytes = merge > stages ? merge : stages;
   const int total = a.rows * (a.hq / c.hkv), chunks = (total + 8 * NT - 1) / (8 * NT);
+  const long long grid = a.min_tiles == 0 ? (long long)B * c.hkv * chunks : blocks;
+  if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   static int most[64] = {0};
   cudaError_t e = kv4_smem((const void*)kv4_decode_kernel<NG, NT>, bytes, most);
   if (e != cudaSuccess) return e;
-  kv4_decode_kernel<NG, NT><<<dim3(c.hkv * chunks, a.splits, B), KV4_WARPS * 32, bytes, stream>>>(a, c, st);
+  kv4_decode_kernel<NG, NT><<<(unsigned)grid, KV4_WARPS * 32, bytes, stream>>>(a, c, B, st);
   e = cudaGetLastError();
-  if (e != cudaSuccess || a.splits == 1) return e;
-  kv4_join_kernel<NT><<<dim3(c.hkv * total, B), c.d, 0, stream>>>(a, c, T::TOKENS);
-  return cudaGetLastError();
+  if (e != cudaSuccess || a.min_tiles == 0) return e;
+  return kv4_follow(kv4_join_kernel<NT>, dim3(c.hkv * total, B), c.d, blocks * 4, stream, a, c, B, blocks, (int)T::TOKENS);
 }
 
 template <int NG>
@@ -776,36 +893,37 @@ static cudaError_t kv4_launch_weights(const Kv4Decode& a, const Kv4Cache& c, int
   cudaError_t e = kv4_smem((const void*)kv4_weights_kernel<NG>, bytes, most);
   if (e != cudaSuccess) return e;
   const long long tiles = (max_len + T::TOKENS - 1) / T::TOKENS, items = (long long)B * c.hkv;
-  long long parts = (148 * 3 * 2 + items - 1) / items;
+  long long parts = 148 * 3 / items;
   if (parts > (tiles + KV4_WARPS - 1) / KV4_WARPS) parts = (tiles + KV4_WARPS - 1) / KV4_WARPS;
   if (parts < 1) parts = 1;
-  kv4_weights_kernel<NG><<<dim3((unsigned)parts, c.hkv, B), KV4_WARPS * 32, bytes, stream>>>(a, c, st);
-  return cudaGetLastError();
+  return kv4_follow(kv4_weights_kernel<NG>, dim3((unsigned)parts, c.hkv, B), KV4_WARPS * 32, bytes, stream, a, c, st);
 }
 
 }  // namespace omni
 
 using namespace omni;
 
-// row_tile: query rows that share a pass over the cache, 8, or 16 for d <= 128.  o_part and lse_part are sized by it.
+// row_tile: query rows that share a pass over the cache, 8, or 16 for d <= 128.  min_tiles 0: a block for every item (a row_tile of a
+// key/value head of a request); else `blocks_at_once` blocks share all tiles of 64 tokens (32 for d = 256) equally, at least min_tiles each,
+// and o_part [blocks_at_once, 2, row_tile, d] and lse_part [blocks_at_once, 2, row_tile] take what they have of shared items.
 extern "C" int omni_kv4_decode(const void* q, long long q_row, int q_head, const void* k_cache, const void* v_cache, long long blocks, int block,
                                int hkv, int d, const int* table, int table_ld, int table_w, const int* seq_lens, int B, int rows, int hq,
-                               float scale, int max_len, int row_tile, int splits, int min_tiles, float* o_part, float* lse_part, void* out, float* lse,
+                               float scale, int max_len, int row_tile, int blocks_at_once, int min_tiles, float* o_part, float* lse_part, void* out, float* lse,
                                float* weights, float decay, void* status, cudaStream_t stream) {
   const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
-  if (!kv4_shape_ok(c) || hq % hkv != 0 || rows < 1 || hkv > 65535 || B > 65535 || splits < 1 || splits > KV4_MAX_PARTS || min_tiles < 1 ||
+  if (!kv4_shape_ok(c) || hq % hkv != 0 || rows < 1 || hkv > 65535 || B > 65535 || min_tiles < 0 ||
       (row_tile != 8 && (row_tile != 16 || d > 128)))
     return -1;
   if (weights != nullptr && (lse == nullptr || rows * (hq / hkv) > 256)) return -2;
-  if (splits > 1 && (o_part == nullptr || lse_part == nullptr)) return -3;
+  if (min_tiles > 0 && (o_part == nullptr || lse_part == nullptr || blocks_at_once < 1 || blocks_at_once > KV4_MAX_BLOCKS)) return -3;
   if (B <= 0) return 0;
   const Kv4Decode a = {(const __nv_bfloat16*)q, q_row, q_head, table, seq_lens, table_ld, table_w, rows, hq, scale * 1.4426950408889634f,
-                       (__nv_bfloat16*)out, lse, weights, decay, block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16, splits, min_tiles, o_part, lse_part};
+                       (__nv_bfloat16*)out, lse, weights, decay, block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16, min_tiles, o_part, lse_part};
   OmniStatus* st = (OmniStatus*)status;
   const bool wide = row_tile == 16;
-  cudaError_t e = d == 64    ? wide ? kv4_launch<1, 2>(a, c, B, st, stream) : kv4_launch<1, 1>(a, c, B, st, stream)
-                  : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, st, stream) : kv4_launch<2, 1>(a, c, B, st, stream)
-                             : kv4_launch<4, 1>(a, c, B, st, stream);
+  cudaError_t e = d == 64    ? wide ? kv4_launch<1, 2>(a, c, B, blocks_at_once, st, stream) : kv4_launch<1, 1>(a, c, B, blocks_at_once, st, stream)
+                  : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, blocks_at_once, st, stream) : kv4_launch<2, 1>(a, c, B, blocks_at_once, st, stream)
+                             : kv4_launch<4, 1>(a, c, B, blocks_at_once, st, stream);
   if (e != cudaSuccess || weights == nullptr) return (int)e;
   e = d == 64 ? kv4_launch_weights<1>(a, c, B, max_len, st, stream) : d == 128 ? kv4_launch_weights<2>(a, c, B, max_len, st, stream)
                                                                               : kv4_launch_weights<4>(a, c, B, max_len, st, stream);

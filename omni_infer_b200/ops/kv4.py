@@ -275,10 +275,12 @@ def kv4_read(k_cache, v_cache, slots):
     return k, v
 
 
-def _parts(items, tiles, resident):
-    """(most parts that a request is cut into, fewest tiles of one) for ``items`` passes over up to ``tiles`` tiles each, with
-    ``resident`` blocks on each of the 148 SMs."""
-    return max(1, min(-(-148 * resident // items), -(-tiles // 4))), 4
+def _blocks(items, tiles, resident):
+    """(blocks, fewest tiles of one) for ``items`` passes over up to ``tiles`` tiles each, with ``resident`` blocks on each of the 148
+    SMs; 0 tiles: a block takes a pass, whole."""
+    if tiles <= 12:
+        return 0, 0
+    return min(148 * resident, -(-items * tiles // 4)), 4
 
 
 def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=None, weights=None, decay=1.0):
@@ -310,14 +312,15 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
         longest = width * block if max_seq_len is None else min(max_seq_len, width * block)
         tile = 16 if d <= 128 and total > 8 else 8
         items = B * hkv * -(-total // tile)
-        splits, min_tiles = _parts(items, -(-longest // (32 if d == 256 else 64)), 3 if tile * d <= 1024 else 2)
+        blocks_at_once, min_tiles = _blocks(items, -(-longest // (32 if d == 256 else 64)), 3 if tile * d <= 1024 else 2)
         lse = torch.empty(T * hq, dtype=torch.float32, device=q.device) if weights is not None else None
         o_part = lse_part = None
-        if splits > 1:
-            part = torch.empty(items * splits * tile * (d + 1), dtype=torch.float32, device=q.device)
-            o_part, lse_part = part, part[items * splits * tile * d:]
+        if min_tiles:
+            n = blocks_at_once * 2 * tile
+            o_part = torch.empty(n * (d + 1), dtype=torch.float32, device=q.device)
+            lse_part = o_part[n * d:]
         _call("omni_kv4_decode", q.device, _p(q), q.stride(0), q.stride(1), _p(k_cache), _p(v_cache), blocks, block, hkv, d, _p(block_table),
-              block_table.stride(0), width, _p(seq_lens), B, T // B, hq, scale, longest, tile, splits, min_tiles, _p(o_part), _p(lse_part), _p(out), _p(lse), _p(weights), decay)
+              block_table.stride(0), width, _p(seq_lens), B, T // B, hq, scale, longest, tile, blocks_at_once, min_tiles, _p(o_part), _p(lse_part), _p(out), _p(lse), _p(weights), decay)
     return out
 
 
