@@ -38,7 +38,7 @@ constexpr int KV4_WARPS = 4, KV4_STAGES = 2, KV4_MAX_BLOCKS = 4096;
 struct Kv4Decode {
   const __nv_bfloat16* q;
   long long q_row;
-  int q_head;
+  int q_head, q_wide;               // q_wide: rows and heads start on 16 bytes
   const int *table, *seq_lens;
   int table_ld, table_w, rows, hq;
   float scale_log2;
@@ -168,7 +168,8 @@ struct Kv4Tile {
 };
 
 // The copies of a warp's tiles: lane l copies one kind of data (a plane of codes, the scales) of one run of `piece` tokens of a tile,
-// which lies in one block.  Block ids are fetched a tile ahead of their use.
+// which lies in one block.  The block ids of 32 runs are fetched by one load, another 32 runs ahead of their use: with the copies of
+// all warps under way, a load that is waited for takes microseconds.
 template <int NG, bool VALUES>
 struct Kv4Feed {
   using T = Kv4Tile<NG, VALUES>;
@@ -176,11 +177,24 @@ struct Kv4Feed {
   long long blk_bytes;
   const int* table;
   int tok_bytes, dst, run;          // bytes a token, place in the stage, first token of the run in the tile (TOKENS: no copy)
-  int t, page, off, step, step_page, step_off;
-  int blk;
+  int off, step, step_off;          // token of the run in its block; tokens from one tile to the next, and what they are in a block
+  int ids, ids_next;                // block ids of run lane % runs of step lane / runs, of these steps and the next ones
+  int at, ahead;                    // steps of `ids` behind us; first token of the tile that ids_next starts with
+  int runs;
 
-  __device__ __forceinline__ void init(const Kv4Decode& a, const Kv4Cache& c, int b, int h, int tile, int stride, int end, OmniStatus* st) {
+  __device__ __forceinline__ int fetch(const Kv4Decode& a, const Kv4Cache& c, int first, int end) const {
+    const int lane = threadIdx.x & 31, t = first + lane / runs * step + lane % runs * a.piece;
+    return t < end && lane % runs * a.piece < T::TOKENS ? table[t / c.block] : -1;
+  }
+  __device__ __forceinline__ void init(const Kv4Decode& a, const Kv4Cache& c, int b, int h, int tile, int stride, int end) {
     const int lane = threadIdx.x & 31, kind = lane % T::KINDS;
+    table = a.table + (long long)b * a.table_ld;
+    step = stride * T::TOKENS;
+    runs = a.piece >= T::TOKENS ? 1 : T::TOKENS / a.piece;
+    at = 0;
+    ids = fetch(a, c, tile * T::TOKENS, end);
+    ahead = tile * T::TOKENS + 32 / runs * step;
+    ids_next = fetch(a, c, ahead, end);
     run = min(lane / T::KINDS * a.piece, T::TOKENS);
     const bool values = VALUES && ((kind >= T::PLANES && kind < 2 * T::PLANES) || kind == 2 * T::PLANES + 1);
     const bool scales = kind >= (VALUES ? 2 : 1) * T::PLANES;
@@ -189,38 +203,28 @@ struct Kv4Feed {
     base = (values ? c.v : c.k) + c.at(0, h) + (scales ? c.block * (32 * NG) : plane * c.block * (32 * T::PER));
     dst = scales ? (values ? T::VS0 : T::KS0) + run * (4 * NG) : (values ? T::V0 : 0) + (plane * T::TOKENS + run) * (32 * T::PER);
     blk_bytes = c.hkv * c.piece();
-    table = a.table + (long long)b * a.table_ld;
-    step = stride * T::TOKENS;
-    step_page = step / c.block;
-    step_off = step - step_page * c.block;
-    t = tile * T::TOKENS + run;
-    page = t / c.block;
-    off = t - page * c.block;
-    fetch(c, end, st);
-  }
-  __device__ __forceinline__ void fetch(const Kv4Cache& c, int end, OmniStatus* st) {
-    blk = -1;
-    if (run < T::TOKENS && t < end) {
-      blk = table[page];
-      if (blk < 0 || blk >= c.blocks) {
-        report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, page);
-        blk = 0;                    // in bounds; the result is reported as wrong
-      }
-    }
+    step_off = step % c.block;
+    off = (tile * T::TOKENS + run) % c.block;
   }
   // Start the copies of the tile in turn, `tokens` of it (a multiple of 16), and go on to the next one
   __device__ __forceinline__ void start(const Kv4Decode& a, const Kv4Cache& c, int tokens, int end, uint8_t* stage, uint64_t* bar, OmniStatus* st) {
     if ((threadIdx.x & 31) == 0) mbar_expect_tx(bar, tokens * T::TOKEN_BYTES);
-    __syncwarp();
-    if (blk >= 0) kv4_bulk(smem_u32(stage) + dst, base + blk * blk_bytes + off * tok_bytes, min(a.piece, tokens - run) * tok_bytes, bar);
-    t += step;
-    page += step_page;
-    off += step_off;
-    if (off >= c.block) {
-      off -= c.block;
-      ++page;
+    int blk = __shfl_sync(0xffffffffu, ids, at * runs + (threadIdx.x & 31) / T::KINDS % runs);
+    if (run < tokens) {
+      if (blk < 0 || blk >= c.blocks) {
+        report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, blk);
+        blk = 0;                    // in bounds; the result is reported as wrong
+      }
+      kv4_bulk(smem_u32(stage) + dst, base + blk * blk_bytes + off * tok_bytes, min(a.piece, tokens - run) * tok_bytes, bar);
     }
-    fetch(c, end, st);
+    off += step_off;
+    if (off >= c.block) off -= c.block;
+    if (++at == 32 / runs) {
+      at = 0;
+      ids = ids_next;
+      ahead += 32 / runs * step;
+      ids_next = fetch(a, c, ahead, end);
+    }
   }
 };
 
@@ -231,41 +235,59 @@ template <int NG>
 struct Kv4Query {
   uint32_t b[NG][4][2];
   float qs[NG][2], unit[2];
-  __device__ __forceinline__ void load(const Kv4Decode& a, int rep, int b0, int h, int r, int total) {
+  // pairs of neighbouring columns as they are
+  static __device__ __forceinline__ void fetch(const Kv4Decode& a, int rep, int b0, int h, int r, int total, uint32_t (&w)[NG][8]) {
     const int c = threadIdx.x & 3;
     const __nv_bfloat16* q = a.q + ((long long)b0 * a.rows + r / rep) * a.q_row + (long long)(h * rep + r % rep) * a.q_head + c * 16;
+    if (r >= total) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[g][i] = 0u;
+    } else if (a.q_wide) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(q + g * 64 + i * 8);
+          w[g][4 * i] = v.x; w[g][4 * i + 1] = v.y; w[g][4 * i + 2] = v.z; w[g][4 * i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          w[g][i] = (uint32_t)__bfloat16_as_ushort(q[g * 64 + 2 * i]) | (uint32_t)__bfloat16_as_ushort(q[g * 64 + 2 * i + 1]) << 16;
+    }
+  }
+  __device__ __forceinline__ void make(const uint32_t (&w)[NG][8], float scale_log2) {
+    const int c = threadIdx.x & 3;
     float most = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int at = g * 64 + (s >> 1) * 8 + (s & 1) * 2 + e;
-          uint32_t v = 0u;
-          if (r < total) v = (uint32_t)__bfloat16_as_ushort(q[at]) | (uint32_t)__bfloat16_as_ushort(q[at + 4]) << 16;
-          b[g][s][e] = v;
-          most = fmaxf(most, fmaxf(fabsf(__uint_as_float(v << 16)), fabsf(__uint_as_float(v & 0xffff0000u))));
-        }
+      for (int i = 0; i < 8; ++i)
+        most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[g][i] << 16)), fabsf(__uint_as_float(w[g][i] & 0xffff0000u))));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     // exponent of the factor: 13 - that of the largest, within what a factor and its inverse can be
     const int e = min(max(13 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100);
-    const float up = copysignf(__uint_as_float((uint32_t)(127 + e) << 23), a.scale_log2);
-    const float un = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23), 0x1p-120f);
+    const float up = copysignf(__uint_as_float((uint32_t)(127 + e) << 23), scale_log2);
+    const float un = fmaxf(fabsf(scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23), 0x1p-120f);
     unit[0] = __shfl_sync(0xffffffffu, un, c * 8);
     unit[1] = __shfl_sync(0xffffffffu, un, c * 8 + 4);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float x = 0.f;
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          const float lo = __uint_as_float(b[g][s][e2] << 16) * up, hi = __uint_as_float(b[g][s][e2] & 0xffff0000u) * up;
-          b[g][s][e2] = kv4_pack(lo, hi);
-          x += lo + hi;
-        }
+      for (int s = 0; s < 4; ++s) {                                        // columns i, i + 4 and i + 1, i + 5 of a word, i = 2 (s & 1)
+        const uint32_t u = w[g][(s >> 1) * 4 + (s & 1)], v = w[g][(s >> 1) * 4 + (s & 1) + 2];
+        const float u0 = __uint_as_float(u << 16) * up, u1 = __uint_as_float(u & 0xffff0000u) * up;
+        const float v0 = __uint_as_float(v << 16) * up, v1 = __uint_as_float(v & 0xffff0000u) * up;
+        b[g][s][0] = kv4_pack(u0, v0);
+        b[g][s][1] = kv4_pack(u1, v1);
+        x += (u0 + v0) + (u1 + v1);
+      }
       x += __shfl_xor_sync(0xffffffffu, x, 1);
       x += __shfl_xor_sync(0xffffffffu, x, 2);
       qs[g][0] = __shfl_sync(0xffffffffu, x, c * 8);
@@ -535,7 +557,10 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     const int stop_tile = stop > 0 ? (stop + T::TOKENS - 1) / T::TOKENS : 0;
     int tile = tile0 + warp, next = tile;
     Kv4Feed<NG, true> feed;
-    feed.init(a, c, b, h, tile, KV4_WARPS, stop, st);
+    feed.init(a, c, b, h, tile, KV4_WARPS, stop);
+    uint32_t raw[NT][NG][8];                                               // asked for ahead of the copies, which would hold them up
+#pragma unroll
+    for (int n = 0; n < NT; ++n) Kv4Query<NG>::fetch(a, rep, b, h, row0 + n * 8 + r, total, raw[n]);
 #pragma unroll
     for (int s = 0; s < KV4_STAGES; ++s, next += KV4_WARPS) {
       const int i = (uses + s) % KV4_STAGES;
@@ -545,7 +570,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     int sees[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      q[n].load(a, rep, b, h, row0 + n * 8 + r, total);
+      q[n].make(raw[n], a.scale_log2);
 #pragma unroll
       for (int x = 0; x < 2; ++x) sees[n][x] = len - a.rows + 1 + min(row0 + n * 8 + cc * 2 + x, total - 1) / rep;
     }
@@ -609,28 +634,50 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
       }
     __syncthreads();
     const bool whole = tile0 == 0 && end_tile == n_tiles;
-    for (int i = threadIdx.x; i < NQ * D; i += KV4_WARPS * 32) {
-      const int row = i / D, d = i - row * D;
-      if (row0 + row >= total) break;
-      float mm = -INFINITY, total_l = 0.f, acc = 0.f;
+    if (threadIdx.x < NQ) {                                                // a warp's factor in place of its maximum; 1 / sum and sum
+      const int row = threadIdx.x;
+      float mm = -INFINITY, total_l = 0.f;
 #pragma unroll
       for (int w = 0; w < KV4_WARPS; ++w) mm = fmaxf(mm, s_m[w * NQ + row]);
 #pragma unroll
       for (int w = 0; w < KV4_WARPS; ++w) {
-        const float mw = s_m[w * NQ + row];
-        const float f = mw == -INFINITY ? (s_l[w * NQ + row] == 0.f ? 0.f : 1.f) : ex2_fast(mw - mm);    // a sum without a maximum is NaN
-        total_l += s_l[w * NQ + row] * f;
-        acc += s_o[((size_t)w * NQ + row) * D + d] * f;
+        const float mw = s_m[w * NQ + row], lw = s_l[w * NQ + row];
+        const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2_fast(mw - mm);       // a sum without a maximum is NaN
+        s_m[w * NQ + row] = f;
+        total_l += lw * f;
       }
-      const float value = total_l == 0.f ? 0.f : acc / total_l, lse = total_l == 0.f ? -INFINITY : mm + __log2f(total_l);
+      s_l[row] = total_l == 0.f ? 0.f : 1.f / total_l;
+      const float lse = total_l == 0.f ? -INFINITY : mm + __log2f(total_l);
+      if (row0 + row < total) {
+        const int head = h * rep + (row0 + row) % rep, tok = (row0 + row) / rep;
+        if (!whole) a.lse_part[((long long)blockIdx.x * 2 + (first ? 0 : 1)) * NQ + row] = lse;
+        else if (a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = lse;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < NQ * D / 4; i += KV4_WARPS * 32) {
+      const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
+      if (row0 + row >= total) break;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < KV4_WARPS; ++w) {
+        const float f = s_m[w * NQ + row];
+        const float4 v = *reinterpret_cast<const float4*>(s_o + ((size_t)w * NQ + row) * D + d);
+        acc[0] = fmaf(v.x, f, acc[0]);
+        acc[1] = fmaf(v.y, f, acc[1]);
+        acc[2] = fmaf(v.z, f, acc[2]);
+        acc[3] = fmaf(v.w, f, acc[3]);
+      }
+      const float by = s_l[row];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[x] = by == 0.f ? 0.f : acc[x] * by;
       if (whole) {
         const int head = h * rep + (row0 + row) % rep, tok = (row0 + row) / rep;
-        a.out[(((long long)b * a.rows + tok) * a.hq + head) * D + d] = __float2bfloat16(value);
-        if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = lse;
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0], acc[1]), hi = __floats2bfloat162_rn(acc[2], acc[3]);
+        *reinterpret_cast<uint2*>(a.out + (((long long)b * a.rows + tok) * a.hq + head) * D + d) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
       } else {
-        const long long at = ((long long)blockIdx.x * 2 + (first ? 0 : 1)) * NQ + row;
-        a.o_part[at * D + d] = value;
-        if (d == 0) a.lse_part[at] = lse;
+        *reinterpret_cast<float4*>(a.o_part + (((long long)blockIdx.x * 2 + (first ? 0 : 1)) * NQ + row) * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       }
     }
     // ---- the next item
@@ -720,7 +767,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   __syncthreads();
   int tile = blockIdx.x * KV4_WARPS + warp, next = tile;
   Kv4Feed<NG, false> feed;
-  feed.init(a, c, b, h, tile, stride, len, st);
+  feed.init(a, c, b, h, tile, stride, len);
 #pragma unroll
   for (int s = 0; s < KV4_STAGES; ++s, next += stride)
     if (next < tiles) feed.start(a, c, min(T::TOKENS, (len - next * T::TOKENS + 15) & ~15), len, stages + s * T::BYTES, bar + s, st);
@@ -738,7 +785,9 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   asm volatile("griddepcontrol.wait;" ::: "memory");                      // the sums are there
   for (int ch = warp; ch < chunks; ch += KV4_WARPS) {
     Kv4Query<NG> q;
-    q.load(a, rep, b, h, ch * 8 + r, total);
+    uint32_t raw[NG][8];
+    Kv4Query<NG>::fetch(a, rep, b, h, ch * 8 + r, total, raw);
+    q.make(raw, a.scale_log2);
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -917,7 +966,8 @@ extern "C" int omni_kv4_decode(const void* q, long long q_row, int q_head, const
   if (weights != nullptr && (lse == nullptr || rows * (hq / hkv) > 256)) return -2;
   if (min_tiles > 0 && (o_part == nullptr || lse_part == nullptr || blocks_at_once < 1 || blocks_at_once > KV4_MAX_BLOCKS)) return -3;
   if (B <= 0) return 0;
-  const Kv4Decode a = {(const __nv_bfloat16*)q, q_row, q_head, table, seq_lens, table_ld, table_w, rows, hq, scale * 1.4426950408889634f,
+  const int wide_q = (uintptr_t)q % 16 == 0 && q_row % 8 == 0 && q_head % 8 == 0;
+  const Kv4Decode a = {(const __nv_bfloat16*)q, q_row, q_head, wide_q, table, seq_lens, table_ld, table_w, rows, hq, scale * 1.4426950408889634f,
                        (__nv_bfloat16*)out, lse, weights, decay, block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16, min_tiles, o_part, lse_part};
   OmniStatus* st = (OmniStatus*)status;
   const bool wide = row_tile == 16;
