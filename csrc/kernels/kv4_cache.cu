@@ -293,67 +293,98 @@ static int kv4_log2(int x) {
 
 using namespace omni;
 
-extern "C" int omni_kv4_write(const void* k, long long k_row, int k_head, const void* v, long long v_row, int v_head, const long long* slots,
-                              long long n, void* k_cache, void* v_cache, long long blocks, int block, int hkv, int d, float* weights,
-                              int* positions, const long long* token_positions, void* status, cudaStream_t stream) {
-  const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
+// The calls take their arguments in a block, as the caller packs them: a call with thirty arguments of their own costs more than the
+// launch.  8-byte fields come first, so that there are no gaps.
+struct Kv4WriteArgs {
+  const void *k, *v;
+  const long long* slots;
+  void *k_cache, *v_cache;
+  float* weights;
+  int* positions;
+  const long long* token_positions;
+  long long k_row, v_row, n, blocks;
+  int k_head, v_head, block, hkv, d, reserved;
+};
+extern "C" int omni_kv4_write(const Kv4WriteArgs* p, void* status, cudaStream_t stream) {
+  const Kv4Cache c = {(uint8_t*)p->k_cache, (uint8_t*)p->v_cache, p->blocks, p->block, p->hkv, p->d};
   if (!kv4_shape_ok(c)) return -1;
-  if ((positions == nullptr) != (token_positions == nullptr)) return -2;
-  if (n <= 0) return 0;
+  if ((p->positions == nullptr) != (p->token_positions == nullptr)) return -2;
+  if (p->n <= 0) return 0;
   Kv4Rows a = {};
-  a.k = (const __nv_bfloat16*)k;
-  a.v = (const __nv_bfloat16*)v;
-  a.k_row = k_row;
-  a.v_row = v_row;
-  a.k_head = k_head;
-  a.v_head = v_head;
-  a.slots = slots;
-  a.n = n;
-  a.weights = weights;
-  a.positions = positions;
-  a.token_positions = token_positions;
-  const int wl = kv4_log2(d / 8);
-  const long long grid = (((n * hkv * 2) << wl) + 255) / 256;
+  a.k = (const __nv_bfloat16*)p->k;
+  a.v = (const __nv_bfloat16*)p->v;
+  a.k_row = p->k_row;
+  a.v_row = p->v_row;
+  a.k_head = p->k_head;
+  a.v_head = p->v_head;
+  a.slots = p->slots;
+  a.n = p->n;
+  a.weights = p->weights;
+  a.positions = p->positions;
+  a.token_positions = p->token_positions;
+  const int wl = kv4_log2(p->d / 8);
+  const long long grid = (((p->n * p->hkv * 2) << wl) + 255) / 256;
   if (grid > 0x7fffffffll) return -3;
-  const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && (k_row | v_row) % 8 == 0 && (k_head | v_head) % 8 == 0;
+  const bool vec = ((uintptr_t)p->k | (uintptr_t)p->v) % 16 == 0 && (p->k_row | p->v_row) % 8 == 0 && (p->k_head | p->v_head) % 8 == 0;
   if (vec) kv4_write_kernel<true><<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
   else kv4_write_kernel<false><<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
   return (int)cudaGetLastError();
 }
 
-extern "C" int omni_kv4_read(const void* k_cache, const void* v_cache, long long blocks, int block, int hkv, int d, const long long* slots,
-                             long long n, void* k_out, void* v_out, void* status, cudaStream_t stream) {
-  const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
+struct Kv4ReadArgs {
+  const void *k_cache, *v_cache;
+  const long long* slots;
+  void *k_out, *v_out;
+  long long n, blocks;
+  int block, hkv, d, reserved;
+};
+extern "C" int omni_kv4_read(const Kv4ReadArgs* p, void* status, cudaStream_t stream) {
+  const Kv4Cache c = {(uint8_t*)p->k_cache, (uint8_t*)p->v_cache, p->blocks, p->block, p->hkv, p->d};
   if (!kv4_shape_ok(c)) return -1;
-  if (n <= 0) return 0;
+  if (p->n <= 0) return 0;
   Kv4Rows a = {};
-  a.k_out = (__nv_bfloat16*)k_out;
-  a.v_out = (__nv_bfloat16*)v_out;
-  a.slots = slots;
-  a.n = n;
-  const int wl = kv4_log2(d / 8);
-  const long long grid = (((n * hkv * 2) << wl) + 255) / 256;
+  a.k_out = (__nv_bfloat16*)p->k_out;
+  a.v_out = (__nv_bfloat16*)p->v_out;
+  a.slots = p->slots;
+  a.n = p->n;
+  const int wl = kv4_log2(p->d / 8);
+  const long long grid = (((p->n * p->hkv * 2) << wl) + 255) / 256;
   if (grid > 0x7fffffffll) return -3;
   kv4_read_kernel<<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
   return (int)cudaGetLastError();
 }
 
-extern "C" int omni_kv4_keep(const float* weights, const int* positions, long long blocks, int block, int hkv, const int* table, int table_ld,
-                             int table_w, const int* seq_lens, const int* seen, int B, int budget, int first, int last, int* keep, int* lens,
-                             int* scratch, void* status, cudaStream_t stream) {
-  if (blocks <= 0 || block < 1 || hkv < 1 || hkv > 65535 || B > 65535 || budget < 1 || first < 0 || last < 0 || first + last > budget) return -1;
-  if (B <= 0) return 0;
-  const Kv4Keep a = {weights, positions, table, seq_lens, seen, blocks, table_ld, table_w, block, hkv, budget, first, last, keep, lens, scratch};
-  kv4_keep_kernel<<<dim3(hkv, B), 1024, 0, stream>>>(a, (OmniStatus*)status);
+struct Kv4KeepArgs {
+  const float* weights;
+  const int *positions, *table, *seq_lens, *seen;
+  int *keep, *lens, *scratch;
+  long long blocks;
+  int block, hkv, table_ld, table_w, batch, budget, first, last;
+};
+extern "C" int omni_kv4_keep(const Kv4KeepArgs* p, void* status, cudaStream_t stream) {
+  if (p->blocks <= 0 || p->block < 1 || p->hkv < 1 || p->hkv > 65535 || p->batch > 65535 || p->budget < 1 || p->first < 0 || p->last < 0 ||
+      p->first + p->last > p->budget)
+    return -1;
+  if (p->batch <= 0) return 0;
+  const Kv4Keep a = {p->weights, p->positions, p->table, p->seq_lens, p->seen, p->blocks, p->table_ld, p->table_w, p->block, p->hkv,
+                     p->budget, p->first, p->last, p->keep, p->lens, p->scratch};
+  kv4_keep_kernel<<<dim3(p->hkv, p->batch), 1024, 0, stream>>>(a, (OmniStatus*)status);
   return (int)cudaGetLastError();
 }
 
-extern "C" int omni_kv4_move(void* k_cache, void* v_cache, long long blocks, int block, int hkv, int d, const int* table, int table_ld, int table_w,
-                             const int* keep, int B, int budget, float* weights, int* positions, void* status, cudaStream_t stream) {
-  const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
-  if (!kv4_shape_ok(c) || hkv > 65535 || B > 65535 || budget < 1) return -1;
-  if (B <= 0) return 0;
-  const Kv4Move a = {table, keep, table_ld, table_w, budget, weights, positions};
-  kv4_move_kernel<<<dim3((budget + 255) / 256, hkv, B), 256, 0, stream>>>(a, c, (OmniStatus*)status);
+struct Kv4MoveArgs {
+  void *k_cache, *v_cache;
+  const int *table, *keep;
+  float* weights;
+  int* positions;
+  long long blocks;
+  int block, hkv, d, table_ld, table_w, batch, budget, reserved;
+};
+extern "C" int omni_kv4_move(const Kv4MoveArgs* p, void* status, cudaStream_t stream) {
+  const Kv4Cache c = {(uint8_t*)p->k_cache, (uint8_t*)p->v_cache, p->blocks, p->block, p->hkv, p->d};
+  if (!kv4_shape_ok(c) || p->hkv > 65535 || p->batch > 65535 || p->budget < 1) return -1;
+  if (p->batch <= 0) return 0;
+  const Kv4Move a = {p->table, p->keep, p->table_ld, p->table_w, p->budget, p->weights, p->positions};
+  kv4_move_kernel<<<dim3((p->budget + 255) / 256, p->hkv, p->batch), 256, 0, stream>>>(a, c, (OmniStatus*)status);
   return (int)cudaGetLastError();
 }

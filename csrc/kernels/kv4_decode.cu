@@ -952,30 +952,41 @@ static cudaError_t kv4_launch_weights(const Kv4Decode& a, const Kv4Cache& c, int
 
 using namespace omni;
 
+// The arguments come in a block, as the caller packs them; 8-byte fields first, so that there are no gaps.
 // row_tile: query rows that share a pass over the cache, 8, or 16 for d <= 128.  min_tiles 0: a block for every item (a row_tile of a
 // key/value head of a request); else `blocks_at_once` blocks share all tiles of 64 tokens (32 for d = 256) equally, at least min_tiles each,
 // and o_part [blocks_at_once, 2, row_tile, d] and lse_part [blocks_at_once, 2, row_tile] take what they have of shared items.
-extern "C" int omni_kv4_decode(const void* q, long long q_row, int q_head, const void* k_cache, const void* v_cache, long long blocks, int block,
-                               int hkv, int d, const int* table, int table_ld, int table_w, const int* seq_lens, int B, int rows, int hq,
-                               float scale, int max_len, int row_tile, int blocks_at_once, int min_tiles, float* o_part, float* lse_part, void* out, float* lse,
-                               float* weights, float decay, void* status, cudaStream_t stream) {
-  const Kv4Cache c = {(uint8_t*)k_cache, (uint8_t*)v_cache, blocks, block, hkv, d};
-  if (!kv4_shape_ok(c) || hq % hkv != 0 || rows < 1 || hkv > 65535 || B > 65535 || min_tiles < 0 ||
-      (row_tile != 8 && (row_tile != 16 || d > 128)))
+struct Kv4DecodeArgs {
+  const void *q, *k_cache, *v_cache;
+  const int *table, *seq_lens;
+  void* out;
+  float *o_part, *lse_part, *lse, *weights;
+  long long q_row, blocks;
+  int q_head, block, hkv, d, table_ld, table_w, batch, rows, hq, max_len, row_tile, blocks_at_once, min_tiles;
+  float scale, decay;
+  int reserved;
+};
+extern "C" int omni_kv4_decode(const Kv4DecodeArgs* p, void* status, cudaStream_t stream) {
+  const int d = p->d, B = p->batch, rep = p->hkv > 0 ? p->hq / p->hkv : 0;
+  const Kv4Cache c = {(uint8_t*)p->k_cache, (uint8_t*)p->v_cache, p->blocks, p->block, p->hkv, d};
+  if (!kv4_shape_ok(c) || p->hq < 1 || p->hq % p->hkv != 0 || p->rows < 1 || p->hkv > 65535 || B > 65535 || p->min_tiles < 0 ||
+      (p->row_tile != 8 && (p->row_tile != 16 || d > 128)))
     return -1;
-  if (weights != nullptr && (lse == nullptr || rows * (hq / hkv) > 256)) return -2;
-  if (min_tiles > 0 && (o_part == nullptr || lse_part == nullptr || blocks_at_once < 1 || blocks_at_once > KV4_MAX_BLOCKS)) return -3;
+  if (p->weights != nullptr && (p->lse == nullptr || p->rows * rep > 256)) return -2;
+  if (p->min_tiles > 0 && (p->o_part == nullptr || p->lse_part == nullptr || p->blocks_at_once < 1 || p->blocks_at_once > KV4_MAX_BLOCKS)) return -3;
   if (B <= 0) return 0;
-  const int wide_q = (uintptr_t)q % 16 == 0 && q_row % 8 == 0 && q_head % 8 == 0;
-  const Kv4Decode a = {(const __nv_bfloat16*)q, q_row, q_head, wide_q, table, seq_lens, table_ld, table_w, rows, hq, scale * 1.4426950408889634f,
-                       (__nv_bfloat16*)out, lse, weights, decay, block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16, min_tiles, o_part, lse_part};
+  const int wide_q = (uintptr_t)p->q % 16 == 0 && p->q_row % 8 == 0 && p->q_head % 8 == 0;
+  const Kv4Decode a = {(const __nv_bfloat16*)p->q, p->q_row, p->q_head, wide_q, p->table, p->seq_lens, p->table_ld, p->table_w, p->rows, p->hq,
+                       p->scale * 1.4426950408889634f, (__nv_bfloat16*)p->out, p->lse, p->weights, p->decay,
+                       p->block % 64 == 0 ? 64 : p->block % 32 == 0 ? 32 : 16, p->min_tiles, p->o_part, p->lse_part};
   OmniStatus* st = (OmniStatus*)status;
-  const bool wide = row_tile == 16;
-  cudaError_t e = d == 64    ? wide ? kv4_launch<1, 2>(a, c, B, blocks_at_once, st, stream) : kv4_launch<1, 1>(a, c, B, blocks_at_once, st, stream)
-                  : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, blocks_at_once, st, stream) : kv4_launch<2, 1>(a, c, B, blocks_at_once, st, stream)
-                             : kv4_launch<4, 1>(a, c, B, blocks_at_once, st, stream);
-  if (e != cudaSuccess || weights == nullptr) return (int)e;
-  e = d == 64 ? kv4_launch_weights<1>(a, c, B, max_len, st, stream) : d == 128 ? kv4_launch_weights<2>(a, c, B, max_len, st, stream)
-                                                                              : kv4_launch_weights<4>(a, c, B, max_len, st, stream);
+  const bool wide = p->row_tile == 16;
+  const int n = p->blocks_at_once;
+  cudaError_t e = d == 64    ? wide ? kv4_launch<1, 2>(a, c, B, n, st, stream) : kv4_launch<1, 1>(a, c, B, n, st, stream)
+                  : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, n, st, stream) : kv4_launch<2, 1>(a, c, B, n, st, stream)
+                             : kv4_launch<4, 1>(a, c, B, n, st, stream);
+  if (e != cudaSuccess || p->weights == nullptr) return (int)e;
+  e = d == 64 ? kv4_launch_weights<1>(a, c, B, p->max_len, st, stream) : d == 128 ? kv4_launch_weights<2>(a, c, B, p->max_len, st, stream)
+                                                                                  : kv4_launch_weights<4>(a, c, B, p->max_len, st, stream);
   return (int)e;
 }

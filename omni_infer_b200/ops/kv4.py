@@ -15,8 +15,8 @@ captured, as their arguments allow.  Block ids and slots outside the cache are r
 are neither written nor read, and the attention of a request with such a block is not to be used."""
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import struct
 
 import torch
 
@@ -168,32 +168,37 @@ def _move_ref(k_cache, v_cache, block_table, keep, weights, positions):
 
 
 # ----------------------------------------------------------------------------- calls
-_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+# The argument blocks of the C calls: pointers and 64-bit numbers, then 32-bit ones
 _ARGS = {
-    "omni_kv4_write": (_P, _L, _I, _P, _L, _I, _P, _L, _P, _P, _L, _I, _I, _I, _P, _P, _P, _P, _P),
-    "omni_kv4_read": (_P, _P, _L, _I, _I, _I, _P, _L, _P, _P, _P, _P),
-    "omni_kv4_keep": (_P, _P, _L, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P),
-    "omni_kv4_move": (_P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P),
-    "omni_kv4_decode": (_P, _L, _I, _P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _P, _P, _P, _F, _P, _P),
+    "omni_kv4_write": struct.Struct("8Q4q6i"),
+    "omni_kv4_read": struct.Struct("5Q2q4i"),
+    "omni_kv4_keep": struct.Struct("8Q1q8i"),
+    "omni_kv4_move": struct.Struct("6Q1q8i"),
+    "omni_kv4_decode": struct.Struct("10Q2q13i2fi"),
 }
 _bound = {}
 
 
 def _call(name, device, *args):
     """Launch on the current stream of the tensors' own device."""
-    fn = _bound.get(name)
-    if fn is None:
+    call = _bound.get(name)
+    if call is None:
         lib = nat.lib()
-        getattr(lib._cdll, name).argtypes = _ARGS[name]
-        fn = _bound[name] = getattr(lib, name)
-    here = contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-    with here:
-        rc = fn(*args, nat.status_buffer(device).data_ptr(), torch.cuda.current_stream(device).cuda_stream)
-    nat.check_rc(rc, name)
+        getattr(lib._cdll, name).argtypes = (ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p)
+        call = _bound[name] = (getattr(lib, name), _ARGS[name].pack)
+    fn, pack = call
+    status, stream = nat.status_buffer(device).data_ptr(), torch._C._cuda_getCurrentRawStream(device.index)
+    if device.index == torch.cuda.current_device():
+        rc = fn(pack(*args), status, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(pack(*args), status, stream)
+    if rc:
+        nat.check_rc(rc, name)
 
 
 def _p(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _check_caches(k_cache, v_cache):
@@ -255,8 +260,8 @@ def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token
         return
     if T == 0:
         return
-    _call("omni_kv4_write", k.device, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _p(slots), T, _p(k_cache), _p(v_cache),
-          blocks, block, hkv, d, _p(weights), _p(positions), _p(token_positions))
+    _call("omni_kv4_write", k.device, _p(k), _p(v), _p(slots), _p(k_cache), _p(v_cache), _p(weights), _p(positions), _p(token_positions),
+          k.stride(0), v.stride(0), T, blocks, k.stride(1), v.stride(1), block, hkv, d, 0)
 
 
 def kv4_read(k_cache, v_cache, slots):
@@ -271,7 +276,7 @@ def kv4_read(k_cache, v_cache, slots):
         return tuple(torch.where(ok, _values_ref(c, s // block, s % block, x), torch.zeros(())).bfloat16() for c, x in ((k_cache, False), (v_cache, True)))
     k, v = (torch.empty(T, hkv, d, dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
     if T:
-        _call("omni_kv4_read", k_cache.device, _p(k_cache), _p(v_cache), blocks, block, hkv, d, _p(slots), T, _p(k), _p(v))
+        _call("omni_kv4_read", k_cache.device, _p(k_cache), _p(v_cache), _p(slots), _p(k), _p(v), T, blocks, block, hkv, d, 0)
     return k, v
 
 
@@ -319,8 +324,9 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
             n = blocks_at_once * 2 * tile
             o_part = torch.empty(n * (d + 1), dtype=torch.float32, device=q.device)
             lse_part = o_part[n * d:]
-        _call("omni_kv4_decode", q.device, _p(q), q.stride(0), q.stride(1), _p(k_cache), _p(v_cache), blocks, block, hkv, d, _p(block_table),
-              block_table.stride(0), width, _p(seq_lens), B, T // B, hq, scale, longest, tile, blocks_at_once, min_tiles, _p(o_part), _p(lse_part), _p(out), _p(lse), _p(weights), decay)
+        _call("omni_kv4_decode", q.device, _p(q), _p(k_cache), _p(v_cache), _p(block_table), _p(seq_lens), _p(out), _p(o_part), _p(lse_part), _p(lse),
+              _p(weights), q.stride(0), blocks, q.stride(1), block, hkv, d, block_table.stride(0), width, B, T // B, hq, longest, tile,
+              blocks_at_once, min_tiles, scale, decay, 0)
     return out
 
 
@@ -348,8 +354,8 @@ def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first
     lens = torch.empty(B, dtype=torch.int32, device=device)
     if B:
         scratch = torch.empty_like(keep)
-        _call("omni_kv4_keep", device, _p(weights), _p(positions), blocks, block, hkv, _p(block_table), block_table.stride(0), block_table.shape[1],
-              _p(seq_lens), _p(seen), B, budget, keep_first, keep_last, _p(keep), _p(lens), _p(scratch))
+        _call("omni_kv4_keep", device, _p(weights), _p(positions), _p(block_table), _p(seq_lens), _p(seen), _p(keep), _p(lens), _p(scratch), blocks,
+              block, hkv, block_table.stride(0), block_table.shape[1], B, budget, keep_first, keep_last)
     return keep, lens
 
 
@@ -367,5 +373,5 @@ def kv4_move(k_cache, v_cache, block_table, keep, weights=None, positions=None):
     if not k_cache.is_cuda:
         _move_ref(k_cache, v_cache, block_table, keep, weights, positions)
     elif B and budget:
-        _call("omni_kv4_move", device, _p(k_cache), _p(v_cache), blocks, block, hkv, d, _p(block_table), block_table.stride(0), block_table.shape[1],
-              _p(keep), B, budget, _p(weights), _p(positions))
+        _call("omni_kv4_move", device, _p(k_cache), _p(v_cache), _p(block_table), _p(keep), _p(weights), _p(positions), blocks, block, hkv, d,
+              block_table.stride(0), block_table.shape[1], B, budget, 0)
