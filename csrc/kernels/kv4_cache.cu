@@ -4,6 +4,7 @@
 // bf16 and codes = round((x - lo) / step) (to nearest, ties to even, 0 where step = 0); it stands for code * step + lo.  lo is one
 // of the bf16 inputs and therefore exact; the step is rounded up so that 15 steps always reach the maximum, and code * step + lo has
 // one rounding in fp32 (code * step has 12 bits).  A group with a NaN, an infinity or a range beyond fp32 is NaN as a whole.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -128,9 +129,11 @@ __device__ __forceinline__ uint32_t kv4_keep_key(float w, int pos, int first, in
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Exclusive sum over a block of 1024 threads; `total` gets the sum.
-__device__ __forceinline__ int kv4_block_scan(int x, int& total) {
-  __shared__ int part[32];
+constexpr int KV4_KEEP_THREADS = 512;
+// Exclusive sum over a block of that many threads
+__device__ __forceinline__ int kv4_block_scan(int x) {
+  constexpr int WARPS = KV4_KEEP_THREADS / 32;
+  __shared__ int part[WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int v = x;
 #pragma unroll
@@ -141,13 +144,14 @@ __device__ __forceinline__ int kv4_block_scan(int x, int& total) {
   __syncthreads();
   if (lane == 31) part[warp] = v;
   __syncthreads();
-  int base = 0, sum = 0;
-  for (int i = 0; i < 32; ++i) {
-    if (i < warp) base += part[i];
-    sum += part[i];
+  int sum = lane < WARPS ? part[lane] : 0;                          // every warp scans the warps' sums by itself
+#pragma unroll
+  for (int o = 1; o < WARPS; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
   }
-  total = sum;
-  return base + v - x;
+  const int base = __shfl_sync(0xffffffffu, sum, warp > 0 ? warp - 1 : 0);
+  return (warp > 0 ? base : 0) + v - x;
 }
 
 struct Kv4Keep {
@@ -155,80 +159,195 @@ struct Kv4Keep {
   const int *positions, *table, *seq_lens, *seen;
   long long blocks;
   int table_ld, table_w, block, hkv, budget, first, last;
-  int *keep, *lens, *holes;         // [B, Hkv, budget], [B], scratch as keep
+  int *keep, *lens, *sources;       // [B, Hkv, budget], [B], scratch as keep
 };
 
-// One block for a request and head: the key of the budget-th heaviest place by a radix selection of 8 bits a pass, then one pass
-// in the order of places that fills the places below the budget that are not kept with the kept places behind it.
-__global__ void __launch_bounds__(1024) kv4_keep_kernel(Kv4Keep a, OmniStatus* st) {
-  const int b = blockIdx.y, h = blockIdx.x;
-  __shared__ int hist[256];
+// A cluster of blocks for a request and head, each with a run of its places.  The keys are read from memory once and kept in shared
+// memory (`cap` of them a block; those beyond are made again when they are needed).  The key of the budget-th heaviest place is
+// found 11, 11 and 10 bits at a time: histograms in shared memory, which every block of the cluster adds up for itself.  Then a
+// thread walks its own run of places, so that ranks (of equal keys, of the places to fill, of the tokens that fill them) are one
+// scan each.  Reads 8 bytes a place; bound by the latency of its some ten steps.
+constexpr int KV4_BINS = 2048, KV4_MOST_BLOCKS = 8;
+__global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a, int cap, OmniStatus* st) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  constexpr int N = KV4_KEEP_THREADS;
+  extern __shared__ uint32_t s_keys[];
+  __shared__ __align__(16) int hist[2][KV4_BINS];                   // highest keys first
+  __shared__ int s_count[2];        // of this block: places to fill, tokens that fill some
+  __shared__ int s_equal;           // keys equal to the last that stays in the blocks ahead
   __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
+  __shared__ int s_left, s_all;
+  const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int b = blockIdx.y, h = blockIdx.x / size, tid = threadIdx.x;
   int n = max(a.seq_lens[b], 0);
   if (n > a.table_w * a.block) {
-    if (threadIdx.x == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
+    if (tid == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
     n = a.table_w * a.block;
   }
   int* keep = a.keep + ((long long)b * a.hkv + h) * a.budget;
-  if (h == 0 && threadIdx.x == 0) a.lens[b] = min(n, a.budget);
+  int* sources = a.sources + ((long long)b * a.hkv + h) * a.budget;
+  if (blockIdx.x == 0 && tid == 0) a.lens[b] = min(n, a.budget);
   if (n <= a.budget) {
-    for (int j = threadIdx.x; j < a.budget; j += 1024) keep[j] = j < n ? j : -1;
+    for (int j = rank * N + tid; j < a.budget; j += size * N) keep[j] = j < n ? j : -1;
     return;
   }
+  const int chunk = (n + size - 1) / size, j0 = rank * chunk, count = max(0, min(chunk, n - j0));
   const int last_from = a.seen[b] - a.last;
-  auto key_of = [&](int j) -> uint32_t {
-    const int blk = a.table[(long long)b * a.table_ld + j / a.block];
+  const int* table = a.table + (long long)b * a.table_ld;
+  auto make_at = [&](int page, int off) -> uint32_t {
+    const int blk = table[page];
     if (blk < 0 || blk >= a.blocks) {
       report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
       return 0u;
     }
-    const long long at = ((long long)blk * a.hkv + h) * a.block + j % a.block;
+    const long long at = ((long long)blk * a.hkv + h) * a.block + off;
     return kv4_keep_key(a.weights[at], a.positions[at], a.first, last_from);
   };
+  auto make = [&](int i) -> uint32_t { return make_at((j0 + i) / a.block, (j0 + i) % a.block); };
+  auto key = [&](int i) -> uint32_t { return i < cap ? s_keys[i] : make(i); };
+  for (int i = tid; i < KV4_BINS; i += N) hist[0][i] = hist[1][i] = 0;
+  __syncthreads();
+  {
+    constexpr int AT_ONCE = 8;                                      // loads under way a thread: block ids, then weights and positions
+    const int pages = N / a.block, rest = N - pages * a.block;
+    int page = (j0 + tid) / a.block, off = (j0 + tid) - page * a.block;
+    for (int i = tid; i < count; i += N * AT_ONCE) {
+      int blk[AT_ONCE], at[AT_ONCE], pos[AT_ONCE];
+      float w[AT_ONCE];
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; ++x) {
+        at[x] = off;
+        blk[x] = i + x * N < count ? table[page] : 0;
+        page += pages;
+        off += rest;
+        if (off >= a.block) {
+          off -= a.block;
+          ++page;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; ++x) {
+        const bool in = blk[x] >= 0 && blk[x] < a.blocks;
+        const long long to = ((long long)(in ? blk[x] : 0) * a.hkv + h) * a.block + at[x];
+        w[x] = a.weights[to];
+        pos[x] = a.positions[to];
+      }
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; ++x) {
+        if (i + x * N >= count) break;
+        uint32_t k = kv4_keep_key(w[x], pos[x], a.first, last_from);
+        if (blk[x] < 0 || blk[x] >= a.blocks) {
+          report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
+          k = 0u;
+        }
+        if (i + x * N < cap) s_keys[i + x * N] = k;
+        atomicAdd(&hist[0][KV4_BINS - 1 - (k >> 21)], 1);
+      }
+    }
+  }
   uint32_t prefix = 0, mask = 0;
   int left = a.budget;                                              // of the places whose key starts with the prefix, so many stay
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < n; j += 1024) {
-      const uint32_t key = key_of(j);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+  bool all_stay = false;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    int* mine = hist[pass & 1];
+    if (pass > 0) {
+      for (int i = tid; i < count; i += N) {
+        const uint32_t k = key(i);
+        if ((k & mask) == prefix) atomicAdd(&mine[bins - 1 - ((k >> shift) & (bins - 1))], 1);
+      }
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int d = 255, rest = left;
-      while (d > 0 && hist[d] < rest) rest -= hist[d--];
-      s_left = rest;
-      s_prefix = prefix | (uint32_t)d << shift;
+    cluster.sync();
+    constexpr int MOST = KV4_BINS / N;                              // bins of a thread, or half as many
+    static_assert(MOST == 4, "four bins are one read");
+    const int each = bins / N;
+    int v[MOST] = {0, 0, 0, 0};
+#pragma unroll
+    for (int r = 0; r < KV4_MOST_BLOCKS; ++r) {
+      if (r >= size) continue;
+      const int* theirs = cluster.map_shared_rank(mine, r) + tid * each;
+      if (each == 4) {
+        const int4 x = *reinterpret_cast<const int4*>(theirs);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      } else {
+        const int2 x = *reinterpret_cast<const int2*>(theirs);
+        v[0] += x.x; v[1] += x.y;
+      }
     }
+    int above = kv4_block_scan(v[0] + v[1] + v[2] + v[3]);
+#pragma unroll
+    for (int d = 0; d < MOST; ++d) {
+      if (above < left && left <= above + v[d]) {
+        s_prefix = prefix | (uint32_t)(bins - 1 - tid * each - d) << shift;
+        s_left = left - above;
+        s_all = v[d];
+      }
+      above += v[d];
+    }
+    if (pass == 1)                                                  // nobody reads the first histogram any more: it serves once more
+      for (int i = tid; i < KV4_BINS; i += N) hist[0][i] = 0;
     __syncthreads();
     prefix = s_prefix;
     left = s_left;
-    mask |= 255u << shift;
+    all_stay = left == s_all;
+    mask |= (uint32_t)(bins - 1) << shift;
     __syncthreads();
+    if (all_stay) break;                                            // no need to tell the places of this prefix apart
   }
-  // `prefix` is the key of the last place that stays; `left` of the places with that key do, the lowest first
-  int* holes = a.holes + ((long long)b * a.hkv + h) * a.budget;
-  int equal = 0, hole = 0, source = 0;                              // found so far
-  for (int j0 = 0; j0 < n; j0 += 1024) {
-    const int j = j0 + threadIdx.x;
-    const uint32_t key = j < n ? key_of(j) : 0u;
-    const bool same = j < n && key == prefix;
-    int all;
-    const int rank = equal + kv4_block_scan(same, all);
-    equal += all;
-    const bool stays = j < n && (key > prefix || (same && rank < left));
-    const bool is_hole = j < a.budget && !stays, is_source = j >= a.budget && stays;
-    if (j < a.budget && stays) keep[j] = j;
-    const int hr = hole + kv4_block_scan(is_hole, all);
-    hole += all;
-    if (is_hole) holes[hr] = j;
-    __syncthreads();                                                // a source's hole may have been found in this chunk
-    const int sr = source + kv4_block_scan(is_source, all);
-    source += all;
-    if (is_source) keep[holes[sr]] = j;
+  // `prefix` begins the keys of the last places that stay; `left` of the places with such keys do, the lowest first.  An odd run a thread:
+  // its reads of shared memory meet no others.
+  const int each = ((count + N - 1) / N) | 1, i0 = min(tid * each, count), i1 = min(i0 + each, count);
+  int equal0 = 0;
+  if (!all_stay) {                                                  // all bits are known: the keys are equal
+    if (tid < 32) {                                                 // their number in the blocks ahead is in the last histograms
+      int x = 0;
+      if (tid < rank) x = cluster.map_shared_rank(hist[0], tid)[1023 - (prefix & 1023)];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      if (tid == 0) s_equal = x;
+    }
+    for (int i = i0; i < i1; ++i) equal0 += key(i) == prefix;
+    equal0 = kv4_block_scan(equal0);                                // s_equal is there after its barriers
+    equal0 += s_equal;
   }
+  // Whether place i stays, asked in order
+  auto stays = [&](int i, int& equal) -> bool {
+    const uint32_t k = key(i) & mask;
+    return k > prefix || (k == prefix && (all_stay || equal++ < left));
+  };
+  int holes = 0, far = 0, equal = equal0;
+  for (int i = i0; i < i1; ++i) {
+    const bool s = stays(i, equal), near = j0 + i < a.budget;
+    holes += near && !s;
+    far += !near && s;
+  }
+  int hole = kv4_block_scan(holes), source = kv4_block_scan(far);
+  if (tid == N - 1) {
+    s_count[0] = hole + holes;
+    s_count[1] = source + far;
+  }
+  cluster.sync();
+#pragma unroll
+  for (int r = 0; r < KV4_MOST_BLOCKS; ++r)
+    if (r < rank) {
+      const int* theirs = cluster.map_shared_rank(s_count, r);
+      hole += theirs[0];
+      source += theirs[1];
+    }
+  equal = equal0;
+  if (j0 < a.budget || far > 0)
+    for (int i = i0; i < i1; ++i) {
+      if (!stays(i, equal)) continue;
+      if (j0 + i < a.budget) keep[j0 + i] = j0 + i;
+      else sources[source++] = j0 + i;
+    }
+  cluster.sync();                                                   // all sources are there, and nobody reads another's memory any more
+  equal = equal0;
+  if (holes > 0)
+    for (int i = i0; i < i1 && j0 + i < a.budget; ++i)
+      if (!stays(i, equal)) keep[j0 + i] = sources[hole++];
 }
 
 struct Kv4Move {
@@ -359,17 +478,38 @@ struct Kv4KeepArgs {
   const int *positions, *table, *seq_lens, *seen;
   int *keep, *lens, *scratch;
   long long blocks;
-  int block, hkv, table_ld, table_w, batch, budget, first, last;
+  int block, hkv, table_ld, table_w, batch, budget, first, last, max_len, reserved;
 };
 extern "C" int omni_kv4_keep(const Kv4KeepArgs* p, void* status, cudaStream_t stream) {
-  if (p->blocks <= 0 || p->block < 1 || p->hkv < 1 || p->hkv > 65535 || p->batch > 65535 || p->budget < 1 || p->first < 0 || p->last < 0 ||
+  if (p->blocks <= 0 || p->block < 1 || p->hkv < 1 || p->hkv > 65535 || p->batch > 65535 || p->budget < 1 || p->max_len < 0 || p->first < 0 || p->last < 0 ||
       p->first + p->last > p->budget)
     return -1;
   if (p->batch <= 0) return 0;
   const Kv4Keep a = {p->weights, p->positions, p->table, p->seq_lens, p->seen, p->blocks, p->table_ld, p->table_w, p->block, p->hkv,
                      p->budget, p->first, p->last, p->keep, p->lens, p->scratch};
-  kv4_keep_kernel<<<dim3(p->hkv, p->batch), 1024, 0, stream>>>(a, (OmniStatus*)status);
-  return (int)cudaGetLastError();
+  // Blocks of a cluster: one for every 2048 places, at most 8; of its keys a block keeps up to 40,000.
+  int size = 1;
+  while (size < KV4_MOST_BLOCKS && p->max_len > 2048 * size) size *= 2;
+  const int run = (p->max_len + size - 1) / size, cap = run < 1024 ? 1024 : run > 40000 ? 40000 : run;
+  static bool asked[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !asked[dev])) {
+    e = cudaFuncSetAttribute(kv4_keep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 40000 * 4);
+    if (e == cudaSuccess && dev < 64) asked[dev] = true;
+  }
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(p->hkv * size, p->batch);
+  config.blockDim = dim3(KV4_KEEP_THREADS);
+  config.dynamicSmemBytes = cap * 4;
+  config.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {(unsigned)size, 1, 1};
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&config, kv4_keep_kernel, a, cap, (OmniStatus*)status);
 }
 
 struct Kv4MoveArgs {

@@ -172,7 +172,7 @@ def _move_ref(k_cache, v_cache, block_table, keep, weights, positions):
 _ARGS = {
     "omni_kv4_write": struct.Struct("8Q4q6i"),
     "omni_kv4_read": struct.Struct("5Q2q4i"),
-    "omni_kv4_keep": struct.Struct("8Q1q8i"),
+    "omni_kv4_keep": struct.Struct("8Q1q10i"),
     "omni_kv4_move": struct.Struct("6Q1q8i"),
     "omni_kv4_decode": struct.Struct("10Q2q13i2fi"),
 }
@@ -314,7 +314,7 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
     if T:
         width, total = block_table.shape[1], T // B * (hq // hkv)
         assert weights is None or total <= 256, f"weights of at most 256 query rows a key/value head at once: {total}"
-        longest = width * block if max_seq_len is None else min(max_seq_len, width * block)
+        longest = width * block if max_seq_len is None else max(0, min(max_seq_len, width * block))
         tile = 16 if d <= 128 and total > 8 else 8
         items = B * hkv * -(-total // tile)
         blocks_at_once, min_tiles = _blocks(items, -(-longest // (32 if d == 256 else 64)), 3 if tile * d <= 1024 else 2)
@@ -337,7 +337,8 @@ def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first
 
     Returns (keep [B, Hkv, budget] int32, lens [B] int32 = the smaller of seq_lens and budget).  keep[b, h, j] is the place whose token
     is to be in place j: j itself where that stays, else one of the kept places from the budget on, in ascending order over the
-    places that become free; -1 from lens[b] on.  Nothing is moved: see ``kv4_move``."""
+    places that become free; -1 from lens[b] on.  Nothing is moved: see ``kv4_move``.  ``max_seq_len``
+    as in ``kv4_decode``."""
     assert weights.dim() == 3, "weights: [blocks, Hkv, block]"
     device = weights.device
     blocks, hkv, block = weights.shape
@@ -354,8 +355,10 @@ def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first
     lens = torch.empty(B, dtype=torch.int32, device=device)
     if B:
         scratch = torch.empty_like(keep)
+        width = block_table.shape[1]
+        longest = width * block if max_seq_len is None else max(0, min(max_seq_len, width * block))
         _call("omni_kv4_keep", device, _p(weights), _p(positions), _p(block_table), _p(seq_lens), _p(seen), _p(keep), _p(lens), _p(scratch), blocks,
-              block, hkv, block_table.stride(0), block_table.shape[1], B, budget, keep_first, keep_last)
+              block, hkv, block_table.stride(0), width, B, budget, keep_first, keep_last, longest, 0)
     return keep, lens
 
 

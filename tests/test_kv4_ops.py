@@ -326,6 +326,28 @@ def test_keep(dev, lens, hkv, block, budget, first, last, ties, nans):
             assert keep[b, h].tolist() == want + [-1] * (budget - len(want)), f"request {b}, head {h}"
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bound", [None, 10, 50_000])
+@pytest.mark.parametrize("lens,budget", [([50_000, 41_003, 4097, 300], 4096), ([330_000], 300_001)])
+def test_keep_of_long_requests(lens, budget, bound):
+    """Whatever the launch is shaped by, and with more places than shared memory holds."""
+    g, hkv, block = _gen(budget), 2, 128
+    width = -(-max(lens) // block)
+    blocks = len(lens) * width
+    table = torch.randperm(blocks, generator=g).view(len(lens), width).to(torch.int32)
+    w = torch.round(torch.rand(blocks, hkv, block, generator=g) * 3000) / 7          # many equal ones
+    pos = torch.randint(0, max(lens), (blocks, hkv, block), generator=g, dtype=torch.int32)
+    seen = [n - n // 9 for n in lens]
+    keep, kept = ops.kv4_keep(w.cuda(), pos.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(seen, dtype=torch.int32).cuda(),
+                              budget, keep_first=3, keep_last=100, max_seq_len=bound)
+    assert kept.tolist() == [min(n, budget) for n in lens]
+    for b, n in enumerate(lens):
+        wb, pb = (x[table[b].long()].transpose(0, 1).flatten(1)[:, :n] for x in (w, pos))
+        for h in range(hkv):
+            want = O.keep(wb[h].tolist(), pb[h].tolist(), n, seen[b], budget, 3, 100)
+            assert keep[b, h].tolist() == want + [-1] * (budget - len(want))
+
+
 @BOTH
 @pytest.mark.parametrize("d,block,hkv", [(64, 16, 3), (128, 48, 2), (256, 32, 1)])
 def test_move(dev, d, block, hkv):
