@@ -6,9 +6,11 @@
 // one rounding in fp32 (code * step has 12 bits).  A group with a NaN, an infinity or a range beyond fp32 is NaN as a whole.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../include/kv4.cuh"
 #include "../include/omni_ptx.cuh"
@@ -28,96 +30,193 @@ struct Kv4Rows {
   float* weights;                   // write: [blocks, Hkv, block] or null, set to zero
   int* positions;                   // write: [blocks, Hkv, block] or null, set to token_positions[i]
   const long long* token_positions;
+  int parts, span;                  // warps of a token, and their heads
 };
 
-// A thread holds one word (8 columns) of one row; the 8 threads of a group find its range with three shuffles.  Bound by memory:
-// reads 2 d bytes and writes 9 d / 16 a row.
-template <bool VEC>
-__global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows a, Kv4Cache c, int words_log2, OmniStatus* st) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int u = (int)(i & ((1 << words_log2) - 1));
-  const long long row = i >> words_log2;                            // (token, head, key or value)
-  const long long th = row >> 1;
-  const bool values = row & 1;
-  const long long tok = th / c.hkv;
-  const int h = (int)(th - tok * c.hkv);
-  if (tok >= a.n) return;                                           // whole rows, and rows are whole groups of 8 threads
-  const unsigned mask = 0xffu << (threadIdx.x & 24);
-  const __nv_bfloat16* src = values ? a.v + tok * a.v_row + (long long)h * a.v_head : a.k + tok * a.k_row + (long long)h * a.k_head;
-  src += u * 8;
-  __nv_bfloat162 x[4];
-  if (VEC) {
-    *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(src);
+// A warp takes a token at a time and walks its heads.  Which word (8 columns) of the keys or of the values a lane has is the same for all
+// heads, so that its addresses are worked out once a token and then go on by a stride.  At d = 128 the 32 lanes have the two rows of a
+// head, at d = 64 those of two heads, at d = 256 the keys' row and then the values'.  Where there are few tokens, several warps share one.
+struct Kv4Place {
+  long long blk;                    // -1: no row
+  int t;
+};
+__device__ __forceinline__ Kv4Place kv4_place(const Kv4Cache& c, long long slot, OmniStatus* st, long long tok) {
+  if (slot < 0) return {-1, 0};
+  Kv4Place p;
+  if (slot < 0x7fffffffll) {        // a 64-bit division costs as much as the rest of the row
+    p.blk = (unsigned)slot / (unsigned)c.block;
+    p.t = (int)slot - (int)p.blk * c.block;
   } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = __halves2bfloat162(src[2 * j], src[2 * j + 1]);
+    p.blk = slot / c.block;
+    p.t = (int)(slot - p.blk * c.block);
   }
-  __nv_bfloat162 lo2 = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3]));
-  __nv_bfloat162 hi2 = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
-  __nv_bfloat16 lo = __hmin_nan(__low2bfloat16(lo2), __high2bfloat16(lo2)), hi = __hmax_nan(__low2bfloat16(hi2), __high2bfloat16(hi2));
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
-    lo = __hmin_nan(lo, __shfl_xor_sync(mask, lo, o));
-    hi = __hmax_nan(hi, __shfl_xor_sync(mask, hi, o));
+  if (p.blk < c.blocks) return p;
+  if ((threadIdx.x & 31) == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_ROWS, (int)tok);
+  return {-1, 0};
+}
+
+// round(x / step), ties to even, for 0 <= x <= 15 step.  The product with the inverse is a whole number at most one off after 1.5 2^23 has
+// rounded it into the lowest bits; code * step is exact (4 and 8 bits) and x - code * step as well (no bit of it lies below those of x and of
+// the step), so that comparing it with half a step settles the code.
+__device__ __forceinline__ uint32_t kv4_nearest(float x, float step, float inverse) {
+  const float up = __fadd_rn(__fmul_rn(x, inverse), 12582912.f);
+  const float off = __fmaf_rn(-__fsub_rn(up, 12582912.f), step, x), twice = 2.f * fabsf(off);
+  uint32_t code = __float_as_uint(up);
+  if (twice > step || (twice == step && (code & 1u))) code += off > 0.f ? 1u : ~0u;
+  return code & 15u;
+}
+
+template <int D>
+struct Kv4Lane {
+  static constexpr int WORDS = D / 8, SIDES = WORDS == 32 ? 2 : 1, HEADS = WORDS == 8 ? 2 : 1;      // steps of a head, heads of a step
+  int u, head;
+  bool values;                      // of the first side
+  __device__ __forceinline__ Kv4Lane() {
+    const int lane = threadIdx.x & 31;
+    u = lane & (WORDS - 1);
+    values = SIDES == 1 && ((lane / WORDS) & 1);
+    head = HEADS == 2 ? lane >> 4 : 0;
   }
-  const float low = __bfloat162float(lo), range = __fsub_rn(__bfloat162float(hi), low);
-  float step = __uint_as_float((__float_as_uint(__fdiv_rn(range, 15.f)) + 0xffffu) & 0xffff0000u);
-  if (!(range < INFINITY)) step = __uint_as_float(0x7fc00000u);     // NaN or infinite
-  uint32_t word = 0;
-  if (step > 0.f) {
+  __device__ __forceinline__ long long word(const Kv4Cache& c, const Kv4Place& p, bool of_values, int h) const {
+    return c.at(p.blk, h) + (of_values ? c.v_word(p.t, u) : c.k_word(p.t, u));
+  }
+  __device__ __forceinline__ long long scale(const Kv4Cache& c, const Kv4Place& p, int h) const { return c.at(p.blk, h) + c.scale_word(p.t, u >> 3); }
+};
+// Token and heads of unit `unit`
+__device__ __forceinline__ long long kv4_unit(const Kv4Rows& a, const Kv4Cache& c, long long unit, int& from, int& to) {
+  const long long tok = a.parts == 1 ? unit : unit < 0x7fffffffll ? (long long)((unsigned)unit / (unsigned)a.parts) : unit / a.parts;
+  from = (int)(unit - tok * a.parts) * a.span;
+  to = min(c.hkv, from + a.span);
+  return tok;
+}
+
+// The 8 lanes of a group find its range with three shuffles.  Reads 2 d bytes and writes 9 d / 16 a row; bound by its
+// instructions.
+template <int D, bool VEC>
+__global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows a, Kv4Cache c, OmniStatus* st) {
+  using L = Kv4Lane<D>;
+  const L lane;
+  const long long warps = (long long)gridDim.x * 8;
+  for (long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); unit < a.n * a.parts; unit += warps) {
+    int from, to;
+    const long long tok = kv4_unit(a, c, unit, from, to);
+    const Kv4Place p = kv4_place(c, a.slots[tok], st, tok);
+    if (p.blk < 0) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __bfloat1622float2(x[j]);
-      const float c0 = fminf(rintf(__fdiv_rn(__fsub_rn(f.x, low), step)), 15.f), c1 = fminf(rintf(__fdiv_rn(__fsub_rn(f.y, low), step)), 15.f);
-      word |= ((uint32_t)c0 | (uint32_t)c1 << 4) << (8 * j);
+    for (int side = 0; side < L::SIDES; ++side) {
+      const bool values = L::SIDES == 2 ? side == 1 : lane.values;
+      const __nv_bfloat16* rows = (values ? a.v + tok * a.v_row : a.k + tok * a.k_row) + lane.u * 8;
+      const int head_step = values ? a.v_head : a.k_head;
+      uint8_t* cache = values ? c.v : c.k;
+      for (int h0 = from; h0 < to; h0 += L::HEADS) {
+        const int h = h0 + lane.head;
+        const bool in = h < to;
+        const __nv_bfloat16* src = rows + (long long)h * head_step;
+        __nv_bfloat162 x[4];
+        if (!in) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = __float2bfloat162_rn(0.f);
+        } else if (VEC) {
+          *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(src);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = __halves2bfloat162(src[2 * j], src[2 * j + 1]);
+        }
+        const __nv_bfloat162 lo2 = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3]));
+        const __nv_bfloat162 hi2 = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
+        __nv_bfloat16 lo = __hmin_nan(__low2bfloat16(lo2), __high2bfloat16(lo2)), hi = __hmax_nan(__low2bfloat16(hi2), __high2bfloat16(hi2));
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+          lo = __hmin_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+          hi = __hmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const float low = __bfloat162float(lo), range = __fsub_rn(__bfloat162float(hi), low);
+        float step = __uint_as_float((__float_as_uint(__fdiv_rn(range, 15.f)) + 0xffffu) & 0xffff0000u);
+        if (!(range < INFINITY)) step = __uint_as_float(0x7fc00000u);                                     // NaN or infinite
+        uint32_t word = 0;
+        if (step > 0.f) {
+          const float lift = step < 0x1p-100f ? 0x1p60f : 1.f, unit = step * lift, inverse = __frcp_rn(unit);      // an inverse that is finite
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = __bfloat1622float2(x[j]);
+            word |= (kv4_nearest(__fsub_rn(f.x, low) * lift, unit, inverse) | kv4_nearest(__fsub_rn(f.y, low) * lift, unit, inverse) << 4) << (8 * j);
+          }
+        }
+        if (!in) continue;
+        *reinterpret_cast<uint32_t*>(cache + lane.word(c, p, values, h)) = word;
+        if ((lane.u & 7) == 0)
+          *reinterpret_cast<uint32_t*>(cache + lane.scale(c, p, h)) = (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
+        if (lane.u == 0 && !values) {
+          const long long at = (p.blk * c.hkv + h) * c.block + p.t;
+          if (a.weights != nullptr) a.weights[at] = 0.f;
+          if (a.positions != nullptr) a.positions[at] = (int)a.token_positions[tok];
+        }
+      }
     }
-  }
-  const long long slot = a.slots[tok];
-  if (slot < 0) return;
-  const long long blk = slot / c.block;
-  if (blk >= c.blocks) {
-    if (u == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_ROWS, (int)tok);
-    return;
-  }
-  const int t = (int)(slot - blk * c.block);
-  uint8_t* piece = (values ? c.v : c.k) + c.at(blk, h);
-  *reinterpret_cast<uint32_t*>(piece + (values ? c.v_word(t, u) : c.k_word(t, u))) = word;
-  if ((u & 7) == 0)
-    *reinterpret_cast<uint32_t*>(piece + c.scale_word(t, u >> 3)) = (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
-  if (u == 0 && !values) {
-    const long long at = (blk * c.hkv + h) * c.block + t;
-    if (a.weights != nullptr) a.weights[at] = 0.f;
-    if (a.positions != nullptr) a.positions[at] = (int)a.token_positions[tok];
   }
 }
 
-// The inverse: one word of codes and its group's word to 8 bf16 values.  Bound by memory: reads 9 d / 16 bytes and writes 2 d a row.
-__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Rows a, Kv4Cache c, int words_log2, OmniStatus* st) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int u = (int)(i & ((1 << words_log2) - 1));
-  const long long row = i >> words_log2;
-  const long long th = row >> 1;
-  const bool values = row & 1;
-  const long long tok = th / c.hkv;
-  const int h = (int)(th - tok * c.hkv);
-  if (tok >= a.n) return;
-  const long long slot = a.slots[tok], blk = slot < 0 ? -1 : slot / c.block;
-  uint4 out = make_uint4(0u, 0u, 0u, 0u);
-  if (blk >= c.blocks) {
-    if (u == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_ROWS, (int)tok);
-  } else if (blk >= 0) {
-    const int t = (int)(slot - blk * c.block);
-    const uint8_t* piece = (values ? c.v : c.k) + c.at(blk, h);
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(piece + (values ? c.v_word(t, u) : c.k_word(t, u)));
-    const uint32_t s = *reinterpret_cast<const uint32_t*>(piece + c.scale_word(t, u >> 3));
-    const float step = kv4_step(s), low = kv4_low(s);
-    __nv_bfloat162 x[4];
+// The inverse: a word of codes and its group's word to 8 bf16 values, four words a lane under way.  Bound by memory: reads 9 d / 16 bytes
+// and writes 2 d a row.
+template <int D>
+__global__ void __launch_bounds__(256, 8) kv4_read_kernel(Kv4Rows a, Kv4Cache c, OmniStatus* st) {
+  using L = Kv4Lane<D>;
+  constexpr int AT_ONCE = 4;
+  const L lane;
+  const long long warps = (long long)gridDim.x * 8, head_bytes = c.piece() * L::HEADS;
+  for (long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); unit < a.n * a.parts; unit += warps) {
+    int from, to;
+    const long long tok = kv4_unit(a, c, unit, from, to);
+    const Kv4Place p = kv4_place(c, a.slots[tok], st, tok);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      x[j] = __floats2bfloat162_rn(fmaf((float)((w >> (8 * j)) & 15u), step, low), fmaf((float)((w >> (8 * j + 4)) & 15u), step, low));
-    out = *reinterpret_cast<uint4*>(x);
+    for (int side = 0; side < L::SIDES; ++side) {
+      const bool values = L::SIDES == 2 ? side == 1 : lane.values;
+      const int h = from + lane.head;
+      const uint8_t* cache = values ? c.v : c.k;
+      const uint8_t *codes = cache + lane.word(c, p, values, h), *scales = cache + lane.scale(c, p, h);
+      __nv_bfloat16* to_row = (values ? a.v_out : a.k_out) + (tok * c.hkv + h) * D + lane.u * 8;
+      int left = p.blk < 0 ? 0 : to - h;                                    // heads of this lane that there are to read
+      for (int h0 = from; h0 < to; h0 += L::HEADS * AT_ONCE) {
+        uint32_t w[AT_ONCE], s[AT_ONCE];
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x) {
+          w[x] = s[x] = 0u;
+          if (x * L::HEADS < left) {
+            w[x] = *reinterpret_cast<const uint32_t*>(codes + x * head_bytes);
+            s[x] = *reinterpret_cast<const uint32_t*>(scales + x * head_bytes);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x) {
+          const float step = kv4_step(s[x]), low = kv4_low(s[x]);
+          __nv_bfloat162 y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // the byte in both halves; 1024 + code and 1024 + 16 code as fp16 numbers, whose conversion runs beside the integer operations
+            const uint32_t pair = (__byte_perm(w[x], 0u, j | 0x4040 | j << 8) & 0x00f0000fu) | 0x64006400u;
+            const float2 code = __half22float2(__hfma2(*reinterpret_cast<const __half2*>(&pair), __floats2half2_rn(1.f, 0.0625f), __floats2half2_rn(-1024.f, -64.f)));
+            y[j] = __floats2bfloat162_rn(fmaf(code.x, step, low), fmaf(code.y, step, low));
+          }
+          if (h0 + x * L::HEADS + lane.head < to) *reinterpret_cast<uint4*>(to_row + x * (L::HEADS * D)) = *reinterpret_cast<uint4*>(y);
+        }
+        codes += head_bytes * AT_ONCE;
+        scales += head_bytes * AT_ONCE;
+        to_row += L::HEADS * AT_ONCE * D;
+        left -= L::HEADS * AT_ONCE;
+      }
+    }
   }
-  *reinterpret_cast<uint4*>((values ? a.v_out : a.k_out) + (th << words_log2) * 8 + u * 8) = out;
+}
+// Blocks of 8 warps, as many as fit the card four times over at most.  A token's heads are shared out to several warps while there are fewer
+// warps than `want`: 4099 tokens of 8 heads take 21 us by a warp a head, 17 us by a warp for two, 26 us by a warp a token.
+static unsigned kv4_row_blocks(Kv4Rows& a, const Kv4Cache& c, long long want) {
+  const int heads = c.d == 64 ? 2 : 1, steps = (c.hkv + heads - 1) / heads;
+  const long long share = (want + a.n - 1) / a.n;
+  const int parts = share < steps ? (int)share : steps, each = (steps + parts - 1) / parts;
+  a.parts = (steps + each - 1) / each;
+  a.span = each * heads;
+  const long long blocks = (a.n * a.parts + 7) / 8, most = 148 * 8 * 4;
+  return (unsigned)(blocks < most ? blocks : most);
 }
 
 // ------------------------------------------------------------------------------------------------ eviction
@@ -357,55 +456,47 @@ struct Kv4Move {
   int* positions;
 };
 
-// A warp looks at 32 places and copies the rows of those that are filled from elsewhere.  Sources lie behind the budget and places
-// below it, so no row is both and the order of the copies does not matter.
+// Eight lanes for a place; those of a place that is filled from elsewhere copy the row, all loads ahead of the stores.  Sources lie behind
+// the budget and places below it, so no row is both and the order of the copies does not matter.  Bound by latency: a place's keep entry,
+// the two block ids, the row.
+template <int GROUPS>
 __global__ void __launch_bounds__(256) kv4_move_kernel(Kv4Move a, Kv4Cache c, OmniStatus* st) {
-  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31;
-  const int j = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 32 + lane;
+  constexpr int PER = GROUPS > 1 ? 2 : 1, PLANES = GROUPS / PER;
+  using Chunk = typename std::conditional<PER == 2, uint2, uint32_t>::type;         // what a lane has of a plane of a row
+  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 7, j = blockIdx.x * 32 + (threadIdx.x >> 3);
+  if (j >= a.budget) return;
+  const int s = a.keep[((long long)b * c.hkv + h) * a.budget + j];
+  if (s < 0 || s == j) return;
   const int* table = a.table + (long long)b * a.table_ld;
-  int from = -1, fb = 0, tb = 0;
-  if (j < a.budget) {
-    const int s = a.keep[((long long)b * c.hkv + h) * a.budget + j];
-    if (s >= 0 && s != j) {
-      const int w0 = s / c.block, w1 = j / c.block;
-      bool ok = s >= a.budget && w0 < a.table_w && w1 < a.table_w;
-      if (ok) {
-        fb = table[w0];
-        tb = table[w1];
-        ok = fb >= 0 && fb < c.blocks && tb >= 0 && tb < c.blocks;
-      }
-      if (ok) from = s;
-      else report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_MOVE, b);
-    }
+  const int w0 = s / c.block, w1 = j / c.block, ft = s - w0 * c.block, tt = j - w1 * c.block;
+  bool ok = s >= a.budget && w0 < a.table_w && w1 < a.table_w;
+  const int fb = ok ? table[w0] : -1, tb = ok ? table[w1] : -1;
+  ok = fb >= 0 && fb < c.blocks && tb >= 0 && tb < c.blocks;
+  if (!ok) {
+    if (lane == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_MOVE, b);
+    return;
   }
-  unsigned todo = __ballot_sync(0xffffffffu, from >= 0);
-  const int words = c.d / 8, groups = c.groups();
-  while (todo) {
-    const int l = __ffs(todo) - 1;
-    todo &= todo - 1;
-    const int s = __shfl_sync(0xffffffffu, from, l), sb = __shfl_sync(0xffffffffu, fb, l), db = __shfl_sync(0xffffffffu, tb, l);
-    const int ft = s % c.block, tt = (j - lane + l) % c.block;
-    const long long fp = c.at(sb, h), tp = c.at(db, h);
-    for (int u = lane; u < words; u += 32) {
-      *reinterpret_cast<uint32_t*>(c.k + tp + c.k_word(tt, u)) = *reinterpret_cast<const uint32_t*>(c.k + fp + c.k_word(ft, u));
-      *reinterpret_cast<uint32_t*>(c.v + tp + c.v_word(tt, u)) = *reinterpret_cast<const uint32_t*>(c.v + fp + c.v_word(ft, u));
-    }
-    if (lane < groups) {
-      *reinterpret_cast<uint32_t*>(c.k + tp + c.scale_word(tt, lane)) = *reinterpret_cast<const uint32_t*>(c.k + fp + c.scale_word(ft, lane));
-      *reinterpret_cast<uint32_t*>(c.v + tp + c.scale_word(tt, lane)) = *reinterpret_cast<const uint32_t*>(c.v + fp + c.scale_word(ft, lane));
-    }
-    if (lane == 31) {
-      const long long x = ((long long)sb * c.hkv + h) * c.block + ft, y = ((long long)db * c.hkv + h) * c.block + tt;
-      if (a.weights != nullptr) a.weights[y] = a.weights[x];
-      if (a.positions != nullptr) a.positions[y] = a.positions[x];
-    }
+  const long long fp = c.at(fb, h), tp = c.at(tb, h);
+  Chunk k[PLANES], v[PLANES];
+  uint32_t scale = 0u, number = 0u;
+#pragma unroll
+  for (int p = 0; p < PLANES; ++p) {
+    k[p] = *reinterpret_cast<const Chunk*>(c.k + fp + (p * c.block + ft) * (32 * PER) + lane * (4 * PER));
+    v[p] = *reinterpret_cast<const Chunk*>(c.v + fp + c.v_word(ft, p * 8 * PER + lane));
   }
-}
-
-static int kv4_log2(int x) {
-  int l = 0;
-  while ((1 << l) < x) ++l;
-  return l;
+  const bool of_k = lane < GROUPS, of_v = lane >= 4 && lane - 4 < GROUPS;
+  if (of_k || of_v) scale = *reinterpret_cast<const uint32_t*>((of_k ? c.k : c.v) + fp + c.scale_word(ft, lane & 3));
+  const long long x = ((long long)fb * c.hkv + h) * c.block + ft, y = ((long long)tb * c.hkv + h) * c.block + tt;
+  if (lane == 0 && a.weights != nullptr) number = __float_as_uint(a.weights[x]);
+  if (lane == 1 && a.positions != nullptr) number = (uint32_t)a.positions[x];
+#pragma unroll
+  for (int p = 0; p < PLANES; ++p) {
+    *reinterpret_cast<Chunk*>(c.k + tp + (p * c.block + tt) * (32 * PER) + lane * (4 * PER)) = k[p];
+    *reinterpret_cast<Chunk*>(c.v + tp + c.v_word(tt, p * 8 * PER + lane)) = v[p];
+  }
+  if (of_k || of_v) *reinterpret_cast<uint32_t*>((of_k ? c.k : c.v) + tp + c.scale_word(tt, lane & 3)) = scale;
+  if (lane == 0 && a.weights != nullptr) a.weights[y] = __uint_as_float(number);
+  if (lane == 1 && a.positions != nullptr) a.positions[y] = (int)number;
 }
 
 }  // namespace omni
@@ -441,12 +532,12 @@ extern "C" int omni_kv4_write(const Kv4WriteArgs* p, void* status, cudaStream_t 
   a.weights = p->weights;
   a.positions = p->positions;
   a.token_positions = p->token_positions;
-  const int wl = kv4_log2(p->d / 8);
-  const long long grid = (((p->n * p->hkv * 2) << wl) + 255) / 256;
-  if (grid > 0x7fffffffll) return -3;
+  const unsigned grid = kv4_row_blocks(a, c, 148 * 128);
   const bool vec = ((uintptr_t)p->k | (uintptr_t)p->v) % 16 == 0 && (p->k_row | p->v_row) % 8 == 0 && (p->k_head | p->v_head) % 8 == 0;
-  if (vec) kv4_write_kernel<true><<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
-  else kv4_write_kernel<false><<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
+  const auto kernel = p->d == 64    ? vec ? kv4_write_kernel<64, true> : kv4_write_kernel<64, false>
+                      : p->d == 128 ? vec ? kv4_write_kernel<128, true> : kv4_write_kernel<128, false>
+                                    : vec ? kv4_write_kernel<256, true> : kv4_write_kernel<256, false>;
+  kernel<<<grid, 256, 0, stream>>>(a, c, (OmniStatus*)status);
   return (int)cudaGetLastError();
 }
 
@@ -466,10 +557,9 @@ extern "C" int omni_kv4_read(const Kv4ReadArgs* p, void* status, cudaStream_t st
   a.v_out = (__nv_bfloat16*)p->v_out;
   a.slots = p->slots;
   a.n = p->n;
-  const int wl = kv4_log2(p->d / 8);
-  const long long grid = (((p->n * p->hkv * 2) << wl) + 255) / 256;
-  if (grid > 0x7fffffffll) return -3;
-  kv4_read_kernel<<<(unsigned)grid, 256, 0, stream>>>(a, c, wl, (OmniStatus*)status);
+  const unsigned grid = kv4_row_blocks(a, c, 148 * 64);
+  const auto kernel = p->d == 64 ? kv4_read_kernel<64> : p->d == 128 ? kv4_read_kernel<128> : kv4_read_kernel<256>;
+  kernel<<<grid, 256, 0, stream>>>(a, c, (OmniStatus*)status);
   return (int)cudaGetLastError();
 }
 
@@ -525,6 +615,9 @@ extern "C" int omni_kv4_move(const Kv4MoveArgs* p, void* status, cudaStream_t st
   if (!kv4_shape_ok(c) || p->hkv > 65535 || p->batch > 65535 || p->budget < 1) return -1;
   if (p->batch <= 0) return 0;
   const Kv4Move a = {p->table, p->keep, p->table_ld, p->table_w, p->budget, p->weights, p->positions};
-  kv4_move_kernel<<<dim3((p->budget + 255) / 256, p->hkv, p->batch), 256, 0, stream>>>(a, c, (OmniStatus*)status);
+  const dim3 grid((p->budget + 31) / 32, p->hkv, p->batch);
+  if (p->d == 64) kv4_move_kernel<1><<<grid, 256, 0, stream>>>(a, c, (OmniStatus*)status);
+  else if (p->d == 128) kv4_move_kernel<2><<<grid, 256, 0, stream>>>(a, c, (OmniStatus*)status);
+  else kv4_move_kernel<4><<<grid, 256, 0, stream>>>(a, c, (OmniStatus*)status);
   return (int)cudaGetLastError();
 }
