@@ -50,6 +50,7 @@ struct Kv4Decode {
   int min_tiles;                    // fewest tiles of a block's share; 0: a block takes one item, whole
   float* o_part;                    // [blocks, 2, 8 NT, d]: what a block has of the item that it starts with, and of the one it ends with
   float* lse_part;                  // [blocks, 2, 8 NT]
+  int2* shared;                     // [B, Hkv, chunks]: where the parts of an item start (2 block + which), and how many there are
 };
 
 __device__ __forceinline__ int kv4_length(const Kv4Decode& a, int block, int b, OmniStatus* st) {
@@ -546,6 +547,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     tile0 = (int)(g - ahead - (long long)item * n_tiles);
     left = min(share, all - g);
   }
+  const long long share = left;                                           // of all blocks but the last
   int uses = 0;                                                            // of this warp's stages so far
   for (bool first = true;; first = false) {
     const int h = item / chunks, row0 = (item - h * chunks) * NQ;
@@ -553,6 +555,11 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
     const int first_sees = len - a.rows + 1 + row0 / rep;                  // of the item's first and last rows
     const int end = len - a.rows + 1 + (min(total, row0 + NQ) - 1) / rep;
     const int end_tile = (int)min((long long)n_tiles, tile0 + left);
+    if (a.min_tiles != 0 && tile0 == 0 && threadIdx.x == 0) {              // `share` is whole here unless this block's is the last
+      const long long rest = n_tiles - end_tile;
+      const int more = rest <= 0 ? 0 : rest <= 0x7fffffffll && share <= 0x7fffffffll ? (int)(((unsigned)rest + (unsigned)share - 1) / (unsigned)share) : (int)((rest + share - 1) / share);
+      a.shared[(long long)b * items + item] = make_int2(2 * blockIdx.x + (first ? 0 : 1), 1 + more);
+    }
     const int stop = min(end, end_tile * T::TOKENS);                       // first token behind this part
     const int stop_tile = stop > 0 ? (stop + T::TOKENS - 1) / T::TOKENS : 0;
     int tile = tile0 + warp, next = tile;
@@ -696,40 +703,39 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
 
 // Items that several blocks have worked on, and requests of no tokens: one block for a query row and head, a thread a column.
 template <int NT>
-__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, int B, int blocks, int tokens) {
+__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c) {
   constexpr int NQ = 8 * NT;
   extern __shared__ float s_f[];                                           // [blocks]
-  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ, items = c.hkv * chunks;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ;
   const int h = blockIdx.x / total, row = blockIdx.x - h * total, b = blockIdx.y, d = threadIdx.x, lane = d & 31;
-  const int item = h * chunks + row / NQ, tiles = kv4_tiles(a, c.block, tokens, b);
-  const long long before = kv4_ahead(a, c.block, tokens, items, 0, b);
-  const long long share = kv4_share(a, before + kv4_ahead(a, c.block, tokens, items, b, B), blocks);
-  const long long g0 = before + (long long)item * tiles, g1 = g0 + tiles;
-  const int i0 = (int)(g0 / share), parts = tiles == 0 ? 0 : (int)((g1 - 1) / share) - i0 + 1;
+  const int head = h * rep + row % rep, tok = row / rep;
+  const bool none = a.table_w == 0 || a.seq_lens[b] <= 0;
   // Every block waits, those without work too: a kernel that follows this one may then count on the one ahead of it being done.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int2 shared = none ? make_int2(0, 0) : a.shared[((long long)b * c.hkv + h) * chunks + row / NQ];
+  const int parts = shared.y;
   if (parts == 1) return;                                                  // written by its only block
-  const int first = g0 == (long long)i0 * share ? 0 : 1;                   // where the first of the blocks has its part
-  const long long at = ((long long)i0 * 2) * NQ + row % NQ;
+  // the first part is where its block says, those of the blocks behind it are their first ones
+  const int first = shared.x, next = (first | 1) + 1, in = row % NQ;
+  auto slot = [&](int s) -> long long { return (long long)(s == 0 ? first : next + 2 * (s - 1)) * NQ + in; };
   // every warp finds the maximum and the sum of the parts by itself
   float mm = -INFINITY, sum = 0.f;
-  for (int s = lane; s < parts; s += 32) mm = fmaxf(mm, a.lse_part[at + (s == 0 ? first : 2 * s) * NQ]);
+  for (int s = lane; s < parts; s += 32) mm = fmaxf(mm, a.lse_part[slot(s)]);
   mm = warp_max(mm);
   for (int s = lane; s < parts; s += 32) {
-    const float v = a.lse_part[at + (s == 0 ? first : 2 * s) * NQ], f = v == -INFINITY ? 0.f : exp2f(v - mm);
+    const float v = a.lse_part[slot(s)], f = v == -INFINITY ? 0.f : exp2f(v - mm);
     sum += f;
     if (d < 32) s_f[s] = f;
   }
   sum = warp_sum(sum);
   __syncthreads();
   float acc = 0.f;
-  const float* o = a.o_part + at * c.d + d;
 #pragma unroll 8
   for (int s = 0; s < parts; ++s) {
-    const float f = s_f[s], v = o[(long long)(s == 0 ? first : 2 * s) * NQ * c.d];
+    const float f = s_f[s], v = a.o_part[slot(s) * c.d + d];
     acc += f == 0.f ? 0.f : f * v;
   }
-  const int head = h * rep + row % rep, tok = row / rep;
   a.out[(((long long)b * a.rows + tok) * a.hq + head) * c.d + d] = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
   if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = sum == 0.f ? -INFINITY : mm + __log2f(sum);
 }
@@ -782,7 +788,6 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
     }
   };
   look(tile);
-  asm volatile("griddepcontrol.wait;" ::: "memory");                      // the sums are there
   for (int ch = warp; ch < chunks; ch += KV4_WARPS) {
     Kv4Query<NG> q;
     uint32_t raw[NG][8];
@@ -793,19 +798,17 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
 #pragma unroll
       for (int x = 0; x < 2; ++x)
         s_q[(ch * NG * 2 + g * 2 + x) * 32 + lane] = make_uint4(q.b[g][2 * x][0], q.b[g][2 * x][1], q.b[g][2 * x + 1][0], q.b[g][2 * x + 1][1]);
-    if (r == 0) {                   // of the rows 2 c and 2 c + 1: their sums and units, and then pairs of qs
-      float lse[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int row = ch * 8 + cc * 2 + x;
-        lse[x] = row < total ? a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep] : INFINITY;
-      }
-      s_row[(ch * ROW) * 4 + cc] = make_float4(lse[0], lse[1], q.unit[0], q.unit[1]);
+    if (r == 0) {                   // of the rows 2 c and 2 c + 1: their sums (below) and units, and then pairs of qs
+      s_row[(ch * ROW) * 4 + cc] = make_float4(INFINITY, INFINITY, q.unit[0], q.unit[1]);
 #pragma unroll
       for (int g = 0; g < NG; g += 2)
         s_row[(ch * ROW + 1 + g / 2) * 4 + cc] = make_float4(q.qs[g][0], q.qs[g][1], g + 1 < NG ? q.qs[(g + 1) % NG][0] : 0.f, g + 1 < NG ? q.qs[(g + 1) % NG][1] : 0.f);
     }
   }
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");                      // the sums are there
+  for (int row = threadIdx.x; row < total; row += KV4_WARPS * 32)
+    reinterpret_cast<float*>(&s_row[(row / 8 * ROW) * 4 + row % 8 / 2])[row & 1] = a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep];
   __syncthreads();
   int it = 0;
   for (; tile < tiles; tile += stride, next += stride, ++it) {
@@ -930,7 +933,7 @@ static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int 
   kv4_decode_kernel<NG, NT><<<(unsigned)grid, KV4_WARPS * 32, bytes, stream>>>(a, c, B, st);
   e = cudaGetLastError();
   if (e != cudaSuccess || a.min_tiles == 0) return e;
-  return kv4_follow(kv4_join_kernel<NT>, dim3(c.hkv * total, B), c.d, blocks * 4, stream, a, c, B, blocks, (int)T::TOKENS);
+  return kv4_follow(kv4_join_kernel<NT>, dim3(c.hkv * total, B), c.d, blocks * 4, stream, a, c);
 }
 
 template <int NG>
@@ -955,12 +958,13 @@ using namespace omni;
 // The arguments come in a block, as the caller packs them; 8-byte fields first, so that there are no gaps.
 // row_tile: query rows that share a pass over the cache, 8, or 16 for d <= 128.  min_tiles 0: a block for every item (a row_tile of a
 // key/value head of a request); else `blocks_at_once` blocks share all tiles of 64 tokens (32 for d = 256) equally, at least min_tiles each,
-// and o_part [blocks_at_once, 2, row_tile, d] and lse_part [blocks_at_once, 2, row_tile] take what they have of shared items.
+// and o_part [blocks_at_once, 2, row_tile, d] and lse_part [blocks_at_once, 2, row_tile] take what they have of shared items, `shared` where that is.
 struct Kv4DecodeArgs {
   const void *q, *k_cache, *v_cache;
   const int *table, *seq_lens;
   void* out;
   float *o_part, *lse_part, *lse, *weights;
+  void* shared;                     // int32 [batch, hkv, row tiles, 2]
   long long q_row, blocks;
   int q_head, block, hkv, d, table_ld, table_w, batch, rows, hq, max_len, row_tile, blocks_at_once, min_tiles;
   float scale, decay;
@@ -973,12 +977,12 @@ extern "C" int omni_kv4_decode(const Kv4DecodeArgs* p, void* status, cudaStream_
       (p->row_tile != 8 && (p->row_tile != 16 || d > 128)))
     return -1;
   if (p->weights != nullptr && (p->lse == nullptr || p->rows * rep > 256)) return -2;
-  if (p->min_tiles > 0 && (p->o_part == nullptr || p->lse_part == nullptr || p->blocks_at_once < 1 || p->blocks_at_once > KV4_MAX_BLOCKS)) return -3;
+  if (p->min_tiles > 0 && (p->o_part == nullptr || p->lse_part == nullptr || p->shared == nullptr || p->blocks_at_once < 1 || p->blocks_at_once > KV4_MAX_BLOCKS)) return -3;
   if (B <= 0) return 0;
   const int wide_q = (uintptr_t)p->q % 16 == 0 && p->q_row % 8 == 0 && p->q_head % 8 == 0;
   const Kv4Decode a = {(const __nv_bfloat16*)p->q, p->q_row, p->q_head, wide_q, p->table, p->seq_lens, p->table_ld, p->table_w, p->rows, p->hq,
                        p->scale * 1.4426950408889634f, (__nv_bfloat16*)p->out, p->lse, p->weights, p->decay,
-                       p->block % 64 == 0 ? 64 : p->block % 32 == 0 ? 32 : 16, p->min_tiles, p->o_part, p->lse_part};
+                       p->block % 64 == 0 ? 64 : p->block % 32 == 0 ? 32 : 16, p->min_tiles, p->o_part, p->lse_part, (int2*)p->shared};
   OmniStatus* st = (OmniStatus*)status;
   const bool wide = p->row_tile == 16;
   const int n = p->blocks_at_once;

@@ -174,7 +174,7 @@ _ARGS = {
     "omni_kv4_read": struct.Struct("5Q2q4i"),
     "omni_kv4_keep": struct.Struct("8Q1q10i"),
     "omni_kv4_move": struct.Struct("6Q1q8i"),
-    "omni_kv4_decode": struct.Struct("10Q2q13i2fi"),
+    "omni_kv4_decode": struct.Struct("11Q2q13i2fi"),
 }
 _bound = {}
 
@@ -319,13 +319,14 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
         items = B * hkv * -(-total // tile)
         blocks_at_once, min_tiles = _blocks(items, -(-longest // (32 if d == 256 else 64)), 3 if tile * d <= 1024 else 2)
         lse = torch.empty(T * hq, dtype=torch.float32, device=q.device) if weights is not None else None
-        o_part = lse_part = None
-        if min_tiles:
+        o_part = lse_part = shared = 0
+        if min_tiles:                                        # partial results, their sums, where the parts of an item are
             n = blocks_at_once * 2 * tile
-            o_part = torch.empty(n * (d + 1), dtype=torch.float32, device=q.device)
-            lse_part = o_part[n * d:]
-        _call("omni_kv4_decode", q.device, _p(q), _p(k_cache), _p(v_cache), _p(block_table), _p(seq_lens), _p(out), _p(o_part), _p(lse_part), _p(lse),
-              _p(weights), q.stride(0), blocks, q.stride(1), block, hkv, d, block_table.stride(0), width, B, T // B, hq, longest, tile,
+            scratch = torch.empty(n * (d + 1) + 2 * items, dtype=torch.float32, device=q.device)
+            o_part = scratch.data_ptr()
+            lse_part, shared = o_part + 4 * n * d, o_part + 4 * n * (d + 1)
+        _call("omni_kv4_decode", q.device, _p(q), _p(k_cache), _p(v_cache), _p(block_table), _p(seq_lens), _p(out), o_part, lse_part, _p(lse),
+              _p(weights), shared, q.stride(0), blocks, q.stride(1), block, hkv, d, block_table.stride(0), width, B, T // B, hq, longest, tile,
               blocks_at_once, min_tiles, scale, decay, 0)
     return out
 
