@@ -187,8 +187,9 @@ def _call(name, device, *args):
         getattr(lib._cdll, name).argtypes = (ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p)
         call = _bound[name] = (getattr(lib, name), _ARGS[name].pack)
     fn, pack = call
-    status, stream = nat.status_buffer(device).data_ptr(), torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
+    index = device.index
+    status, stream = (nat._status.get(index) if index in nat._status else nat.status_buffer(index)).data_ptr(), torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
         rc = fn(pack(*args), status, stream)
     else:
         with torch.cuda.device(device):
@@ -202,52 +203,54 @@ def _p(t):
 
 
 def _check_caches(k_cache, v_cache):
-    """(blocks, Hkv, block, d) of a pair of caches."""
-    assert k_cache.dtype == v_cache.dtype == torch.uint8 and k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "a pair of uint8 caches of one shape"
-    assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.device == v_cache.device, "contiguous caches on one device"
-    blocks, hkv, block, row = k_cache.shape
+    """(blocks, Hkv, block, d, device) of a pair of caches."""
+    shape, device = k_cache.shape, k_cache.device
+    assert k_cache.dtype is torch.uint8 and v_cache.dtype is torch.uint8 and len(shape) == 4 and shape == v_cache.shape, "a pair of uint8 caches of one shape"
+    assert k_cache.is_contiguous() and v_cache.is_contiguous() and device == v_cache.device, "contiguous caches on one device"
+    blocks, hkv, block, row = shape
     d = row * 16 // 9
     assert d in DIMS and row * 16 == d * 9 and block > 0 and block % 16 == 0 and hkv > 0, \
         f"rows of 9 d / 16 bytes with d in {DIMS} and blocks of a multiple of 16 tokens: {row}, {block}"
-    return blocks, hkv, block, d
+    return blocks, hkv, block, d, device
 
 
-def _check_ints(device, dtype=torch.int32, **tensors):
-    for name, t in tensors.items():
-        assert t.dtype == dtype and t.device == device and (t.dim() == 0 or t.stride(-1) == 1), f"{name}: {dtype} on {device}, rows without gaps"
+def _check_rows(name, x, hkv, d, device):
+    assert x.dtype is torch.bfloat16 and x.device == device and x.dim() == 3 and x.stride(2) == 1 and x.shape[2] == d and (hkv is None or x.shape[1] == hkv), \
+        f"{name}: bf16 [rows, {'heads' if hkv is None else hkv}, {d}] on {device}, columns without gaps"
 
 
-def _check_per_place(device, shape, **tensors):
+def _check_numbers(name, x, n, device, dtype=torch.int32):
+    """One number for each of n requests or tokens (any number of them: n None)."""
+    assert x.dtype is dtype and x.device == device and x.dim() == 1 and x.is_contiguous() and (n is None or x.shape[0] == n), \
+        f"{name}: contiguous {dtype} [{'n' if n is None else n}] on {device}"
+
+
+def _check_per_place(name, x, shape, device, dtype=torch.float32):
     """``weights`` and ``positions``: a number for every place of the caches."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        dtype = torch.int32 if name == "positions" else torch.float32
-        assert t.dtype == dtype and t.device == device and t.is_contiguous() and tuple(t.shape) == shape, f"{name}: contiguous {dtype} {list(shape)}"
+    assert x.dtype is dtype and x.device == device and x.is_contiguous() and x.shape == shape, f"{name}: contiguous {dtype} {list(shape)} on {device}"
 
 
 def _check_table(table, device, B):
-    _check_ints(device, block_table=table)
-    assert table.dim() == 2 and table.shape[0] >= B, f"block_table: a row for each of the {B} requests"
+    assert table.dtype is torch.int32 and table.device == device and table.dim() == 2 and table.shape[0] >= B and table.stride(1) == 1, \
+        f"block_table: int32 on {device}, a row without gaps for each of the {B} requests"
 
 
 def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token_positions=None):
     """Rows k, v [T, Hkv, d] (bf16; any row and head pitch) into the slots ``slots`` [T] int64 (block * block size + place in the
     block; negative: not stored).  The slots of a call differ.  ``weights`` / ``positions`` [blocks, Hkv, block], where given, are
     set to 0 and to ``token_positions`` [T] int64 in those slots."""
-    blocks, hkv, block, d = _check_caches(k_cache, v_cache)
-    for name, x in (("k", k), ("v", v)):
-        assert x.dim() == 3 and x.dtype == torch.bfloat16 and x.shape[1:] == (hkv, d) and x.device == k_cache.device, \
-            f"{name}: bf16 [T, {hkv}, {d}] on {k_cache.device}"
-        assert x.stride(2) == 1, f"{name}: columns without gaps"
+    blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
+    _check_rows("k", k, hkv, d, device)
+    _check_rows("v", v, hkv, d, device)
     T = k.shape[0]
-    _check_ints(k.device, torch.int64, slots=slots)
-    assert v.shape[0] == T and slots.shape == (T,), "a row of v and a slot for every row of k"
-    _check_per_place(k.device, (blocks, hkv, block), weights=weights, positions=positions)
+    assert v.shape[0] == T, "a row of v for every row of k"
+    _check_numbers("slots", slots, T, device, torch.int64)
     assert (positions is None) == (token_positions is None), "positions and token_positions come together"
-    if token_positions is not None:
-        _check_ints(k.device, torch.int64, token_positions=token_positions)
-        assert token_positions.shape == (T,)
+    if weights is not None:
+        _check_per_place("weights", weights, (blocks, hkv, block), device)
+    if positions is not None:
+        _check_per_place("positions", positions, (blocks, hkv, block), device, torch.int32)
+        _check_numbers("token_positions", token_positions, T, device, torch.int64)
     if not k.is_cuda:
         _write_ref(k, slots, k_cache, False)
         _write_ref(v, slots, v_cache, True)
@@ -260,23 +263,23 @@ def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token
         return
     if T == 0:
         return
-    _call("omni_kv4_write", k.device, _p(k), _p(v), _p(slots), _p(k_cache), _p(v_cache), _p(weights), _p(positions), _p(token_positions),
+    _call("omni_kv4_write", device, k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(weights), _p(positions), _p(token_positions),
           k.stride(0), v.stride(0), T, blocks, k.stride(1), v.stride(1), block, hkv, d, 0)
 
 
 def kv4_read(k_cache, v_cache, slots):
     """(k, v) [T, Hkv, d] bf16 of the slots ``slots`` [T] int64; zeros for negative ones.  A slot may be named more than once."""
-    blocks, hkv, block, d = _check_caches(k_cache, v_cache)
-    _check_ints(k_cache.device, torch.int64, slots=slots)
-    assert slots.dim() == 1
+    blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
+    _check_numbers("slots", slots, None, device, torch.int64)
     T = slots.shape[0]
     if not k_cache.is_cuda:
         s = slots.clamp_min(0)
         ok = (slots >= 0)[:, None, None]
         return tuple(torch.where(ok, _values_ref(c, s // block, s % block, x), torch.zeros(())).bfloat16() for c, x in ((k_cache, False), (v_cache, True)))
-    k, v = (torch.empty(T, hkv, d, dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
+    k = torch.empty((T, hkv, d), dtype=torch.bfloat16, device=device)
+    v = torch.empty((T, hkv, d), dtype=torch.bfloat16, device=device)
     if T:
-        _call("omni_kv4_read", k_cache.device, _p(k_cache), _p(v_cache), _p(slots), _p(k), _p(v), T, blocks, block, hkv, d, 0)
+        _call("omni_kv4_read", device, k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, blocks, block, hkv, d, 0)
     return k, v
 
 
@@ -298,19 +301,18 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
     would write the same numbers: give ``weights`` only where blocks belong to one request.  At most 256 rows times query
     heads of a key/value head then.  ``max_seq_len`` (a bound of
     ``seq_lens``) shapes the launch; without it the width of the block table does."""
-    blocks, hkv, block, d = _check_caches(k_cache, v_cache)
-    assert q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == d and q.device == k_cache.device and q.stride(2) == 1, \
-        f"q: bf16 [rows, Hq, {d}] on {k_cache.device}, columns without gaps"
+    blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
+    _check_rows("q", q, None, d, device)
+    _check_numbers("seq_lens", seq_lens, None, device)
     T, hq, B = q.shape[0], q.shape[1], seq_lens.shape[0]
     assert hq > 0 and hq % hkv == 0, f"{hq} query heads do not divide over {hkv} key/value heads"
     assert T == 0 if B == 0 else T > 0 and T % B == 0, f"{T} rows are not the same number for each of {B} requests"
-    _check_ints(q.device, seq_lens=seq_lens)
-    assert seq_lens.dim() == 1
-    _check_table(block_table, q.device, B)
-    _check_per_place(q.device, (blocks, hkv, block), weights=weights)
+    _check_table(block_table, device, B)
+    if weights is not None:
+        _check_per_place("weights", weights, (blocks, hkv, block), device)
     if not q.is_cuda:
         return kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights, decay)
-    out = torch.empty(T, hq, d, dtype=q.dtype, device=q.device)
+    out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=device)
     if T:
         width, total = block_table.shape[1], T // B * (hq // hkv)
         assert weights is None or total <= 256, f"weights of at most 256 query rows a key/value head at once: {total}"
@@ -318,15 +320,15 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
         tile = 16 if d <= 128 and total > 8 else 8
         items = B * hkv * -(-total // tile)
         blocks_at_once, min_tiles = _blocks(items, -(-longest // (32 if d == 256 else 64)), 3 if tile * d <= 1024 else 2)
-        lse = torch.empty(T * hq, dtype=torch.float32, device=q.device) if weights is not None else None
+        lse = torch.empty(T * hq, dtype=torch.float32, device=device) if weights is not None else None
         o_part = lse_part = shared = 0
         if min_tiles:                                        # partial results, their sums, where the parts of an item are
             n = blocks_at_once * 2 * tile
-            scratch = torch.empty(n * (d + 1) + 2 * items, dtype=torch.float32, device=q.device)
+            scratch = torch.empty(n * (d + 1) + 2 * items, dtype=torch.float32, device=device)
             o_part = scratch.data_ptr()
             lse_part, shared = o_part + 4 * n * d, o_part + 4 * n * (d + 1)
-        _call("omni_kv4_decode", q.device, _p(q), _p(k_cache), _p(v_cache), _p(block_table), _p(seq_lens), _p(out), o_part, lse_part, _p(lse),
-              _p(weights), shared, q.stride(0), blocks, q.stride(1), block, hkv, d, block_table.stride(0), width, B, T // B, hq, longest, tile,
+        _call("omni_kv4_decode", device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(),
+              o_part, lse_part, _p(lse), _p(weights), shared, q.stride(0), blocks, q.stride(1), block, hkv, d, block_table.stride(0), width, B, T // B, hq, longest, tile,
               blocks_at_once, min_tiles, scale, decay, 0)
     return out
 
@@ -341,24 +343,26 @@ def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first
     places that become free; -1 from lens[b] on.  Nothing is moved: see ``kv4_move``.  ``max_seq_len``
     as in ``kv4_decode``."""
     assert weights.dim() == 3, "weights: [blocks, Hkv, block]"
-    device = weights.device
-    blocks, hkv, block = weights.shape
-    _check_per_place(device, (blocks, hkv, block), weights=weights, positions=positions)
+    device, shape = weights.device, weights.shape
+    blocks, hkv, block = shape
+    _check_per_place("weights", weights, shape, device)
+    _check_per_place("positions", positions, shape, device, torch.int32)
+    _check_numbers("seq_lens", seq_lens, None, device)
     B = seq_lens.shape[0]
-    _check_ints(device, seq_lens=seq_lens, seen=seen)
-    assert seq_lens.shape == seen.shape == (B,)
+    _check_numbers("seen", seen, B, device)
     _check_table(block_table, device, B)
     assert budget >= 1 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, \
         f"a budget of {budget} tokens holds at least the {keep_first} first and {keep_last} last ones"
     if not weights.is_cuda:
         return kv4_keep_ref(weights, positions, block_table, seq_lens, seen, budget, keep_first, keep_last)
-    keep = torch.empty(B, hkv, budget, dtype=torch.int32, device=device)
+    keep = torch.empty((B, hkv, budget), dtype=torch.int32, device=device)
     lens = torch.empty(B, dtype=torch.int32, device=device)
     if B:
-        scratch = torch.empty_like(keep)
+        scratch = torch.empty((B, hkv, budget), dtype=torch.int32, device=device)
         width = block_table.shape[1]
         longest = width * block if max_seq_len is None else max(0, min(max_seq_len, width * block))
-        _call("omni_kv4_keep", device, _p(weights), _p(positions), _p(block_table), _p(seq_lens), _p(seen), _p(keep), _p(lens), _p(scratch), blocks,
+        _call("omni_kv4_keep", device, weights.data_ptr(), positions.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), seen.data_ptr(),
+              keep.data_ptr(), lens.data_ptr(), scratch.data_ptr(), blocks,
               block, hkv, block_table.stride(0), width, B, budget, keep_first, keep_last, longest, 0)
     return keep, lens
 
@@ -367,15 +371,17 @@ def kv4_move(k_cache, v_cache, block_table, keep, weights=None, positions=None):
     """Brings the tokens that ``keep`` [B, Hkv, budget] names (see ``kv4_keep``) to their places, in place, with their weights and
     positions where given.  What other places hold is left.  Requests that share a block would lose tokens of one another: copy
     such blocks first."""
-    blocks, hkv, block, d = _check_caches(k_cache, v_cache)
-    device = k_cache.device
-    assert keep.dim() == 3 and keep.shape[1] == hkv and keep.is_contiguous() and keep.dtype == torch.int32 and keep.device == device, \
+    blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
+    assert keep.dim() == 3 and keep.shape[1] == hkv and keep.is_contiguous() and keep.dtype is torch.int32 and keep.device == device, \
         f"keep: contiguous int32 [B, {hkv}, budget] on {device}"
     B, _, budget = keep.shape
     _check_table(block_table, device, B)
-    _check_per_place(device, (blocks, hkv, block), weights=weights, positions=positions)
+    if weights is not None:
+        _check_per_place("weights", weights, (blocks, hkv, block), device)
+    if positions is not None:
+        _check_per_place("positions", positions, (blocks, hkv, block), device, torch.int32)
     if not k_cache.is_cuda:
         _move_ref(k_cache, v_cache, block_table, keep, weights, positions)
     elif B and budget:
-        _call("omni_kv4_move", device, _p(k_cache), _p(v_cache), _p(block_table), _p(keep), _p(weights), _p(positions), blocks, block, hkv, d,
+        _call("omni_kv4_move", device, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), keep.data_ptr(), _p(weights), _p(positions), blocks, block, hkv, d,
               block_table.stride(0), block_table.shape[1], B, budget, 0)
