@@ -157,10 +157,10 @@ __device__ __forceinline__ void kv4_lds(uint32_t (&w)[N], const uint8_t* p) {
   }
 }
 
-template <int NG, bool VALUES>
+template <int NG, bool VALUES, int TOK = NG == 4 ? 32 : 64>
 struct Kv4Tile {
   static constexpr int PER = NG > 1 ? 2 : 1, PLANES = NG / PER;
-  static constexpr int TOKENS = NG == 4 ? 32 : 64;
+  static constexpr int TOKENS = TOK;
   static constexpr int CODES = TOKENS * 32 * NG, SCALES = TOKENS * 4 * NG;
   static constexpr int V0 = CODES, KS0 = VALUES ? 2 * CODES : CODES, VS0 = KS0 + SCALES;
   static constexpr int BYTES = VALUES ? 2 * (CODES + SCALES) : CODES + SCALES;
@@ -171,9 +171,9 @@ struct Kv4Tile {
 // The copies of a warp's tiles: lane l copies one kind of data (a plane of codes, the scales) of one run of `piece` tokens of a tile,
 // which lies in one block.  The block ids of 32 runs are fetched by one load, another 32 runs ahead of their use: with the copies of
 // all warps under way, a load that is waited for takes microseconds.
-template <int NG, bool VALUES>
+template <int NG, bool VALUES, int TOK = NG == 4 ? 32 : 64>
 struct Kv4Feed {
-  using T = Kv4Tile<NG, VALUES>;
+  using T = Kv4Tile<NG, VALUES, TOK>;
   const uint8_t* base;              // of this lane's kind and head, in block 0
   long long blk_bytes;
   const int* table;
@@ -298,9 +298,9 @@ struct Kv4Query {
 };
 
 // Key codes minus 8 of 16 tokens of a staged tile
-template <int NG, bool VALUES>
+template <int NG, bool VALUES, int TOK = NG == 4 ? 32 : 64>
 struct Kv4Keys {
-  using T = Kv4Tile<NG, VALUES>;
+  using T = Kv4Tile<NG, VALUES, TOK>;
   uint32_t w[T::PLANES][2][2 * T::PER], sc[2][NG];
   __device__ __forceinline__ void load(const uint8_t* stage, int sub) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
@@ -743,153 +743,169 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c) 
 // The weights that the rows give a request's tokens: the scores of the staged keys once more, against the finished sums.  Reading the
 // keys twice costs as much as keeping the scores of 8 query rows would, and nothing more for more rows; 16 tokens are unpacked once for
 // all rows, whose fragments stand in shared memory.
-template <int NG>
-__global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decode a, Kv4Cache c, OmniStatus* st) {
-  using T = Kv4Tile<NG, false>;
+template <int NG, int TOK>
+__global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decode a, Kv4Cache c, int B, OmniStatus* st) {
+  using T = Kv4Tile<NG, false, TOK>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[KV4_WARPS * KV4_STAGES];
   __shared__ int abort_flag;
+  __shared__ float s_w[KV4_WARPS][TOK];
+  constexpr int ROW = 1 + (NG + 1) / 2, EACH = (TOK + 31) / 32;
   const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + 7) / 8;
-  const int h = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
-  const int len = kv4_length(a, c.block, b, st), tiles = (len + T::TOKENS - 1) / T::TOKENS;
-  const int stride = gridDim.x * KV4_WARPS;
-  if (blockIdx.x * KV4_WARPS >= tiles) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");                    // as in the join
-    return;
-  }
   uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
   uint4* s_q = reinterpret_cast<uint4*>(smem + KV4_WARPS * KV4_STAGES * T::BYTES);      // [chunks][NG][2][32]
-  float4* s_row = reinterpret_cast<float4*>(s_q + chunks * NG * 64);                     // [chunks][1 + NG / 2][4]: see below
-  __shared__ float s_w[KV4_WARPS][T::TOKENS];
-  constexpr int ROW = 1 + (NG + 1) / 2;
+  float4* s_row = reinterpret_cast<float4*>(s_q + chunks * NG * 64);                     // [chunks][ROW][4]: see below
   uint64_t* bar = bars + warp * KV4_STAGES;
   if (threadIdx.x == 0) abort_flag = 0;
   if (lane == 0) {
     for (int s = 0; s < KV4_STAGES; ++s) mbar_init(bar + s, 1);
     mbar_fence_init();
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_proxy_async_smem();
   }
   __syncthreads();
-  int tile = blockIdx.x * KV4_WARPS + warp, next = tile;
-  Kv4Feed<NG, false> feed;
-  feed.init(a, c, b, h, tile, stride, len);
-#pragma unroll
-  for (int s = 0; s < KV4_STAGES; ++s, next += stride)
-    if (next < tiles) feed.start(a, c, min(T::TOKENS, (len - next * T::TOKENS + 15) & ~15), len, stages + s * T::BYTES, bar + s, st);
-  // the places of the weights of a lane's tokens of the next tile
-  constexpr int EACH = T::TOKENS / 32;
-  int place[EACH];
-  auto look = [&](int of) {
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int t = of * T::TOKENS + i * 32 + lane;
-      place[i] = of < tiles && t < len ? a.table[(long long)b * a.table_ld + t / c.block] : -1;
-    }
-  };
-  look(tile);
-  for (int ch = warp; ch < chunks; ch += KV4_WARPS) {
-    Kv4Query<NG> q;
-    uint32_t raw[NG][8];
-    Kv4Query<NG>::fetch(a, rep, b, h, ch * 8 + r, total, raw);
-    q.make(raw, a.scale_log2);
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        s_q[(ch * NG * 2 + g * 2 + x) * 32 + lane] = make_uint4(q.b[g][2 * x][0], q.b[g][2 * x][1], q.b[g][2 * x + 1][0], q.b[g][2 * x + 1][1]);
-    if (r == 0) {                   // of the rows 2 c and 2 c + 1: their sums (below) and units, and then pairs of qs
-      s_row[(ch * ROW) * 4 + cc] = make_float4(INFINITY, INFINITY, q.unit[0], q.unit[1]);
-#pragma unroll
-      for (int g = 0; g < NG; g += 2)
-        s_row[(ch * ROW + 1 + g / 2) * 4 + cc] = make_float4(q.qs[g][0], q.qs[g][1], g + 1 < NG ? q.qs[(g + 1) % NG][0] : 0.f, g + 1 < NG ? q.qs[(g + 1) % NG][1] : 0.f);
-    }
+  // shares as in the decode kernel, an item being a key/value head of a request
+  const long long all = kv4_ahead(a, c.block, TOK, c.hkv, 0, B);
+  const long long even = (all + gridDim.x - 1) / gridDim.x, share = even > KV4_WARPS ? even : KV4_WARPS, g = blockIdx.x * share;
+  if (g >= all) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");                    // as in the join
+    return;
   }
-  __syncthreads();
-  asm volatile("griddepcontrol.wait;" ::: "memory");                      // the sums are there
-  for (int row = threadIdx.x; row < total; row += KV4_WARPS * 32)
-    reinterpret_cast<float*>(&s_row[(row / 8 * ROW) * 4 + row % 8 / 2])[row & 1] = a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep];
-  __syncthreads();
-  int it = 0;
-  for (; tile < tiles; tile += stride, next += stride, ++it) {
-    const int st_i = it % KV4_STAGES;
-    uint8_t* stage = stages + st_i * T::BYTES;
-    float* to[EACH];
-    float old[EACH];
+  long long ahead, left = min(share, all - g);
+  int b = kv4_find(a, c.block, TOK, c.hkv, B, g, ahead), n_tiles = kv4_tiles(a, c.block, TOK, b);
+  int h = (int)((g - ahead) / n_tiles), tile0 = (int)(g - ahead - (long long)h * n_tiles), uses = 0;
+  for (bool first = true;; first = false) {
+    const int len = kv4_length(a, c.block, b, st), end_tile = (int)min((long long)n_tiles, tile0 + left), stop = min(len, end_tile * TOK);
+    int tile = tile0 + warp, next = tile;
+    Kv4Feed<NG, false, TOK> feed;
+    feed.init(a, c, b, h, tile, KV4_WARPS, stop);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int t = tile * T::TOKENS + i * 32 + lane;
-      to[i] = place[i] >= 0 && place[i] < c.blocks ? a.weights + ((long long)place[i] * c.hkv + h) * c.block + t % c.block : nullptr;
-      old[i] = to[i] != nullptr && a.decay != 0.f ? *to[i] : 0.f;
+    for (int s = 0; s < KV4_STAGES; ++s, next += KV4_WARPS) {
+      const int i = (uses + s) % KV4_STAGES;
+      if (next < end_tile) feed.start(a, c, min(TOK, (len - next * TOK + 15) & ~15), stop, stages + i * T::BYTES, bar + i, st);
     }
-    look(tile + stride);
-    if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (it / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_WEIGHTS, tile))) break;
-#pragma unroll 1
-    for (int u = 0; u < T::TOKENS / 16; ++u) {
-      const int t0 = tile * T::TOKENS + u * 16;
-      if (t0 >= len) break;
-      const bool edge = t0 + 16 > len - a.rows + 1;
-      Kv4Keys<NG, false> k;
-      k.load(stage, u);
-      uint32_t f[NG][4][4];
+    // the blocks of a lane's tokens of the next tile
+    int place[EACH];
+    auto look = [&](int of) {
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+      for (int i = 0; i < EACH; ++i) {
+        const int t = of * TOK + i * 32 + lane;
+        place[i] = (EACH > 1 || lane < TOK) && t < stop ? a.table[(long long)b * a.table_ld + t / c.block] : -1;
+      }
+    };
+    look(tile);
+    for (int ch = warp; ch < chunks; ch += KV4_WARPS) {
+      Kv4Query<NG> q;
+      uint32_t raw[NG][8];
+      Kv4Query<NG>::fetch(a, rep, b, h, ch * 8 + r, total, raw);
+      q.make(raw, a.scale_log2);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) k.fragment(g, x, f[g][x]);
-      float w[2] = {0.f, 0.f};
-#pragma unroll 1
-      for (int ch = 0; ch < chunks; ++ch) {
-        const float4 row = s_row[ch * ROW * 4 + cc];
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint4 v = s_q[(ch * NG * 2 + g * 2 + x) * 32 + lane];
-            const uint32_t b0[2] = {v.x, v.y}, b1[2] = {v.z, v.w};
-            kv4_mma(acc, f[g][2 * x], b0);
-            kv4_mma(acc, f[g][2 * x + 1], b1);
-          }
-          const float4 sums = s_row[(ch * ROW + 1 + g / 2) * 4 + cc];
-          const float qs[2] = {g & 1 ? sums.z : sums.x, g & 1 ? sums.w : sums.y};
-          const uint32_t word[2] = {k.sc[0][g], k.sc[1][g]};
-          kv4_score(s, acc, word, qs);
-        }
+      for (int g2 = 0; g2 < NG; ++g2)
 #pragma unroll
         for (int x = 0; x < 2; ++x)
+          s_q[(ch * NG * 2 + g2 * 2 + x) * 32 + lane] = make_uint4(q.b[g2][2 * x][0], q.b[g2][2 * x][1], q.b[g2][2 * x + 1][0], q.b[g2][2 * x + 1][1]);
+      if (r == 0) {                 // of the rows 2 c and 2 c + 1: their sums (below) and units, and then pairs of qs
+        s_row[(ch * ROW) * 4 + cc] = make_float4(INFINITY, INFINITY, q.unit[0], q.unit[1]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float p = ex2_fast(fmaf(s[2 * e + x], x ? row.w : row.z, -(x ? row.y : row.x)));
-            if (edge || (ch + 1) * 8 > total) {                            // rows beyond the last, tokens that the row does not see
-              const int i = ch * 8 + cc * 2 + x;
-              if (i >= total || t0 + r + 8 * e >= len - a.rows + 1 + i / rep) p = 0.f;
-            }
-            w[e] += p;
-          }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        w[e] += __shfl_xor_sync(0xffffffffu, w[e], 1);
-        w[e] += __shfl_xor_sync(0xffffffffu, w[e], 2);
-        if (cc == 0) s_w[warp][u * 16 + r + 8 * e] = w[e];
+        for (int g2 = 0; g2 < NG; g2 += 2)
+          s_row[(ch * ROW + 1 + g2 / 2) * 4 + cc] =
+              make_float4(q.qs[g2][0], q.qs[g2][1], g2 + 1 < NG ? q.qs[(g2 + 1) % NG][0] : 0.f, g2 + 1 < NG ? q.qs[(g2 + 1) % NG][1] : 0.f);
       }
     }
-    __syncwarp();
+    __syncthreads();
+    if (first) asm volatile("griddepcontrol.wait;" ::: "memory");         // the sums are there
+    for (int row = threadIdx.x; row < total; row += KV4_WARPS * 32)
+      reinterpret_cast<float*>(&s_row[(row / 8 * ROW) * 4 + row % 8 / 2])[row & 1] = a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep];
+    __syncthreads();
+    for (; tile < end_tile; tile += KV4_WARPS, next += KV4_WARPS, ++uses) {
+      const int st_i = uses % KV4_STAGES;
+      uint8_t* stage = stages + st_i * T::BYTES;
+      float* to[EACH];
+      float old[EACH];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i)
-      if (to[i] != nullptr) *to[i] = a.decay == 0.f ? s_w[warp][i * 32 + lane] : fmaf(a.decay, old[i], s_w[warp][i * 32 + lane]);
-    __syncwarp();
-    if (next < tiles) feed.start(a, c, min(T::TOKENS, (len - next * T::TOKENS + 15) & ~15), len, stage, bar + st_i, st);
-  }
-  __syncthreads();
-  if (abort_flag != 0) {
-    if (threadIdx.x == 0) report_abort(&abort_flag, st);
-    for (int s = 0; s < KV4_STAGES; ++s) {
-      const int left = it + s;
-      if (tile + s * stride < tiles) {
-        for (int i = 0; i < 1 << 16 && !mbar_try_wait(bar + left % KV4_STAGES, (left / KV4_STAGES) & 1); ++i) {}
+      for (int i = 0; i < EACH; ++i) {
+        const int t = tile * TOK + i * 32 + lane;
+        to[i] = place[i] >= 0 && place[i] < c.blocks ? a.weights + ((long long)place[i] * c.hkv + h) * c.block + t % c.block : nullptr;
+        old[i] = to[i] != nullptr && a.decay != 0.f ? *to[i] : 0.f;
       }
+      look(tile + KV4_WARPS);
+      if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (uses / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_WEIGHTS, tile))) break;
+#pragma unroll 1
+      for (int u = 0; u < TOK / 16; ++u) {
+        const int t0 = tile * TOK + u * 16;
+        if (t0 >= len) break;
+        const bool edge = t0 + 16 > len - a.rows + 1;
+        Kv4Keys<NG, false, TOK> k;
+        k.load(stage, u);
+        uint32_t f[NG][4][4];
+#pragma unroll
+        for (int g2 = 0; g2 < NG; ++g2)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) k.fragment(g2, x, f[g2][x]);
+        float w[2] = {0.f, 0.f};
+#pragma unroll 1
+        for (int ch = 0; ch < chunks; ++ch) {
+          const float4 row = s_row[ch * ROW * 4 + cc];
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int g2 = 0; g2 < NG; ++g2) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint4 v = s_q[(ch * NG * 2 + g2 * 2 + x) * 32 + lane];
+              const uint32_t b0[2] = {v.x, v.y}, b1[2] = {v.z, v.w};
+              kv4_mma(acc, f[g2][2 * x], b0);
+              kv4_mma(acc, f[g2][2 * x + 1], b1);
+            }
+            const float4 sums = s_row[(ch * ROW + 1 + g2 / 2) * 4 + cc];
+            const float qs[2] = {g2 & 1 ? sums.z : sums.x, g2 & 1 ? sums.w : sums.y};
+            const uint32_t word[2] = {k.sc[0][g2], k.sc[1][g2]};
+            kv4_score(s, acc, word, qs);
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float p = ex2_fast(fmaf(s[2 * e + x], x ? row.w : row.z, -(x ? row.y : row.x)));
+              if (edge || (ch + 1) * 8 > total) {                         // rows beyond the last, tokens that the row does not see
+                const int i = ch * 8 + cc * 2 + x;
+                if (i >= total || t0 + r + 8 * e >= len - a.rows + 1 + i / rep) p = 0.f;
+              }
+              w[e] += p;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          w[e] += __shfl_xor_sync(0xffffffffu, w[e], 1);
+          w[e] += __shfl_xor_sync(0xffffffffu, w[e], 2);
+          if (cc == 0) s_w[warp][u * 16 + r + 8 * e] = w[e];
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < EACH; ++i)
+        if (to[i] != nullptr) *to[i] = a.decay == 0.f ? s_w[warp][i * 32 + lane] : fmaf(a.decay, old[i], s_w[warp][i * 32 + lane]);
+      __syncwarp();
+      if (next < end_tile) feed.start(a, c, min(TOK, (len - next * TOK + 15) & ~15), stop, stage, bar + st_i, st);
+    }
+    __syncthreads();
+    if (abort_flag != 0) {
+      if (threadIdx.x == 0) report_abort(&abort_flag, st);
+      for (int s = 0; s < KV4_STAGES; ++s) {
+        const int i = uses + s;
+        if (tile + s * KV4_WARPS < end_tile) {
+          for (int k = 0; k < 1 << 16 && !mbar_try_wait(bar + i % KV4_STAGES, (i / KV4_STAGES) & 1); ++k) {}
+        }
+      }
+      return;
+    }
+    left -= end_tile - tile0;
+    if (left <= 0) return;
+    tile0 = 0;
+    if (++h == c.hkv) {
+      h = 0;
+      do n_tiles = kv4_tiles(a, c.block, TOK, ++b);
+      while (n_tiles == 0);
     }
   }
 }
@@ -936,19 +952,16 @@ static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int 
   return kv4_follow(kv4_join_kernel<NT>, dim3(c.hkv * total, B), c.d, blocks * 4, stream, a, c);
 }
 
-template <int NG>
+template <int NG, int TOK>
 static cudaError_t kv4_launch_weights(const Kv4Decode& a, const Kv4Cache& c, int B, int max_len, OmniStatus* st, cudaStream_t stream) {
-  using T = Kv4Tile<NG, false>;
   const int total = a.rows * (a.hq / c.hkv), chunks = (total + 7) / 8;
-  const int bytes = KV4_WARPS * KV4_STAGES * T::BYTES + chunks * (NG * 64 * 16 + (1 + (NG + 1) / 2) * 4 * 16);
+  const int bytes = KV4_WARPS * KV4_STAGES * Kv4Tile<NG, false, TOK>::BYTES + chunks * (NG * 64 * 16 + (1 + (NG + 1) / 2) * 4 * 16);
   static int most[64] = {0};
-  cudaError_t e = kv4_smem((const void*)kv4_weights_kernel<NG>, bytes, most);
+  cudaError_t e = kv4_smem((const void*)kv4_weights_kernel<NG, TOK>, bytes, most);
   if (e != cudaSuccess) return e;
-  const long long tiles = (max_len + T::TOKENS - 1) / T::TOKENS, items = (long long)B * c.hkv;
-  long long parts = 148 * 3 / items;
-  if (parts > (tiles + KV4_WARPS - 1) / KV4_WARPS) parts = (tiles + KV4_WARPS - 1) / KV4_WARPS;
-  if (parts < 1) parts = 1;
-  return kv4_follow(kv4_weights_kernel<NG>, dim3((unsigned)parts, c.hkv, B), KV4_WARPS * 32, bytes, stream, a, c, st);
+  const long long shares = ((long long)B * c.hkv * ((max_len + TOK - 1) / TOK) + KV4_WARPS - 1) / KV4_WARPS, resident = 148 * 3;
+  const unsigned grid = (unsigned)(shares < 1 ? 1 : shares < resident ? shares : resident);
+  return kv4_follow(kv4_weights_kernel<NG, TOK>, dim3(grid), KV4_WARPS * 32, bytes, stream, a, c, B, st);
 }
 
 }  // namespace omni
@@ -990,7 +1003,11 @@ extern "C" int omni_kv4_decode(const Kv4DecodeArgs* p, void* status, cudaStream_
                   : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, n, st, stream) : kv4_launch<2, 1>(a, c, B, n, st, stream)
                              : kv4_launch<4, 1>(a, c, B, n, st, stream);
   if (e != cudaSuccess || p->weights == nullptr) return (int)e;
-  e = d == 64 ? kv4_launch_weights<1>(a, c, B, p->max_len, st, stream) : d == 128 ? kv4_launch_weights<2>(a, c, B, p->max_len, st, stream)
-                                                                                  : kv4_launch_weights<4>(a, c, B, p->max_len, st, stream);
+  // Many rows make a tile long: shorter ones are shared out more evenly (16 rows of 8 heads over 30,011 tokens twice: 64 tokens a tile xx us,
+  // 16 yy us).
+  const bool fine = p->rows * rep > 32;
+  e = d == 64    ? fine ? kv4_launch_weights<1, 16>(a, c, B, p->max_len, st, stream) : kv4_launch_weights<1, 64>(a, c, B, p->max_len, st, stream)
+      : d == 128 ? fine ? kv4_launch_weights<2, 16>(a, c, B, p->max_len, st, stream) : kv4_launch_weights<2, 64>(a, c, B, p->max_len, st, stream)
+                 : fine ? kv4_launch_weights<4, 16>(a, c, B, p->max_len, st, stream) : kv4_launch_weights<4, 32>(a, c, B, p->max_len, st, stream);
   return (int)e;
 }
