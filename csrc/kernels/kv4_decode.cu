@@ -130,6 +130,13 @@ __device__ __forceinline__ void kv4_mma(float (&c)[4], const uint32_t (&a)[4], c
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
+// The same into d, from c
+__device__ __forceinline__ void kv4_mma_from(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], const float (&c)[4]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -232,10 +239,12 @@ struct Kv4Feed {
 // Fragments of 8 query rows (row r: query token r / rep, head h rep + r % rep) as fp16 numbers, each row times a power of two that
 // brings its largest number to 2^13 .. 2^14: bf16 numbers keep all their bits down to 2^-28 of the largest.  qs are the sums of the
 // groups, unit what brings scores to units of log 2 (its sign is that of the query), for the rows 2 c and 2 c + 1.
+// Key codes of odd columns are left as 16 (64 + code): their queries are a 16th.  The products start from `base`, which takes off what
+// the codes have too much: 64 for the odd columns, and too little: 8 for the even ones.
 template <int NG>
 struct Kv4Query {
   uint32_t b[NG][4][2];
-  float qs[NG][2], unit[2];
+  float qs[NG][2], base[NG][4], unit[2];
   // pairs of neighbouring columns as they are
   static __device__ __forceinline__ void fetch(const Kv4Decode& a, int rep, int b0, int h, int r, int total, uint32_t (&w)[NG][8]) {
     const int c = threadIdx.x & 3;
@@ -279,25 +288,33 @@ struct Kv4Query {
     unit[1] = __shfl_sync(0xffffffffu, un, c * 8 + 4);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      float x = 0.f;
+      float even = 0.f, odd = 0.f;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {                                        // columns i, i + 4 and i + 1, i + 5 of a word, i = 2 (s & 1)
         const uint32_t u = w[g][(s >> 1) * 4 + (s & 1)], v = w[g][(s >> 1) * 4 + (s & 1) + 2];
         const float u0 = __uint_as_float(u << 16) * up, u1 = __uint_as_float(u & 0xffff0000u) * up;
         const float v0 = __uint_as_float(v << 16) * up, v1 = __uint_as_float(v & 0xffff0000u) * up;
         b[g][s][0] = kv4_pack(u0, v0);
-        b[g][s][1] = kv4_pack(u1, v1);
-        x += (u0 + v0) + (u1 + v1);
+        b[g][s][1] = kv4_pack(u1 * 0.0625f, v1 * 0.0625f);
+        even += u0 + v0;
+        odd += u1 + v1;
       }
-      x += __shfl_xor_sync(0xffffffffu, x, 1);
-      x += __shfl_xor_sync(0xffffffffu, x, 2);
-      qs[g][0] = __shfl_sync(0xffffffffu, x, c * 8);
-      qs[g][1] = __shfl_sync(0xffffffffu, x, c * 8 + 4);
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        even += __shfl_xor_sync(0xffffffffu, even, d);
+        odd += __shfl_xor_sync(0xffffffffu, odd, d);
+      }
+      const float sum = even + odd, from = fmaf(odd, -64.f, even * 8.f);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        qs[g][x] = __shfl_sync(0xffffffffu, sum, c * 8 + 4 * x);
+        base[g][x] = base[g][2 + x] = __shfl_sync(0xffffffffu, from, c * 8 + 4 * x);
+      }
     }
   }
 };
 
-// Key codes minus 8 of 16 tokens of a staged tile
+// Key codes of 16 tokens of a staged tile, minus 8 those of even columns and 16 (64 + code) those of odd ones
 template <int NG, bool VALUES, int TOK = NG == 4 ? 32 : 64>
 struct Kv4Keys {
   using T = Kv4Tile<NG, VALUES, TOK>;
@@ -315,9 +332,9 @@ struct Kv4Keys {
   __device__ __forceinline__ void fragment(int g, int s, uint32_t (&a)[4]) const {       // s: 16 columns of the group
     const uint32_t w0 = w[g / T::PER][0][g % T::PER * 2 + (s >> 1)], w1 = w[g / T::PER][1][g % T::PER * 2 + (s >> 1)];
     if (s & 1) {
-      a[0] = kv4_code<2>(w0); a[1] = kv4_code<2>(w1); a[2] = kv4_code<3>(w0); a[3] = kv4_code<3>(w1);
+      a[0] = kv4_code<2>(w0); a[1] = kv4_code<2>(w1); a[2] = kv4_bits<0x00f000f0u>(w0 >> 8); a[3] = kv4_bits<0x00f000f0u>(w1 >> 8);
     } else {
-      a[0] = kv4_code<0>(w0); a[1] = kv4_code<0>(w1); a[2] = kv4_code<1>(w0); a[3] = kv4_code<1>(w1);
+      a[0] = kv4_code<0>(w0); a[1] = kv4_code<0>(w1); a[2] = kv4_bits<0x00f000f0u>(w0); a[3] = kv4_bits<0x00f000f0u>(w1);
     }
   }
 };
@@ -326,9 +343,9 @@ struct Kv4Keys {
 __device__ __forceinline__ void kv4_score(float (&s)[4], const float (&acc)[4], const uint32_t (&word)[2], const float (&qs)[2]) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const float step = kv4_step(word[e]), mid = fmaf(step, 8.f, kv4_low(word[e]));
+    const float step = kv4_step(word[e]), low = kv4_low(word[e]);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) s[2 * e + x] = fmaf(step, acc[2 * e + x], fmaf(mid, qs[x], s[2 * e + x]));
+    for (int x = 0; x < 2; ++x) s[2 * e + x] = fmaf(step, acc[2 * e + x], fmaf(low, qs[x], s[2 * e + x]));
   }
 }
 
@@ -376,13 +393,14 @@ struct Kv4Sums {
       for (int g = 0; g < NG; ++g) {
         float acc[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-#pragma unroll
         for (int x = 0; x < 4; ++x) {
           uint32_t f[4];
           k.fragment(g, x, f);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) kv4_mma(acc[n], f, q[n].b[g][x]);
+          for (int n = 0; n < NT; ++n) {
+            if (x == 0) kv4_mma_from(acc[n], f, q[n].b[g][x], q[n].base[g]);
+            else kv4_mma(acc[n], f, q[n].b[g][x]);
+          }
         }
         const uint32_t word[2] = {k.sc[0][g], k.sc[1][g]};
 #pragma unroll
@@ -750,7 +768,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   __shared__ __align__(8) uint64_t bars[KV4_WARPS * KV4_STAGES];
   __shared__ int abort_flag;
   __shared__ float s_w[KV4_WARPS][TOK];
-  constexpr int ROW = 1 + (NG + 1) / 2, EACH = (TOK + 31) / 32;
+  constexpr int ROW = 1 + NG, EACH = (TOK + 31) / 32;
   const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + 7) / 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
   uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
@@ -804,12 +822,10 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
 #pragma unroll
         for (int x = 0; x < 2; ++x)
           s_q[(ch * NG * 2 + g2 * 2 + x) * 32 + lane] = make_uint4(q.b[g2][2 * x][0], q.b[g2][2 * x][1], q.b[g2][2 * x + 1][0], q.b[g2][2 * x + 1][1]);
-      if (r == 0) {                 // of the rows 2 c and 2 c + 1: their sums (below) and units, and then pairs of qs
+      if (r == 0) {                 // of the rows 2 c and 2 c + 1: their sums (below) and units, and for each group qs and base
         s_row[(ch * ROW) * 4 + cc] = make_float4(INFINITY, INFINITY, q.unit[0], q.unit[1]);
 #pragma unroll
-        for (int g2 = 0; g2 < NG; g2 += 2)
-          s_row[(ch * ROW + 1 + g2 / 2) * 4 + cc] =
-              make_float4(q.qs[g2][0], q.qs[g2][1], g2 + 1 < NG ? q.qs[(g2 + 1) % NG][0] : 0.f, g2 + 1 < NG ? q.qs[(g2 + 1) % NG][1] : 0.f);
+        for (int g2 = 0; g2 < NG; ++g2) s_row[(ch * ROW + 1 + g2) * 4 + cc] = make_float4(q.qs[g2][0], q.qs[g2][1], q.base[g2][0], q.base[g2][1]);
       }
     }
     __syncthreads();
@@ -849,7 +865,8 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
           float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int g2 = 0; g2 < NG; ++g2) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            const float4 sums = s_row[(ch * ROW + 1 + g2) * 4 + cc];
+            float acc[4] = {sums.z, sums.w, sums.z, sums.w};
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const uint4 v = s_q[(ch * NG * 2 + g2 * 2 + x) * 32 + lane];
@@ -857,8 +874,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
               kv4_mma(acc, f[g2][2 * x], b0);
               kv4_mma(acc, f[g2][2 * x + 1], b1);
             }
-            const float4 sums = s_row[(ch * ROW + 1 + g2 / 2) * 4 + cc];
-            const float qs[2] = {g2 & 1 ? sums.z : sums.x, g2 & 1 ? sums.w : sums.y};
+            const float qs[2] = {sums.x, sums.y};
             const uint32_t word[2] = {k.sc[0][g2], k.sc[1][g2]};
             kv4_score(s, acc, word, qs);
           }
@@ -955,7 +971,7 @@ static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int 
 template <int NG, int TOK>
 static cudaError_t kv4_launch_weights(const Kv4Decode& a, const Kv4Cache& c, int B, int max_len, OmniStatus* st, cudaStream_t stream) {
   const int total = a.rows * (a.hq / c.hkv), chunks = (total + 7) / 8;
-  const int bytes = KV4_WARPS * KV4_STAGES * Kv4Tile<NG, false, TOK>::BYTES + chunks * (NG * 64 * 16 + (1 + (NG + 1) / 2) * 4 * 16);
+  const int bytes = KV4_WARPS * KV4_STAGES * Kv4Tile<NG, false, TOK>::BYTES + chunks * (NG * 64 * 16 + (1 + NG) * 4 * 16);
   static int most[64] = {0};
   cudaError_t e = kv4_smem((const void*)kv4_weights_kernel<NG, TOK>, bytes, most);
   if (e != cudaSuccess) return e;
