@@ -59,39 +59,35 @@ __device__ __forceinline__ int kv4_length(const Kv4Decode& a, int block, int b, 
   if (threadIdx.x == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_DECODE, b);
   return a.table_w * block;
 }
-// Work is cut into equal shares.  An item is a tile of query rows of a key/value head of a request; the items of a request one after the
-// other, requests one after the other, their tiles are numbered through, and block i of the grid takes the tiles from i * share on.  A
-// warp finds the tiles ahead of request `b`, and their total, in one pass over the lengths.
+// Work is cut into equal shares.  An item is a tile of query rows of a key/value head of a request (in the weights kernel all rows).  With
+// few items each is cut into parts of its own, so that no block has to change items: of `share` tiles at most, where share is the least that
+// surely leaves no more parts than blocks (parts are at most total / share and one for each item).  Otherwise the tiles of all items are
+// numbered through, items of a request one after the other, and block i takes those from i * share on: what it has of the item that
+// it starts with and of the one that it ends with are parts of these.  A warp finds its block's tiles by a scan of the lengths.
+struct Kv4Work {
+  int b, item, tile0, n_tiles, parts;       // parts: of the item, where the block has it alone to itself; else 0
+  long long left, share;
+};
 __device__ __forceinline__ int kv4_tiles(const Kv4Decode& a, int block, int tokens, int b) {
   return (min(max(a.seq_lens[b], 0), a.table_w * block) + tokens - 1) / tokens;
 }
-__device__ __forceinline__ long long kv4_warp_sum(long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+__device__ __forceinline__ long long kv4_ceil(long long x, long long by) {       // a 64-bit division takes as long as a load
+  return ((x | by) >> 31) == 0 ? (long long)(((unsigned)x + (unsigned)by - 1) / (unsigned)by) : (x + by - 1) / by;
 }
-__device__ __forceinline__ long long kv4_ahead(const Kv4Decode& a, int block, int tokens, int items, int from, int to) {
-  long long n = 0;
-  for (int b = from + (threadIdx.x & 31); b < to; b += 32) n += kv4_tiles(a, block, tokens, b);
-  return kv4_warp_sum(n) * items;
-}
-__device__ __forceinline__ long long kv4_share(const Kv4Decode& a, long long total, int blocks) {
-  const long long even = (total + blocks - 1) / blocks;
-  return even > a.min_tiles ? even : a.min_tiles;
-}
-// Request of tile g, and the tiles ahead of it; -1 behind the last
-__device__ __forceinline__ int kv4_find(const Kv4Decode& a, int block, int tokens, int items, int B, long long g, long long& ahead) {
+// Request that has unit i when request b has of(b) of them, and the units ahead of it; -1 behind the last
+template <typename F>
+__device__ __forceinline__ int kv4_find(int B, long long i, F of, long long& ahead) {
   const int lane = threadIdx.x & 31;
   ahead = 0;
   for (int b0 = 0; b0 < B; b0 += 32) {
-    const long long mine = b0 + lane < B ? (long long)kv4_tiles(a, block, tokens, b0 + lane) * items : 0;
+    const long long mine = b0 + lane < B ? of(b0 + lane) : 0;
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, ahead + upto > g);
+    const unsigned past = __ballot_sync(0xffffffffu, ahead + upto > i);
     if (past != 0) {
       const int l = __ffs(past) - 1;
       ahead += __shfl_sync(0xffffffffu, upto - mine, l);
@@ -100,6 +96,46 @@ __device__ __forceinline__ int kv4_find(const Kv4Decode& a, int block, int token
     ahead += __shfl_sync(0xffffffffu, upto, 31);
   }
   return -1;
+}
+__device__ __forceinline__ bool kv4_work(const Kv4Decode& a, int block, int tokens, int items, int B, int least, Kv4Work& w) {
+  long long all = 0;
+  int busy = 0;
+  for (int b = threadIdx.x & 31; b < B; b += 32) {
+    const int n = kv4_tiles(a, block, tokens, b);
+    all += n;
+    busy += n > 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    busy += __shfl_xor_sync(0xffffffffu, busy, o);
+  }
+  all *= items;
+  const long long some = (long long)busy * items, blocks = gridDim.x;
+  long long ahead;
+  if (some * 8 <= blocks) {                 // an eighth of the blocks at most for want of divisibility
+    w.share = max((long long)least, kv4_ceil(all, blocks - some));
+    w.b = kv4_find(B, blockIdx.x, [&](int b) { return items * kv4_ceil(kv4_tiles(a, block, tokens, b), w.share); }, ahead);
+    if (w.b < 0) return false;
+    w.n_tiles = kv4_tiles(a, block, tokens, w.b);
+    w.parts = (int)kv4_ceil(w.n_tiles, w.share);
+    const int i = blockIdx.x - (int)ahead;
+    w.item = i / w.parts;
+    const int part = i - w.item * w.parts, each = w.n_tiles / w.parts, more = w.n_tiles - each * w.parts;
+    w.tile0 = part * each + min(part, more);
+    w.left = each + (part < more ? 1 : 0);
+    return true;
+  }
+  w.parts = 0;
+  w.share = max((long long)least, kv4_ceil(all, blocks));
+  const long long g = blockIdx.x * w.share;
+  if (g >= all) return false;
+  w.b = kv4_find(B, g, [&](int b) { return (long long)items * kv4_tiles(a, block, tokens, b); }, ahead);
+  w.n_tiles = kv4_tiles(a, block, tokens, w.b);
+  w.item = (int)((g - ahead) / w.n_tiles);
+  w.tile0 = (int)(g - ahead - (long long)w.item * w.n_tiles);
+  w.left = min(w.share, all - g);
+  return true;
 }
 
 // The codes minus 8 of the nibbles I of both halves of a word, as an fp16 pair, exactly.  Behind the exponent of 1024 a code in bits
@@ -546,41 +582,29 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;");
 
-  // this block's tiles, from item `item` of request `b` on
-  int b, item, tile0, n_tiles;
-  long long left;
+  Kv4Work w;
   if (a.min_tiles == 0) {
-    b = blockIdx.x / items;
-    item = blockIdx.x - b * items;
-    tile0 = 0;
-    n_tiles = kv4_tiles(a, c.block, T::TOKENS, b);
-    left = n_tiles;
-  } else {
-    const long long all = kv4_ahead(a, c.block, T::TOKENS, items, 0, B), share = kv4_share(a, all, gridDim.x), g = blockIdx.x * share;
-    long long ahead;
-    if (g >= all) return;
-    b = kv4_find(a, c.block, T::TOKENS, items, B, g, ahead);
-    n_tiles = kv4_tiles(a, c.block, T::TOKENS, b);
-    item = (int)((g - ahead) / n_tiles);
-    tile0 = (int)(g - ahead - (long long)item * n_tiles);
-    left = min(share, all - g);
+    w.b = blockIdx.x / items;
+    w.item = blockIdx.x - w.b * items;
+    w.tile0 = w.parts = 0;
+    w.left = w.n_tiles = kv4_tiles(a, c.block, T::TOKENS, w.b);
+  } else if (!kv4_work(a, c.block, T::TOKENS, items, B, a.min_tiles, w)) {
+    return;
   }
-  const long long share = left;                                           // of all blocks but the last
-  int uses = 0;                                                            // of this warp's stages so far
+  int uses = 0, turn = 0;                                                  // of this warp's stages so far; the warp that the next tile falls to
   for (bool first = true;; first = false) {
-    const int h = item / chunks, row0 = (item - h * chunks) * NQ;
+    const int b = w.b, h = w.item / chunks, row0 = (w.item - h * chunks) * NQ, tile0 = w.tile0, n_tiles = w.n_tiles;
     const int len = kv4_length(a, c.block, b, st);
     const int first_sees = len - a.rows + 1 + row0 / rep;                  // of the item's first and last rows
     const int end = len - a.rows + 1 + (min(total, row0 + NQ) - 1) / rep;
-    const int end_tile = (int)min((long long)n_tiles, tile0 + left);
-    if (a.min_tiles != 0 && tile0 == 0 && threadIdx.x == 0) {              // `share` is whole here unless this block's is the last
-      const long long rest = n_tiles - end_tile;
-      const int more = rest <= 0 ? 0 : rest <= 0x7fffffffll && share <= 0x7fffffffll ? (int)(((unsigned)rest + (unsigned)share - 1) / (unsigned)share) : (int)((rest + share - 1) / share);
-      a.shared[(long long)b * items + item] = make_int2(2 * blockIdx.x + (first ? 0 : 1), 1 + more);
+    const int end_tile = (int)min((long long)n_tiles, tile0 + w.left);
+    if (a.min_tiles != 0 && tile0 == 0 && threadIdx.x == 0) {              // the blocks behind this one take a share each of what is left
+      const int parts = w.parts > 0 ? w.parts : end_tile == n_tiles ? 1 : 1 + (int)kv4_ceil(n_tiles - end_tile, w.share);
+      a.shared[(long long)b * items + w.item] = make_int2(2 * blockIdx.x + (first ? 0 : 1), parts);
     }
     const int stop = min(end, end_tile * T::TOKENS);                       // first token behind this part
     const int stop_tile = stop > 0 ? (stop + T::TOKENS - 1) / T::TOKENS : 0;
-    int tile = tile0 + warp, next = tile;
+    int tile = tile0 + ((warp - turn) & (KV4_WARPS - 1)), next = tile;
     Kv4Feed<NG, true> feed;
     feed.init(a, c, b, h, tile, KV4_WARPS, stop);
     uint32_t raw[NT][NG][8];                                               // asked for ahead of the copies, which would hold them up
@@ -706,13 +730,14 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
       }
     }
     // ---- the next item
-    left -= end_tile - tile0;
-    if (left <= 0) return;
-    tile0 = 0;
-    if (++item == items) {
-      item = 0;
-      do n_tiles = kv4_tiles(a, c.block, T::TOKENS, ++b);                  // tiles are left, so there is a request that has some
-      while (n_tiles == 0);
+    w.left -= end_tile - tile0;
+    if (w.left <= 0) return;
+    turn += max(0, stop_tile - tile0);
+    w.tile0 = 0;
+    if (++w.item == items) {
+      w.item = 0;
+      do w.n_tiles = kv4_tiles(a, c.block, T::TOKENS, ++w.b);              // tiles are left, so there is a request that has some
+      while (w.n_tiles == 0);
     }
     fence_proxy_async_smem();                                              // the sums in shared memory come before the next copies
     __syncthreads();
@@ -737,22 +762,29 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c) 
   // the first part is where its block says, those of the blocks behind it are their first ones
   const int first = shared.x, next = (first | 1) + 1, in = row % NQ;
   auto slot = [&](int s) -> long long { return (long long)(s == 0 ? first : next + 2 * (s - 1)) * NQ + in; };
+  constexpr int AHEAD = 16;                                                // partial results that are asked for together with the sums
+  float v[AHEAD];
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s) v[s] = s < parts ? a.o_part[slot(s) * c.d + d] : 0.f;
   // every warp finds the maximum and the sum of the parts by itself
   float mm = -INFINITY, sum = 0.f;
   for (int s = lane; s < parts; s += 32) mm = fmaxf(mm, a.lse_part[slot(s)]);
   mm = warp_max(mm);
   for (int s = lane; s < parts; s += 32) {
-    const float v = a.lse_part[slot(s)], f = v == -INFINITY ? 0.f : exp2f(v - mm);
+    const float x = a.lse_part[slot(s)], f = x == -INFINITY ? 0.f : exp2f(x - mm);
     sum += f;
     if (d < 32) s_f[s] = f;
   }
   sum = warp_sum(sum);
   __syncthreads();
   float acc = 0.f;
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s)
+    if (s < parts && s_f[s] != 0.f) acc = fmaf(s_f[s], v[s], acc);
 #pragma unroll 8
-  for (int s = 0; s < parts; ++s) {
-    const float f = s_f[s], v = a.o_part[slot(s) * c.d + d];
-    acc += f == 0.f ? 0.f : f * v;
+  for (int s = AHEAD; s < parts; ++s) {
+    const float f = s_f[s], x = a.o_part[slot(s) * c.d + d];
+    acc += f == 0.f ? 0.f : f * x;
   }
   a.out[(((long long)b * a.rows + tok) * a.hq + head) * c.d + d] = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
   if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = sum == 0.f ? -INFINITY : mm + __log2f(sum);
@@ -782,19 +814,16 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
     fence_proxy_async_smem();
   }
   __syncthreads();
-  // shares as in the decode kernel, an item being a key/value head of a request
-  const long long all = kv4_ahead(a, c.block, TOK, c.hkv, 0, B);
-  const long long even = (all + gridDim.x - 1) / gridDim.x, share = even > KV4_WARPS ? even : KV4_WARPS, g = blockIdx.x * share;
-  if (g >= all) {
+  Kv4Work w;
+  if (!kv4_work(a, c.block, TOK, c.hkv, B, KV4_WARPS, w)) {
     asm volatile("griddepcontrol.wait;" ::: "memory");                    // as in the join
     return;
   }
-  long long ahead, left = min(share, all - g);
-  int b = kv4_find(a, c.block, TOK, c.hkv, B, g, ahead), n_tiles = kv4_tiles(a, c.block, TOK, b);
-  int h = (int)((g - ahead) / n_tiles), tile0 = (int)(g - ahead - (long long)h * n_tiles), uses = 0;
+  int uses = 0, turn = 0;
   for (bool first = true;; first = false) {
-    const int len = kv4_length(a, c.block, b, st), end_tile = (int)min((long long)n_tiles, tile0 + left), stop = min(len, end_tile * TOK);
-    int tile = tile0 + warp, next = tile;
+    const int b = w.b, h = w.item, tile0 = w.tile0;
+    const int len = kv4_length(a, c.block, b, st), end_tile = (int)min((long long)w.n_tiles, tile0 + w.left), stop = min(len, end_tile * TOK);
+    int tile = tile0 + ((warp - turn) & (KV4_WARPS - 1)), next = tile;
     Kv4Feed<NG, false, TOK> feed;
     feed.init(a, c, b, h, tile, KV4_WARPS, stop);
 #pragma unroll
@@ -858,7 +887,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
         for (int g2 = 0; g2 < NG; ++g2)
 #pragma unroll
           for (int x = 0; x < 4; ++x) k.fragment(g2, x, f[g2][x]);
-        float w[2] = {0.f, 0.f};
+        float sum[2] = {0.f, 0.f};
 #pragma unroll 1
         for (int ch = 0; ch < chunks; ++ch) {
           const float4 row = s_row[ch * ROW * 4 + cc];
@@ -887,14 +916,14 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
                 const int i = ch * 8 + cc * 2 + x;
                 if (i >= total || t0 + r + 8 * e >= len - a.rows + 1 + i / rep) p = 0.f;
               }
-              w[e] += p;
+              sum[e] += p;
             }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          w[e] += __shfl_xor_sync(0xffffffffu, w[e], 1);
-          w[e] += __shfl_xor_sync(0xffffffffu, w[e], 2);
-          if (cc == 0) s_w[warp][u * 16 + r + 8 * e] = w[e];
+          sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+          sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+          if (cc == 0) s_w[warp][u * 16 + r + 8 * e] = sum[e];
         }
       }
       __syncwarp();
@@ -915,13 +944,14 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
       }
       return;
     }
-    left -= end_tile - tile0;
-    if (left <= 0) return;
-    tile0 = 0;
-    if (++h == c.hkv) {
-      h = 0;
-      do n_tiles = kv4_tiles(a, c.block, TOK, ++b);
-      while (n_tiles == 0);
+    w.left -= end_tile - tile0;
+    if (w.left <= 0) return;
+    turn += end_tile - tile0;
+    w.tile0 = 0;
+    if (++w.item == c.hkv) {
+      w.item = 0;
+      do w.n_tiles = kv4_tiles(a, c.block, TOK, ++w.b);
+      while (w.n_tiles == 0);
     }
   }
 }
