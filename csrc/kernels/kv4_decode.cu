@@ -746,7 +746,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
 
 // Items that several blocks have worked on, and requests of no tokens: one block for a query row and head, a thread a column.
 template <int NT>
-__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c) {
+__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, int blocks) {
   constexpr int NQ = 8 * NT;
   extern __shared__ float s_f[];                                           // [blocks]
   asm volatile("griddepcontrol.launch_dependents;");
@@ -757,7 +757,8 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c) 
   // Every block waits, those without work too: a kernel that follows this one may then count on the one ahead of it being done.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 shared = none ? make_int2(0, 0) : a.shared[((long long)b * c.hkv + h) * chunks + row / NQ];
-  const int parts = shared.y;
+  // after a wait that ran out it may be anything
+  const int parts = shared.x >= 0 && shared.y >= 0 && shared.x / 2 + shared.y <= blocks ? shared.y : 0;
   if (parts == 1) return;                                                  // written by its only block
   // the first part is where its block says, those of the blocks behind it are their first ones
   const int first = shared.x, next = (first | 1) + 1, in = row % NQ;
@@ -995,7 +996,7 @@ static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int 
   kv4_decode_kernel<NG, NT><<<(unsigned)grid, KV4_WARPS * 32, bytes, stream>>>(a, c, B, st);
   e = cudaGetLastError();
   if (e != cudaSuccess || a.min_tiles == 0) return e;
-  return kv4_follow(kv4_join_kernel<NT>, dim3(c.hkv * total, B), c.d, blocks * 4, stream, a, c);
+  return kv4_follow(kv4_join_kernel<NT>, dim3(c.hkv * total, B), c.d, blocks * 4, stream, a, c, blocks);
 }
 
 template <int NG, int TOK>
