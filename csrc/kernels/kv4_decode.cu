@@ -113,7 +113,7 @@ __device__ __forceinline__ bool kv4_work(const Kv4Decode& a, int block, int toke
   all *= items;
   const long long some = (long long)busy * items, blocks = gridDim.x;
   long long ahead;
-  if (some * 8 <= blocks) {                 // an eighth of the blocks at most for want of divisibility
+  if (some * 2 <= blocks) {                 // up to 218 uneven items of 444 blocks: 14 us against 17, 48 against 51; above, waste
     w.share = max((long long)least, kv4_ceil(all, blocks - some));
     w.b = kv4_find(B, blockIdx.x, [&](int b) { return items * kv4_ceil(kv4_tiles(a, block, tokens, b), w.share); }, ahead);
     if (w.b < 0) return false;
