@@ -577,9 +577,9 @@ extern "C" int omni_kv4_keep(const Kv4KeepArgs* p, void* status, cudaStream_t st
   if (p->batch <= 0) return 0;
   const Kv4Keep a = {p->weights, p->positions, p->table, p->seq_lens, p->seen, p->blocks, p->table_ld, p->table_w, p->block, p->hkv,
                      p->budget, p->first, p->last, p->keep, p->lens, p->scratch};
-  // Blocks of a cluster: one for every 2048 places, at most 8; of its keys a block keeps up to 40,000.
+  // Blocks of a cluster: one for every 8192 places, at most 8; of its keys a block keeps up to 40,000.
   int size = 1;
-  while (size < KV4_MOST_BLOCKS && p->max_len > 2048 * size) size *= 2;
+  while (size < KV4_MOST_BLOCKS && p->max_len > 8192 * size) size *= 2;
   const int run = (p->max_len + size - 1) / size, cap = run < 1024 ? 1024 : run > 40000 ? 40000 : run;
   static bool asked[64] = {false};
   int dev = 0;
