@@ -258,7 +258,7 @@ struct Kv4Keep {
   const int *positions, *table, *seq_lens, *seen;
   long long blocks;
   int table_ld, table_w, block, hkv, budget, first, last;
-  int *keep, *lens, *sources;       // [B, Hkv, budget], [B], scratch as keep
+  int *keep, *lens, *sources;       // [B, Hkv, budget], [B], scratch as keep (null where no request has over 2 KV4_BINS places)
 };
 
 // A cluster of blocks for a request and head, each with a run of its places.  The keys are read from memory once and kept in shared
@@ -285,7 +285,6 @@ __global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a
     n = a.table_w * a.block;
   }
   int* keep = a.keep + ((long long)b * a.hkv + h) * a.budget;
-  int* sources = a.sources + ((long long)b * a.hkv + h) * a.budget;
   if (blockIdx.x == 0 && tid == 0) a.lens[b] = min(n, a.budget);
   if (n <= a.budget) {
     for (int j = rank * N + tid; j < a.budget; j += size * N) keep[j] = j < n ? j : -1;
@@ -435,6 +434,8 @@ __global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a
       hole += theirs[0];
       source += theirs[1];
     }
+  // The tokens that fill places, in order: at most half of all places, so that those of up to 4096 find room in the histograms
+  int* sources = size == 1 && n <= 2 * KV4_BINS ? hist[0] : a.sources + ((long long)b * a.hkv + h) * a.budget;
   equal = equal0;
   if (j0 < a.budget || far > 0)
     for (int i = i0; i < i1; ++i) {
@@ -574,6 +575,7 @@ extern "C" int omni_kv4_keep(const Kv4KeepArgs* p, void* status, cudaStream_t st
   if (p->blocks <= 0 || p->block < 1 || p->hkv < 1 || p->hkv > 65535 || p->batch > 65535 || p->budget < 1 || p->max_len < 0 || p->first < 0 || p->last < 0 ||
       p->first + p->last > p->budget)
     return -1;
+  if (p->scratch == nullptr && (long long)p->table_w * p->block > 2 * KV4_BINS) return -2;
   if (p->batch <= 0) return 0;
   const Kv4Keep a = {p->weights, p->positions, p->table, p->seq_lens, p->seen, p->blocks, p->table_ld, p->table_w, p->block, p->hkv,
                      p->budget, p->first, p->last, p->keep, p->lens, p->scratch};

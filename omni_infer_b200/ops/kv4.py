@@ -188,7 +188,8 @@ def _call(name, device, *args):
         call = _bound[name] = (getattr(lib, name), _ARGS[name].pack)
     fn, pack = call
     index = device.index
-    status, stream = (nat._status.get(index) if index in nat._status else nat.status_buffer(index)).data_ptr(), torch._C._cuda_getCurrentRawStream(index)
+    status = nat._status.get(index)
+    status, stream = (nat.status_buffer(index) if status is None else status).data_ptr(), torch._C._cuda_getCurrentRawStream(index)
     if index == torch._C._cuda_getDevice():
         rc = fn(pack(*args), status, stream)
     else:
@@ -358,11 +359,11 @@ def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first
     keep = torch.empty((B, hkv, budget), dtype=torch.int32, device=device)
     lens = torch.empty(B, dtype=torch.int32, device=device)
     if B:
-        scratch = torch.empty((B, hkv, budget), dtype=torch.int32, device=device)
         width = block_table.shape[1]
+        scratch = torch.empty((B, hkv, budget), dtype=torch.int32, device=device) if width * block > 4096 else None
         longest = width * block if max_seq_len is None else max(0, min(max_seq_len, width * block))
         _call("omni_kv4_keep", device, weights.data_ptr(), positions.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), seen.data_ptr(),
-              keep.data_ptr(), lens.data_ptr(), scratch.data_ptr(), blocks,
+              keep.data_ptr(), lens.data_ptr(), _p(scratch), blocks,
               block, hkv, block_table.stride(0), width, B, budget, keep_first, keep_last, longest, 0)
     return keep, lens
 
