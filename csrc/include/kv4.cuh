@@ -47,7 +47,7 @@ __device__ __forceinline__ float kv4_step(uint32_t w) { return __uint_as_float(w
 __device__ __forceinline__ float kv4_low(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 inline bool kv4_shape_ok(const Kv4Cache& c) {
-  return c.blocks > 0 && c.hkv > 0 && c.block >= 16 && c.block % 16 == 0 && (c.d == 64 || c.d == 128 || c.d == 256) &&
+  return c.blocks > 0 && c.hkv > 0 && c.block >= 16 && c.block <= 1 << 20 && c.block % 16 == 0 && (c.d == 64 || c.d == 128 || c.d == 256) &&
          ((uintptr_t)c.k | (uintptr_t)c.v) % 16 == 0;
 }
 

@@ -4,22 +4,27 @@
 //   out  [B rows, Hq, d] bf16 = sum_t p_t v_t,  p = softmax_t(scale q k_t),  k_t and v_t = code * step + lowest
 //   weights[t] = decay * weights[t] + sum over the rows and the query heads of a key/value head of p_t
 //
-// Codes go to the tensor cores as they are.  The bits of a code placed at the top of the mantissa of 1.0 make the bf16 number
-// 1 + code / 16, one shift and one and-or for two codes, exactly; then
-//   q k_t = sum over groups  16 step (sum q (1 + code / 16)) + (lowest - 16 step) (sum q)
-//   out   = sum over groups  sum_t (16 step p_t) (1 + code / 16)  +  sum_t p_t (lowest - 16 step)
-// so keys and values are never rounded, the steps multiply fp32 scores and fp32 weights, and the terms without codes are a few
-// fp32 multiply-adds a token.  The weights of the second product, 16 step p_t, are carried as two bf16 numbers (16 bits of mantissa):
-// with one the rounding of the weights would be as large as that of the result.
+// Codes go to the tensor cores as whole numbers, exactly, and steps multiply fp32 numbers:
+//   q k_t = sum over groups  step_t (sum q code) + lowest_t (sum q)
+//   out   = sum over groups  sum_t (step_t p_t) (code - 8)  +  sum_t p_t (lowest_t + 8 step_t)
+// so keys and values are never rounded.  Behind the exponent of 1024 a code is an fp16 number with an offset (kv4_code below).  Queries become fp16
+// numbers without loss (a power of two for each row); the weights of the second product, step p_t, are rounded to fp16 once, after a
+// power of two that follows the largest step: 11 bits against the 8 of the result.  Values go in around 0: their offset would cost the
+// fp32 sums over a long cache the bits that they need.
 //
-// A row of keys takes 72 bytes at d = 128 and a tile of 16 tokens serves 8 query rows per product, so the op is bound by memory as
-// long as unpacking keeps up: 7 integer operations for 8 key codes, 17 for 16 value codes.
+// A token takes 144 bytes of keys and values at d = 128 and a tile of 16 tokens serves 8 query rows per product.  Unpacking bounds the
+// kernel: integer and packed fp16 instructions issue every other cycle each and hardly overlap; some 145 + 48 of them a tile of 16 tokens
+// and 8 rows, 70 fp32 ones and 16 products make 550 cycles of an SM quarter against the 387 in which the tile's bytes arrive.  Two and
+// three blocks an SM run equally fast.  Of the memory's 6.46 TB/s a long cache gets 5.4 once the first tiles are there.
+// Products in e4m3, in which a code needs no offset, are slower: they are carried out as four times as many fp16 ones (130 us against 82).
 //
-// The query rows of a key/value head (rows x heads of its group, in tiles of 8) are the columns of the products (mma.sync
-// m16n8k16), tokens and then columns of the head their rows: S = K Q^T, O^T = V^T P^T.  P^T wants tokens along its rows, which is what
-// movmatrix makes of S.  Each warp walks tiles of 64 tokens (32 at d = 256) by itself: one lane group starts bulk copies of the tile's
-// codes and scales, two tiles ahead, an mbarrier a stage says when they are there.  No block-wide wait stands in the loop.  The warps'
-// results meet in shared memory at the end, those of the parts of a long request in a second kernel.
+// The query rows of a key/value head (rows x heads of its group, in tiles of 8) are the columns of the products (mma.sync m16n8k16), tokens and
+// then columns of the head their rows: S = K Q^T, O^T = V^T P^T.  So a group of 8 heads wastes nothing, and P^T, which wants tokens along its
+// rows, is what movmatrix makes of S.  tcgen05 products would want 64 or 128 rows and the unpacked codes in shared memory.
+//
+// Each warp walks tiles of 64 tokens (32 at d = 256) by itself: bulk copies of the tile's codes and scales two tiles ahead, an mbarrier
+// for each stage.  No block-wide wait stands in the loop.  The warps' results meet in shared memory at the end, those of the parts of a
+// long request in a second kernel, the weights come from a third, each started while the one ahead of it ends.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -317,7 +322,7 @@ struct Kv4Query {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     // exponent of the factor: 13 - that of the largest, within what a factor and its inverse can be
-    const int e = min(max(13 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100);
+    const int e = min(max(13 - ((int)(__float_as_uint(most) >> 23) - 127), -120), 120);
     const float up = copysignf(__uint_as_float((uint32_t)(127 + e) << 23), scale_log2);
     const float un = fmaxf(fabsf(scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23), 0x1p-120f);
     unit[0] = __shfl_sync(0xffffffffu, un, c * 8);
@@ -1050,8 +1055,8 @@ extern "C" int omni_kv4_decode(const Kv4DecodeArgs* p, void* status, cudaStream_
                   : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, n, st, stream) : kv4_launch<2, 1>(a, c, B, n, st, stream)
                              : kv4_launch<4, 1>(a, c, B, n, st, stream);
   if (e != cudaSuccess || p->weights == nullptr) return (int)e;
-  // Many rows make a tile long: shorter ones are shared out more evenly (16 rows of 8 heads over 30,011 tokens twice: 64 tokens a tile xx us,
-  // 16 yy us).
+  // Many rows make a tile long: shorter ones are shared out more evenly (16 rows of 8 heads over 30,011 tokens twice: 160 us in all, 167
+  // with 64 tokens a tile).
   const bool fine = p->rows * rep > 32;
   e = d == 64    ? fine ? kv4_launch_weights<1, 16>(a, c, B, p->max_len, st, stream) : kv4_launch_weights<1, 64>(a, c, B, p->max_len, st, stream)
       : d == 128 ? fine ? kv4_launch_weights<2, 16>(a, c, B, p->max_len, st, stream) : kv4_launch_weights<2, 64>(a, c, B, p->max_len, st, stream)

@@ -17,21 +17,22 @@ def stored(x):
     return (code * step + lo).flatten(-2), step.squeeze(-1), lo.squeeze(-1)
 
 
-def attention(q, k, v, scale, k_step, k_low):
-    """q [r, d], k, v [n, d] (64 bits) -> out, weights, and the bound of the error of each in fp32 arithmetic.
+def attention(q, k, v, scale, k_step, k_low, v_step, v_low):
+    """q [r, d], k, v [n, d] (64 bits) -> out, weights p, and what fp32 sums and 16-bit products may be off by: the relative error of the
+    weights, sum p |v|, and an absolute error of the result.
 
-    Scores.  A kernel may sum q (16 + code) step and q (lowest - 16 step) apart, so an fp32 sum of d products has an error of at
-    most (d + 16) 2^-24 sum_i |q_i| (32 step_i + |low_i| + 16 step_i) scale =: e.  A weight p = exp(s) / sum exp is then off by
-    a factor of at most exp(2 e), and by 2^-20 more for its own exponentials (2^-22 each) and sums.
-    Values.  Weights times steps may be carried in two bf16 parts (2^-16 of the value each), times codes plus 16 (up to 31) against
-    a value that is known up to half a step: at most 2^-16 * 31 * step sum p =: c on top, and the rounding of the result."""
+    Scores.  A kernel may multiply q by codes with an offset of up to 64 and take the offset off in the sum, and add q lowest: an fp32 sum
+    of d products has an error of at most (d + 16) 2^-24 sum_i |q_i| ((64 + 15 + 64) step_i + |lowest_i|) scale =: e.  A weight
+    p = exp(s) / sum exp is then off by a factor of at most exp(2 e), and by 2^-20 more for its exponentials (2^-22 each) and sums.
+    Values.  step p may be rounded to fp16 (half a step is 2^-11 of it) ahead of its product with code - 8, while sum p (lowest + 8 step) is
+    carried in fp32: an error of at most 2^-11 sum_t p_t |v_t - lowest_t - 8 step_t|."""
     s = q.double() @ k.T * scale
     p = torch.softmax(s, -1)
     d = q.shape[-1]
-    mag = (48 * k_step + k_low.abs()).repeat_interleave(64, -1)
+    mag = (143 * k_step + k_low.abs()).repeat_interleave(64, -1)
     e = ((d + 16) * 2.0 ** -24 * abs(scale) * (q.double().abs() @ mag.T)).amax(-1, keepdim=True)
     rel = torch.expm1(2 * e) + 2.0 ** -20
-    return p @ v, p, rel, p @ v.abs()
+    return p @ v, p, rel, p @ v.abs(), 2.0 ** -11 * (p @ (v - (v_low + 8 * v_step).repeat_interleave(64, -1)).abs())
 
 
 def keep(weights, positions, n, seen, budget, first, last):

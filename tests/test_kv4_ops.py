@@ -141,7 +141,7 @@ def _check_decode(f, q, rows, scale, out, weights=None, old=None, decay=0.0):
     tol_w = torch.zeros_like(want_w) if want_w is not None else None
     for b, n in enumerate(f.lens):
         k, k_step, k_low = O.stored(f.k[b])
-        v, v_step, _ = O.stored(f.v[b])
+        v, v_step, v_low = O.stored(f.v[b])
         t = torch.arange(n)
         blk = f.table[b].long()[t // f.block]
         for h in range(f.hkv):
@@ -151,8 +151,8 @@ def _check_decode(f, q, rows, scale, out, weights=None, old=None, decay=0.0):
                 if m <= 0:
                     assert (got == 0).all()
                     continue
-                o, p, rel, mass = O.attention(q[b * rows + r, h * rep:(h + 1) * rep], k[:m, h], v[:m, h], scale, k_step[:m, h], k_low[:m, h])
-                carried = 2.0 ** -16 * 31 * (p @ v_step[:m, h]).repeat_interleave(64, -1)
+                o, p, rel, mass, carried = O.attention(q[b * rows + r, h * rep:(h + 1) * rep], k[:m, h], v[:m, h], scale, k_step[:m, h], k_low[:m, h],
+                                                       v_step[:m, h], v_low[:m, h])
                 bound = 2.0 ** -8 * o.abs() + (1 + 2.0 ** -8) * (rel * mass + carried) + 1e-38
                 assert ((got - o).abs() <= bound).all(), f"request {b}, row {r}, head {h}: {((got - o).abs() - bound).max():.3g} over the bound"
                 sums[:m] += p.sum(0)
@@ -228,6 +228,19 @@ def test_attention_of_any_magnitude(dev, q_scale, k_scale, v_scale, scale):
     w = torch.zeros(f.k_cache.shape[:3], device=dev)
     out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, scale, weights=w, decay=0.0)
     _check_decode(f, q, 1, scale, out, w, torch.zeros(f.k_cache.shape[:3]))
+
+
+@BOTH
+@pytest.mark.parametrize("shift", [1, 3, 8])
+def test_queries_of_any_pitch(dev, shift):
+    """Rows and heads that do not start on 16 bytes, and the largest and smallest bf16 numbers."""
+    f = Filled(17, [150, 3], 2, 128, 32, dev, k_scale=1e-3)
+    q = torch.randn(4, 9, 128 + 16, generator=_gen(3)).bfloat16()[:, 1:7, shift:shift + 128]
+    q[1] *= 1e-38
+    q[2] *= 1e37
+    q = q.to(dev) if dev == "cpu" else torch.randn(4, 9, 128 + 16, device=dev).bfloat16()[:, 1:7, shift:shift + 128].copy_(q)
+    out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 1e-34)
+    _check_decode(f, q, 2, 1e-34, out)
 
 
 @BOTH
@@ -393,7 +406,7 @@ def test_a_request_with_a_budget(dev):
     table = torch.randperm(8, generator=g).view(2, 4).to(torch.int32).to(dev)
     w, pos = torch.zeros(8, hkv, block, device=dev), torch.zeros(8, hkv, block, dtype=torch.int32, device=dev)
     lens = [0, 0]
-    mine = [[[] for _ in range(hkv)] for _ in range(B)]      # per head: [key row, value row, its steps and lows, weight, position]
+    mine = [[[] for _ in range(hkv)] for _ in range(B)]      # per head: [key row, value row, key steps, key lows, value steps, weight, position, value lows]
     for step in range(75):
         live = [b for b in range(B) if b == 0 or step >= 20]  # the second request comes later
         k, v = _rows(g, B, hkv, d), _rows(g, B, hkv, d, levels=False)
@@ -403,9 +416,9 @@ def test_a_request_with_a_budget(dev):
         for b in live:
             slots[b] = int(table[b, lens[b] // block]) * block + lens[b] % block
             lens[b] += 1
-            (ks, kst, kl), (vs, vst, _) = O.stored(k[b]), O.stored(v[b])
+            (ks, kst, kl), (vs, vst, vl) = O.stored(k[b]), O.stored(v[b])
             for h in range(hkv):
-                mine[b][h].append([ks[h], vs[h], kst[h], kl[h], vst[h], 0.0, seen[b] - 1])
+                mine[b][h].append([ks[h], vs[h], kst[h], kl[h], vst[h], 0.0, seen[b] - 1, vl[h]])
         n = torch.tensor(lens, dtype=torch.int32, device=dev)
         at = torch.tensor(seen, device=dev) - 1
         ops.kv4_write(k.to(dev), v.to(dev), slots.to(dev), kc, vc, weights=w, positions=pos, token_positions=at)
@@ -413,9 +426,8 @@ def test_a_request_with_a_budget(dev):
         for b in live:
             for h in range(hkv):
                 rows = mine[b][h]
-                ks, vs, kst, kl, vst = (torch.stack([r[i] for r in rows]) for i in range(5))
-                o, p, rel, mass = O.attention(q[b, h * rep:(h + 1) * rep], ks, vs, d ** -0.5, kst, kl)
-                carried = 2.0 ** -16 * 31 * (p @ vst).repeat_interleave(64, -1)
+                ks, vs, kst, kl, vst, vl = (torch.stack([r[i] for r in rows]) for i in (0, 1, 2, 3, 4, 7))
+                o, p, rel, mass, carried = O.attention(q[b, h * rep:(h + 1) * rep], ks, vs, d ** -0.5, kst, kl, vst, vl)
                 assert ((out[b, h * rep:(h + 1) * rep] - o).abs() <= 2.0 ** -8 * o.abs() + 1.01 * (rel * mass + carried)).all(), f"step {step}"
                 blk, t = table[b].long().cpu()[torch.arange(lens[b]) // block], torch.arange(lens[b]) % block
                 now = w.cpu()[blk, h, t]
@@ -561,6 +573,14 @@ REFUSED = {
 def test_refusals(what):
     with pytest.raises(AssertionError):
         REFUSED[what](_args())
+
+
+@pytest.mark.gpu
+def test_caches_off_16_bytes_are_refused():
+    buf = torch.zeros(2 * 16 * 36 + 8, dtype=torch.uint8, device="cuda")[8:].view(1, 2, 16, 36)
+    kc, vc = ops.kv4_cache(1, 16, 2, 64, "cuda")
+    with pytest.raises(RuntimeError, match="omni_kv4_read"):
+        ops.kv4_read(kc, buf, torch.zeros(1, dtype=torch.int64, device="cuda"))
 
 
 @pytest.mark.gpu
