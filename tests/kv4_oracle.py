@@ -24,15 +24,21 @@ def attention(q, k, v, scale, k_step, k_low, v_step, v_low):
     Scores.  A kernel may multiply q by codes with an offset of up to 64 and take the offset off in the sum, and add q lowest: an fp32 sum
     of d products has an error of at most (d + 16) 2^-24 sum_i |q_i| ((64 + 15 + 64) step_i + |lowest_i|) scale =: e.  A weight
     p = exp(s) / sum exp is then off by a factor of at most exp(2 e), and by 2^-20 more for its exponentials (2^-22 each) and sums.
-    Values.  step p may be rounded to fp16 (half a step is 2^-11 of it) ahead of its product with code - 8, while sum p (lowest + 8 step) is
-    carried in fp32: an error of at most 2^-11 sum_t p_t |v_t - lowest_t - 8 step_t|."""
+    Values.  With mid = lowest + 8 step, step p may be rounded to fp16 (half a step is 2^-11 of it) ahead of its product with code - 8, while
+    sum p mid is carried in fp32: an error of at most 2^-11 sum_t p_t |v_t - mid_t|.  Both are fp32 sums of n terms, a few multiplications and
+    additions more: (n + 16) 2^-24 sum_t p_t (|v_t - mid_t| + |mid_t|), which is not small against v where it is far below mid.  The fp16
+    numbers are step p 128 / M, with M at most twice the largest step and the largest p at least 1 ahead of the division by sum p: below their
+    smallest they are off by 2^-25, which 8 M / 128 multiplies: 2^-28 max step for each of the n tokens at most."""
     s = q.double() @ k.T * scale
     p = torch.softmax(s, -1)
     d = q.shape[-1]
     mag = (143 * k_step + k_low.abs()).repeat_interleave(64, -1)
     e = ((d + 16) * 2.0 ** -24 * abs(scale) * (q.double().abs() @ mag.T)).amax(-1, keepdim=True)
     rel = torch.expm1(2 * e) + 2.0 ** -20
-    return p @ v, p, rel, p @ v.abs(), 2.0 ** -11 * (p @ (v - (v_low + 8 * v_step).repeat_interleave(64, -1)).abs())
+    mid = (v_low + 8 * v_step).repeat_interleave(64, -1)
+    far = (v - mid).abs()
+    return p @ v, p, rel, p @ v.abs(), 2.0 ** -11 * (p @ far) + (len(v) + 16) * 2.0 ** -24 * (p @ (far + mid.abs())) \
+        + len(v) * 2.0 ** -28 * v_step.amax(0).repeat_interleave(64, -1)
 
 
 def keep(weights, positions, n, seen, budget, first, last):

@@ -178,6 +178,12 @@ SHAPES = [
     ([40, 1000], 16, 16, 2, 128, 128),
     ([70, 31], 3, 5, 1, 256, 16),
     ([2100], 1, 12, 4, 64, 80),
+    # many rows a key/value head
+    ([65], 33, 1, 1, 128, 16),
+    ([700, 0, 64, 8], 9, 8, 1, 128, 64),
+    ([100, 3, 257], 20, 10, 1, 64, 32),
+    ([1030], 17, 24, 3, 128, 128),
+    ([5000], 16, 8, 1, 128, 128),
 ]
 
 
@@ -220,14 +226,15 @@ def test_attention_is_split_over_long_caches(bound, B, n, hkv, rep):
 
 
 @BOTH
+@pytest.mark.parametrize("rows", [1, 5])
 @pytest.mark.parametrize("q_scale,k_scale,v_scale,scale", [(40.0, 1.0, 1.0, 0.09), (1.0, 1.0, 1e-20, 0.09), (1.0, 1.0, 1e6, 0.09), (0.0, 1.0, 1.0, 0.09),
                                                          (1.0, 100.0, 1.0, 1e-3), (1.0, 1.0, 1.0, -0.3), (1.0, 1.0, 1.0, 0.0)])
-def test_attention_of_any_magnitude(dev, q_scale, k_scale, v_scale, scale):
+def test_attention_of_any_magnitude(dev, q_scale, k_scale, v_scale, scale, rows):
     f = Filled(5, [333, 64], 2, 128, 16, dev, k_scale=k_scale, v_scale=v_scale)
-    q = (q_scale * torch.randn(2, 16, 128, generator=_gen(7))).bfloat16().to(dev)
+    q = (q_scale * torch.randn(2 * rows, 16, 128, generator=_gen(7))).bfloat16().to(dev)
     w = torch.zeros(f.k_cache.shape[:3], device=dev)
     out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, scale, weights=w, decay=0.0)
-    _check_decode(f, q, 1, scale, out, w, torch.zeros(f.k_cache.shape[:3]))
+    _check_decode(f, q, rows, scale, out, w, torch.zeros(f.k_cache.shape[:3]))
 
 
 @BOTH
@@ -267,7 +274,8 @@ def test_queries_with_one_large_column(dev, outlier):
 
 
 @BOTH
-def test_rising_scores(dev):
+@pytest.mark.parametrize("rows", [1, 5])
+def test_rising_scores(dev, rows):
     """Scores that rise, fall and stand still along the cache by far more than what an exponential holds: the running maximum has to
     follow them."""
     d, n = 128, 640
@@ -277,26 +285,30 @@ def test_rising_scores(dev):
         lift = {"up": t, "down": n - t, "peak": 500.0 * (t == 321)}[shape]
         f.k[0][:, 0, 0] = (lift * 2).bfloat16()
         ops.kv4_write(f.k[0].to(dev), f.v[0].to(dev), f.slots[0].to(dev), f.k_cache, f.v_cache)
-        q = torch.randn(1, 8, d, generator=_gen(1))
+        q = torch.randn(rows, 8, d, generator=_gen(1))
         q[:, :, 0] = torch.tensor([4.0, 1.0, 0.25, 0.0, -1.0, -4.0, 30.0, 2.0])
         q = q.bfloat16().to(dev)
         w = torch.zeros(f.k_cache.shape[:3], device=dev)
         out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.5, weights=w, decay=0.0)
-        _check_decode(f, q, 1, 0.5, out, w, torch.zeros(f.k_cache.shape[:3]))
+        _check_decode(f, q, rows, 0.5, out, w, torch.zeros(f.k_cache.shape[:3]))
 
 
 @BOTH
-def test_nan_stays_where_it_is_seen(dev):
-    f = Filled(21, [100, 100], 2, 128, 16, dev)
+@pytest.mark.parametrize("rows", [1, 20])
+def test_nan_stays_where_it_is_seen(dev, rows):
+    n = 100
+    f = Filled(21, [n, n], 2, 128, 16, dev)
     f.v[0][50, 1, 3] = float("nan")                          # a value of request 0, head 1: the columns of its group
     f.k[1][20, 0, 0] = float("inf")                          # a key of request 1, head 0: all columns of the head's queries
+    f.v[1][n - 1, 1, 100] = float("-inf")                    # a value that only the last row sees
     for b in (0, 1):
         ops.kv4_write(f.k[b].to(dev), f.v[b].to(dev), f.slots[b].to(dev), f.k_cache, f.v_cache)
-    q = torch.randn(2, 4, 128, generator=_gen(1)).bfloat16().to(dev)
-    out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.1).cpu()
-    nan = torch.zeros(2, 4, 128, dtype=torch.bool)
-    nan[0, 2:, :64] = True
-    nan[1, :2] = True
+    q = torch.randn(2 * rows, 4, 128, generator=_gen(1)).bfloat16().to(dev)
+    out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.1).cpu().view(2, rows, 4, 128)
+    nan = torch.zeros(2, rows, 4, 128, dtype=torch.bool)
+    nan[0, :, 2:, :64] = True
+    nan[1, :, :2] = True
+    nan[1, -1, 2:, 64:] = True
     assert torch.equal(out.isnan(), nan)
 
 
