@@ -318,9 +318,9 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
         width, total = block_table.shape[1], T // B * (hq // hkv)
         assert weights is None or total <= 256, f"weights of at most 256 query rows a key/value head at once: {total}"
         longest = width * block if max_seq_len is None else max(0, min(max_seq_len, width * block))
-        tile = 8 if d > 128 or total <= 8 else 16 if total <= 32 else 128
+        tile = 16 if d <= 128 and total > 8 else 8
         items = B * hkv * -(-total // tile)
-        blocks_at_once, min_tiles = _blocks(items, -(-longest // (32 if d == 256 else 64)), 2 if tile * d > 1024 else 3)
+        blocks_at_once, min_tiles = _blocks(items, -(-longest // (32 if d == 256 else 64)), 3 if tile * d <= 1024 else 2)
         lse = torch.empty(T * hq, dtype=torch.float32, device=device) if weights is not None else None
         o_part = lse_part = shared = 0
         if min_tiles:                                        # partial results, their sums, where the parts of an item are
