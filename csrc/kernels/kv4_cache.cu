@@ -259,39 +259,35 @@ struct Kv4Keep {
   const int *positions, *table, *seq_lens, *seen;
   long long blocks;
   int table_ld, table_w, block, hkv, budget, first, last;
-  int *keep, *lens, *sources;       // [B, Hkv, budget], [B], scratch as keep (null where no request has over 2 KV4_BINS places)
+  int *keep, *lens, *scratch;       // [B, Hkv, budget], [B], scratch as keep (null where no request has over 2 KV4_BINS places)
 };
 
 // A cluster of blocks for a request and head, each with a run of its places.  The keys are read from memory once and kept in shared
 // memory (`cap` of them a block; those beyond are made again when they are needed).  The key of the budget-th heaviest place is
 // found 11, 11 and 10 bits at a time: histograms in shared memory, which every block of the cluster adds up for itself.  Then a
-// thread walks its own run of places, so that ranks (of equal keys, of the places to fill, of the tokens that fill them) are one
-// scan each.  Reads 8 bytes a place; bound by the latency of its some ten steps.
+// warp walks its own run of places, and ranks (of equal keys, of the places to fill, of the tokens that fill them) are counts of its
+// votes and sums over the warps and blocks ahead.  Reads 8 bytes a place; bound by the latency of its some ten steps.
 constexpr int KV4_BINS = 2048, KV4_MOST_BLOCKS = 8;
-__global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a, int cap, OmniStatus* st) {
+__host__ __device__ constexpr int kv4_keep_run(int n, int size) { return ((n + size - 1) / size + 3) & ~3; }      // places of a block
+struct Kv4KeepShared {
+  int hist[2][KV4_BINS];            // highest keys first
+  int run[3][KV4_KEEP_THREADS / 32];                                // of the warps' runs: equal keys, places to fill, tokens that fill some
+  int count[2];                     // of this block: places to fill, tokens that fill some
+  int equal;                        // keys equal to the last that stays in the blocks ahead
+  uint32_t prefix;
+  int left, all;
+};
+// ALL: the keys of a run find room in shared memory.  VEC: places that are read at once, 4 where blocks and addresses allow (a run is 15 keys a
+// thread of two blocks an SM: it is instructions that count, not bytes).
+template <bool ALL, int VEC>
+__device__ __forceinline__ void kv4_keep_body(const Kv4Keep& a, int n, int cap, uint32_t* s_keys, Kv4KeepShared& sh, OmniStatus* st) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   constexpr int N = KV4_KEEP_THREADS;
-  extern __shared__ uint32_t s_keys[];
-  __shared__ __align__(16) int hist[2][KV4_BINS];                   // highest keys first
-  __shared__ int s_count[2];        // of this block: places to fill, tokens that fill some
-  __shared__ int s_equal;           // keys equal to the last that stays in the blocks ahead
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left, s_all;
   const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.y, h = blockIdx.x / size, tid = threadIdx.x;
-  int n = max(a.seq_lens[b], 0);
-  if (n > a.table_w * a.block) {
-    if (tid == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
-    n = a.table_w * a.block;
-  }
   int* keep = a.keep + ((long long)b * a.hkv + h) * a.budget;
-  if (blockIdx.x == 0 && tid == 0) a.lens[b] = min(n, a.budget);
-  if (n <= a.budget) {
-    for (int j = rank * N + tid; j < a.budget; j += size * N) keep[j] = j < n ? j : -1;
-    return;
-  }
-  const int chunk = (n + size - 1) / size, j0 = rank * chunk, count = max(0, min(chunk, n - j0));
+  const int chunk = kv4_keep_run(n, size), j0 = rank * chunk, count = max(0, min(chunk, n - j0));
   const int last_from = a.seen[b] - a.last;
   const int* table = a.table + (long long)b * a.table_ld;
   auto make_at = [&](int page, int off) -> uint32_t {
@@ -304,20 +300,20 @@ __global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a
     return kv4_keep_key(a.weights[at], a.positions[at], a.first, last_from);
   };
   auto make = [&](int i) -> uint32_t { return make_at((j0 + i) / a.block, (j0 + i) % a.block); };
-  auto key = [&](int i) -> uint32_t { return i < cap ? s_keys[i] : make(i); };
-  for (int i = tid; i < KV4_BINS; i += N) hist[0][i] = hist[1][i] = 0;
+  auto key = [&](int i) -> uint32_t { return ALL || i < cap ? s_keys[i] : make(i); };
+  for (int i = tid; i < KV4_BINS; i += N) sh.hist[0][i] = sh.hist[1][i] = 0;
   __syncthreads();
   {
-    constexpr int AT_ONCE = 8;                                      // loads under way a thread: block ids, then weights and positions
-    const int pages = N / a.block, rest = N - pages * a.block;
-    int page = (j0 + tid) / a.block, off = (j0 + tid) - page * a.block;
-    for (int i = tid; i < count; i += N * AT_ONCE) {
-      int blk[AT_ONCE], at[AT_ONCE], pos[AT_ONCE];
-      float w[AT_ONCE];
+    constexpr int AT_ONCE = VEC == 4 ? 4 : 8, STEP = N * VEC;        // loads under way a thread: block ids, then weights and positions
+    const int pages = STEP / a.block, rest = STEP - pages * a.block, stride = a.hkv * a.block, base = h * a.block;
+    int page = (j0 + tid * VEC) / a.block, off = (j0 + tid * VEC) - page * a.block;
+    for (int i0 = tid * VEC; i0 < count; i0 += STEP * AT_ONCE) {
+      int blk[AT_ONCE], at[AT_ONCE], pos[AT_ONCE][VEC];
+      float w[AT_ONCE][VEC];
 #pragma unroll
       for (int x = 0; x < AT_ONCE; ++x) {
-        at[x] = off;
-        blk[x] = i + x * N < count ? table[page] : 0;
+        at[x] = base + off;
+        blk[x] = i0 + x * STEP < count ? table[page] : 0;
         page += pages;
         off += rest;
         if (off >= a.block) {
@@ -328,20 +324,31 @@ __global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a
 #pragma unroll
       for (int x = 0; x < AT_ONCE; ++x) {
         const bool in = blk[x] >= 0 && blk[x] < a.blocks;
-        const long long to = ((long long)(in ? blk[x] : 0) * a.hkv + h) * a.block + at[x];
-        w[x] = a.weights[to];
-        pos[x] = a.positions[to];
+        const long long from = (long long)(in ? blk[x] : 0) * stride + at[x];
+        if (VEC == 4) {
+          *reinterpret_cast<float4*>(w[x]) = *reinterpret_cast<const float4*>(a.weights + from);
+          *reinterpret_cast<int4*>(pos[x]) = *reinterpret_cast<const int4*>(a.positions + from);
+        } else {
+          w[x][0] = a.weights[from];
+          pos[x][0] = a.positions[from];
+        }
       }
 #pragma unroll
       for (int x = 0; x < AT_ONCE; ++x) {
-        if (i + x * N >= count) break;
-        uint32_t k = kv4_keep_key(w[x], pos[x], a.first, last_from);
-        if (blk[x] < 0 || blk[x] >= a.blocks) {
-          report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
-          k = 0u;
+        const int i = i0 + x * STEP;
+        if (i >= count) break;
+        const bool in = blk[x] >= 0 && blk[x] < a.blocks;
+        if (!in) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
+        uint32_t k[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          k[e] = in ? kv4_keep_key(w[x][e], pos[x][e], a.first, last_from) : 0u;
+          if (VEC == 1 || i + e < count) atomicAdd(&sh.hist[0][KV4_BINS - 1 - (k[e] >> 21)], 1);
         }
-        if (i + x * N < cap) s_keys[i + x * N] = k;
-        atomicAdd(&hist[0][KV4_BINS - 1 - (k >> 21)], 1);
+        if (ALL || i < cap) {                                       // cap is a multiple of 4
+          if (VEC == 4) *reinterpret_cast<uint4*>(s_keys + i) = *reinterpret_cast<uint4*>(k);
+          else s_keys[i] = k[0];
+        }
       }
     }
   }
@@ -351,7 +358,7 @@ __global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    int* mine = hist[pass & 1];
+    int* mine = sh.hist[pass & 1];
     if (pass > 0) {
       for (int i = tid; i < count; i += N) {
         const uint32_t k = key(i);
@@ -379,76 +386,135 @@ __global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a
 #pragma unroll
     for (int d = 0; d < MOST; ++d) {
       if (above < left && left <= above + v[d]) {
-        s_prefix = prefix | (uint32_t)(bins - 1 - tid * each - d) << shift;
-        s_left = left - above;
-        s_all = v[d];
+        sh.prefix = prefix | (uint32_t)(bins - 1 - tid * each - d) << shift;
+        sh.left = left - above;
+        sh.all = v[d];
       }
       above += v[d];
     }
     if (pass == 1)                                                  // nobody reads the first histogram any more: it serves once more
-      for (int i = tid; i < KV4_BINS; i += N) hist[0][i] = 0;
+      for (int i = tid; i < KV4_BINS; i += N) sh.hist[0][i] = 0;
     __syncthreads();
-    prefix = s_prefix;
-    left = s_left;
-    all_stay = left == s_all;
+    prefix = sh.prefix;
+    left = sh.left;
+    all_stay = left == sh.all;
     mask |= (uint32_t)(bins - 1) << shift;
     __syncthreads();
     if (all_stay) break;                                            // no need to tell the places of this prefix apart
   }
-  // `prefix` begins the keys of the last places that stay; `left` of the places with such keys do, the lowest first.  An odd run a thread:
-  // its reads of shared memory meet no others.
-  const int each = ((count + N - 1) / N) | 1, i0 = min(tid * each, count), i1 = min(i0 + each, count);
+  // `prefix` begins the keys of the last places that stay; `left` of the places with such keys do, the lowest first.  A warp walks a run of the
+  // block's places, 32 at a time, so that a place's rank is a count of votes.
+  const int warp = tid >> 5, lane = tid & 31;
+  const uint32_t below = (1u << lane) - 1u;
+  const int each = (count + N - 1) / N * 32, i0 = min(warp * each, count), i1 = min(i0 + each, count);
+  auto ahead = [&](int x) -> int { return __reduce_add_sync(0xffffffffu, lane < warp ? sh.run[x][lane] : 0); };
   int equal0 = 0;
   if (!all_stay) {                                                  // all bits are known: the keys are equal
     if (tid < 32) {                                                 // their number in the blocks ahead is in the last histograms
-      int x = 0;
-      if (tid < rank) x = cluster.map_shared_rank(hist[0], tid)[1023 - (prefix & 1023)];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      if (tid == 0) s_equal = x;
+      const int x = __reduce_add_sync(0xffffffffu, tid < rank ? cluster.map_shared_rank(sh.hist[0], tid)[1023 - (prefix & 1023)] : 0);
+      if (tid == 0) sh.equal = x;
     }
-    for (int i = i0; i < i1; ++i) equal0 += key(i) == prefix;
-    equal0 = kv4_block_scan(equal0);                                // s_equal is there after its barriers
-    equal0 += s_equal;
+    int mine = 0;
+#pragma unroll 4
+    for (int i = i0 + lane; i < i0 + each; i += 32) mine += __popc(__ballot_sync(0xffffffffu, i < i1 && key(i) == prefix));
+    if (lane == 0) sh.run[0][warp] = mine;
+    __syncthreads();
+    equal0 = sh.equal + ahead(0);
   }
-  // Whether place i stays, asked in order
-  auto stays = [&](int i, int& equal) -> bool {
-    const uint32_t k = key(i) & mask;
-    return k > prefix || (k == prefix && (all_stay || equal++ < left));
+  // Which of a warp's next 32 places stay.  Later walks find the votes where the run's first keys were: a word for 32 keys.
+  auto decide = [&](int i, int& equal) -> uint32_t {
+    const uint32_t k = i < i1 ? key(i) & mask : 0u;
+    const bool above = i < i1 && k > prefix, last = i < i1 && k == prefix;
+    if (all_stay) return __ballot_sync(0xffffffffu, above || last);
+    const uint32_t votes = __ballot_sync(0xffffffffu, last);
+    const bool s = above || (last && equal + __popc(votes & below) < left);
+    equal += __popc(votes);
+    return __ballot_sync(0xffffffffu, s);
+  };
+  auto again = [&](int i, int& equal) -> uint32_t { return ALL ? s_keys[i0 + (i - i0) / 32] : decide(i, equal); };
+  const int near = max(0, min(i1 - i0, a.budget - j0 - i0));        // the run's first places are to be filled, the others may fill some
+  auto near_of = [&](int i) -> uint32_t {                           // of the 32 with i
+    const int x = near - (i - i0 - lane);
+    return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u;
   };
   int holes = 0, far = 0, equal = equal0;
-  for (int i = i0; i < i1; ++i) {
-    const bool s = stays(i, equal), near = j0 + i < a.budget;
-    holes += near && !s;
-    far += !near && s;
+#pragma unroll 4
+  for (int i = i0 + lane; i < i0 + each; i += 32) {
+    const uint32_t stay = decide(i, equal), first = near_of(i);
+    holes += __popc(~stay & first);
+    far += __popc(stay & ~first);
+    if (ALL && lane == 0 && i < i1) s_keys[i0 + (i - i0) / 32] = stay;      // the vote was behind the reads of these keys
   }
-  int hole = kv4_block_scan(holes), source = kv4_block_scan(far);
-  if (tid == N - 1) {
-    s_count[0] = hole + holes;
-    s_count[1] = source + far;
+  if (lane == 0) {
+    sh.run[1][warp] = holes;
+    sh.run[2][warp] = far;
+  }
+  __syncthreads();
+  int hole = ahead(1), source = ahead(2);
+  if (tid == N - 32) {
+    sh.count[0] = hole + holes;
+    sh.count[1] = source + far;
   }
   cluster.sync();
+  if (rank > 0) {
+    const int* theirs = cluster.map_shared_rank(sh.count, lane < rank ? lane : 0);
+    hole += __reduce_add_sync(0xffffffffu, lane < rank ? theirs[0] : 0);
+    source += __reduce_add_sync(0xffffffffu, lane < rank ? theirs[1] : 0);
+  }
+  // The places to fill, in order: at most half of all places, so that those of up to 4096 find room in the histograms
+  int* list = size == 1 && n <= 2 * KV4_BINS ? sh.hist[0] : a.scratch + ((long long)b * a.hkv + h) * a.budget;
+  equal = equal0;
+#pragma unroll 4
+  for (int i = i0 + lane; i - lane < i0 + near; i += 32) {
+    const uint32_t stay = again(i, equal), open = ~stay & near_of(i);
+    if (i < i0 + near) {
+      if (stay >> lane & 1u) keep[j0 + i] = j0 + i;
+      else list[hole + __popc(open & below)] = j0 + i;
+    }
+    hole += __popc(open);
+  }
+  cluster.sync();                                                   // the list is there, and nobody reads another's memory any more
+  if (far == 0) return;
+  constexpr int AT_ONCE = 8;                                        // loads under way a thread
+  equal = equal0;
+  for (int i = i0 + lane; i < i0 + each; i += 32 * AT_ONCE) {
+    int to[AT_ONCE];
 #pragma unroll
-  for (int r = 0; r < KV4_MOST_BLOCKS; ++r)
-    if (r < rank) {
-      const int* theirs = cluster.map_shared_rank(s_count, r);
-      hole += theirs[0];
-      source += theirs[1];
+    for (int x = 0; x < AT_ONCE; ++x) {
+      const int at = i + x * 32;
+      to[x] = -1;
+      if (at - lane < i1) {
+        const uint32_t fill = again(at, equal) & ~near_of(at);
+        if (fill >> lane & 1u) to[x] = list[source + __popc(fill & below)];
+        source += __popc(fill);
+      }
     }
-  // The tokens that fill places, in order: at most half of all places, so that those of up to 4096 find room in the histograms
-  int* sources = size == 1 && n <= 2 * KV4_BINS ? hist[0] : a.sources + ((long long)b * a.hkv + h) * a.budget;
-  equal = equal0;
-  if (j0 < a.budget || far > 0)
-    for (int i = i0; i < i1; ++i) {
-      if (!stays(i, equal)) continue;
-      if (j0 + i < a.budget) keep[j0 + i] = j0 + i;
-      else sources[source++] = j0 + i;
-    }
-  cluster.sync();                                                   // all sources are there, and nobody reads another's memory any more
-  equal = equal0;
-  if (holes > 0)
-    for (int i = i0; i < i1 && j0 + i < a.budget; ++i)
-      if (!stays(i, equal)) keep[j0 + i] = sources[hole++];
+#pragma unroll
+    for (int x = 0; x < AT_ONCE; ++x)
+      if (to[x] >= 0) keep[to[x]] = j0 + i + x * 32;
+  }
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a, int cap, OmniStatus* st) {
+  extern __shared__ __align__(16) uint32_t s_keys[];
+  __shared__ __align__(16) Kv4KeepShared sh;
+  constexpr int N = KV4_KEEP_THREADS;
+  const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.y, h = blockIdx.x / size, tid = threadIdx.x;
+  int n = max(a.seq_lens[b], 0);
+  if (n > a.table_w * a.block) {
+    if (tid == 0) report_status(st, OMNI_ERR_BOUNDS, KV4_SITE_KEEP, b);
+    n = a.table_w * a.block;
+  }
+  int* keep = a.keep + ((long long)b * a.hkv + h) * a.budget;
+  if (blockIdx.x == 0 && tid == 0) a.lens[b] = min(n, a.budget);
+  if (n <= a.budget) {
+    for (int j = rank * N + tid; j < a.budget; j += size * N) keep[j] = j < n ? j : -1;
+    return;
+  }
+  if (kv4_keep_run(n, size) <= cap) kv4_keep_body<true, VEC>(a, n, cap, s_keys, sh, st);
+  else kv4_keep_body<false, VEC>(a, n, cap, s_keys, sh, st);
 }
 
 struct Kv4Move {
@@ -574,7 +640,7 @@ struct Kv4KeepArgs {
 };
 extern "C" int omni_kv4_keep(const Kv4KeepArgs* p, void* status, cudaStream_t stream) {
   if (p->blocks <= 0 || p->block < 1 || p->hkv < 1 || p->hkv > 65535 || p->batch > 65535 || p->budget < 1 || p->max_len < 0 || p->first < 0 || p->last < 0 ||
-      p->first + p->last > p->budget)
+      p->first + p->last > p->budget || (long long)p->hkv * p->block > 0x7fffffffll)
     return -1;
   if (p->scratch == nullptr && (long long)p->table_w * p->block > 2 * KV4_BINS) return -2;
   if (p->batch <= 0) return 0;
@@ -583,13 +649,15 @@ extern "C" int omni_kv4_keep(const Kv4KeepArgs* p, void* status, cudaStream_t st
   // Blocks of a cluster: one for every 8192 places, at most 8; of its keys a block keeps up to 40,000.
   int size = 1;
   while (size < KV4_MOST_BLOCKS && p->max_len > 8192 * size) size *= 2;
-  const int run = (p->max_len + size - 1) / size, cap = run < 1024 ? 1024 : run > 40000 ? 40000 : run;
-  static bool asked[64] = {false};
+  const int run = kv4_keep_run(p->max_len, size), cap = run < 1024 ? 1024 : run > 40000 ? 40000 : run;
+  const bool vec = p->block % 4 == 0 && ((uintptr_t)p->weights | (uintptr_t)p->positions) % 16 == 0;
+  const auto kernel = vec ? kv4_keep_kernel<4> : kv4_keep_kernel<1>;
+  static bool asked[2][64] = {{false}};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev >= 64 || !asked[dev])) {
-    e = cudaFuncSetAttribute(kv4_keep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 40000 * 4);
-    if (e == cudaSuccess && dev < 64) asked[dev] = true;
+  if (e == cudaSuccess && (dev >= 64 || !asked[vec][dev])) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 40000 * 4);
+    if (e == cudaSuccess && dev < 64) asked[vec][dev] = true;
   }
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t config = {};
@@ -602,7 +670,7 @@ extern "C" int omni_kv4_keep(const Kv4KeepArgs* p, void* status, cudaStream_t st
   attr.val.clusterDim = {(unsigned)size, 1, 1};
   config.attrs = &attr;
   config.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&config, kv4_keep_kernel, a, cap, (OmniStatus*)status);
+  return (int)cudaLaunchKernelEx(&config, kernel, a, cap, (OmniStatus*)status);
 }
 
 struct Kv4MoveArgs {
