@@ -229,10 +229,10 @@ __device__ __forceinline__ uint32_t kv4_keep_key(float w, int pos, int first, in
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-constexpr int KV4_KEEP_THREADS = 512;
 // Exclusive sum over a block of that many threads
+template <int THREADS>
 __device__ __forceinline__ int kv4_block_scan(int x) {
-  constexpr int WARPS = KV4_KEEP_THREADS / 32;
+  constexpr int WARPS = THREADS / 32;
   __shared__ int part[WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int v = x;
@@ -267,11 +267,11 @@ struct Kv4Keep {
 // found 11, 11 and 10 bits at a time: histograms in shared memory, which every block of the cluster adds up for itself.  Then a
 // warp walks its own run of places, and ranks (of equal keys, of the places to fill, of the tokens that fill them) are counts of its
 // votes and sums over the warps and blocks ahead.  Reads 8 bytes a place; bound by the latency of its some ten steps.
-constexpr int KV4_BINS = 2048, KV4_MOST_BLOCKS = 8;
+constexpr int KV4_BINS = 2048, KV4_MOST_BLOCKS = 8, KV4_MOST_KEYS = 40000;
 __host__ __device__ constexpr int kv4_keep_run(int n, int size) { return ((n + size - 1) / size + 3) & ~3; }      // places of a block
 struct Kv4KeepShared {
   int hist[2][KV4_BINS];            // highest keys first
-  int run[3][KV4_KEEP_THREADS / 32];                                // of the warps' runs: equal keys, places to fill, tokens that fill some
+  int run[3][32];                                                 // of the warps' runs: equal keys, places to fill, tokens that fill some
   int count[2];                     // of this block: places to fill, tokens that fill some
   int equal;                        // keys equal to the last that stays in the blocks ahead
   uint32_t prefix;
@@ -279,11 +279,10 @@ struct Kv4KeepShared {
 };
 // ALL: the keys of a run find room in shared memory.  VEC: places that are read at once, 4 where blocks and addresses allow (a run is 15 keys a
 // thread of two blocks an SM: it is instructions that count, not bytes).
-template <bool ALL, int VEC>
+template <bool ALL, int VEC, int N>
 __device__ __forceinline__ void kv4_keep_body(const Kv4Keep& a, int n, int cap, uint32_t* s_keys, Kv4KeepShared& sh, OmniStatus* st) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  constexpr int N = KV4_KEEP_THREADS;
   const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.y, h = blockIdx.x / size, tid = threadIdx.x;
   int* keep = a.keep + ((long long)b * a.hkv + h) * a.budget;
@@ -367,22 +366,27 @@ __device__ __forceinline__ void kv4_keep_body(const Kv4Keep& a, int n, int cap, 
     }
     cluster.sync();
     constexpr int MOST = KV4_BINS / N;                              // bins of a thread, or half as many
-    static_assert(MOST == 4, "four bins are one read");
     const int each = bins / N;
-    int v[MOST] = {0, 0, 0, 0};
+    int v[MOST], all = 0;
+#pragma unroll
+    for (int d = 0; d < MOST; ++d) v[d] = 0;
 #pragma unroll
     for (int r = 0; r < KV4_MOST_BLOCKS; ++r) {
       if (r >= size) continue;
       const int* theirs = cluster.map_shared_rank(mine, r) + tid * each;
       if (each == 4) {
         const int4 x = *reinterpret_cast<const int4*>(theirs);
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-      } else {
+        v[0] += x.x; v[1] += x.y; v[MOST - 2] += x.z; v[MOST - 1] += x.w;
+      } else if (each == 2) {
         const int2 x = *reinterpret_cast<const int2*>(theirs);
         v[0] += x.x; v[1] += x.y;
+      } else {
+        v[0] += *theirs;
       }
     }
-    int above = kv4_block_scan(v[0] + v[1] + v[2] + v[3]);
+#pragma unroll
+    for (int d = 0; d < MOST; ++d) all += v[d];
+    int above = kv4_block_scan<N>(all);
 #pragma unroll
     for (int d = 0; d < MOST; ++d) {
       if (above < left && left <= above + v[d]) {
@@ -495,11 +499,10 @@ __device__ __forceinline__ void kv4_keep_body(const Kv4Keep& a, int n, int cap, 
   }
 }
 
-template <int VEC>
-__global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a, int cap, OmniStatus* st) {
+template <int VEC, int N>
+__global__ void __launch_bounds__(N, 1024 / N) kv4_keep_kernel(Kv4Keep a, int cap, OmniStatus* st) {
   extern __shared__ __align__(16) uint32_t s_keys[];
   __shared__ __align__(16) Kv4KeepShared sh;
-  constexpr int N = KV4_KEEP_THREADS;
   const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.y, h = blockIdx.x / size, tid = threadIdx.x;
   int n = max(a.seq_lens[b], 0);
@@ -513,8 +516,8 @@ __global__ void __launch_bounds__(KV4_KEEP_THREADS, 2) kv4_keep_kernel(Kv4Keep a
     for (int j = rank * N + tid; j < a.budget; j += size * N) keep[j] = j < n ? j : -1;
     return;
   }
-  if (kv4_keep_run(n, size) <= cap) kv4_keep_body<true, VEC>(a, n, cap, s_keys, sh, st);
-  else kv4_keep_body<false, VEC>(a, n, cap, s_keys, sh, st);
+  if (kv4_keep_run(n, size) <= cap) kv4_keep_body<true, VEC, N>(a, n, cap, s_keys, sh, st);
+  else kv4_keep_body<false, VEC, N>(a, n, cap, s_keys, sh, st);
 }
 
 struct Kv4Move {
@@ -646,23 +649,30 @@ extern "C" int omni_kv4_keep(const Kv4KeepArgs* p, void* status, cudaStream_t st
   if (p->batch <= 0) return 0;
   const Kv4Keep a = {p->weights, p->positions, p->table, p->seq_lens, p->seen, p->blocks, p->table_ld, p->table_w, p->block, p->hkv,
                      p->budget, p->first, p->last, p->keep, p->lens, p->scratch};
-  // Blocks of a cluster: one for every 8192 places, at most 8; of its keys a block keeps up to 40,000.
+  // Blocks of a cluster: one for every 8192 places, at most 8, while all clusters find room at once (an SM takes one block of 1024 threads,
+  // and the SMs that are left where clusters of 8 do not fit lie idle): 32 items of 60001 places take 25 us with 4 blocks each, 57 with 8; 64 items
+  // 41 with 2 and 51 with 4; 16 of 130000 41 with 4 and 53 with 8; 8 of 20000 20 with 4 and 22 with 2.  A block keeps 40,000 keys;
+  // beyond 8 times that they are made again.
+  const long long items = (long long)p->hkv * p->batch;
   int size = 1;
-  while (size < KV4_MOST_BLOCKS && p->max_len > 8192 * size) size *= 2;
-  const int run = kv4_keep_run(p->max_len, size), cap = run < 1024 ? 1024 : run > 40000 ? 40000 : run;
-  const bool vec = p->block % 4 == 0 && ((uintptr_t)p->weights | (uintptr_t)p->positions) % 16 == 0;
-  const auto kernel = vec ? kv4_keep_kernel<4> : kv4_keep_kernel<1>;
-  static bool asked[2][64] = {{false}};
+  while (size < KV4_MOST_BLOCKS &&
+         (p->max_len > KV4_MOST_KEYS * size || (p->max_len > 8192 * size && items * size * 2 <= (size == 4 ? 112 : 128))))
+    size *= 2;
+  const int run = kv4_keep_run(p->max_len, size), cap = run < 1024 ? 1024 : run > KV4_MOST_KEYS ? KV4_MOST_KEYS : run;
+  // 128 items of 8000 places take 20 us with 1024 threads each and 22 with 512, 128 of 2176 14 and 13.
+  const bool large = p->max_len > 4096, vec = p->block % 4 == 0 && ((uintptr_t)p->weights | (uintptr_t)p->positions) % 16 == 0;
+  const auto kernel = large ? vec ? kv4_keep_kernel<4, 1024> : kv4_keep_kernel<1, 1024> : vec ? kv4_keep_kernel<4, 512> : kv4_keep_kernel<1, 512>;
+  static bool asked[4][64] = {{false}};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev >= 64 || !asked[vec][dev])) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 40000 * 4);
-    if (e == cudaSuccess && dev < 64) asked[vec][dev] = true;
+  if (e == cudaSuccess && (dev >= 64 || !asked[2 * large + vec][dev])) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KV4_MOST_KEYS * 4);
+    if (e == cudaSuccess && dev < 64) asked[2 * large + vec][dev] = true;
   }
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(p->hkv * size, p->batch);
-  config.blockDim = dim3(KV4_KEEP_THREADS);
+  config.blockDim = dim3(large ? 1024 : 512);
   config.dynamicSmemBytes = cap * 4;
   config.stream = stream;
   cudaLaunchAttribute attr = {};

@@ -373,6 +373,22 @@ def test_keep_of_long_requests(lens, budget, bound):
             assert keep[b, h].tolist() == want + [-1] * (budget - len(want))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hkv,block,off,lens", [(1, 10, 0, [2001, 30]), (3, 16, 1, [5000, 999]), (3, 16, 2, [20_000, 4099]), (33, 64, 0, [17_001, 9000])])
+def test_keep_of_any_block_and_address(hkv, block, off, lens):
+    """Blocks of other sizes than a cache's, numbers that do not start on 16 bytes, and more heads than clusters find room for at once."""
+    g, budget, width = _gen(hkv), 500, -(-max(lens) // block)
+    blocks = len(lens) * width
+    table = torch.randperm(blocks, generator=g).view(len(lens), width).to(torch.int32)
+    w = torch.exp(3 * torch.randn(blocks, hkv, block, generator=g))
+    pos = torch.randint(0, max(lens), w.shape, generator=g, dtype=torch.int32)
+    wd, pd = (torch.empty(x.numel() + off, dtype=x.dtype, device="cuda")[off:].view(x.shape).copy_(x) for x in (w, pos))
+    n = torch.tensor(lens, dtype=torch.int32)
+    keep, _ = ops.kv4_keep(wd, pd, table.cuda(), n.cuda(), n.cuda(), budget, keep_first=5, keep_last=20)
+    want, _ = ops.kv4_keep(w, pos, table, n, n, budget, keep_first=5, keep_last=20)
+    assert torch.equal(keep.cpu(), want)
+
+
 @BOTH
 @pytest.mark.parametrize("d,block,hkv", [(64, 16, 3), (128, 48, 2), (256, 32, 1)])
 def test_move(dev, d, block, hkv):
