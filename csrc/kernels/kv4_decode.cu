@@ -20,7 +20,9 @@
 //
 // The query rows of a key/value head (rows x heads of its group, in tiles of 8) are the columns of the products (mma.sync m16n8k16), tokens and
 // then columns of the head their rows: S = K Q^T, O^T = V^T P^T.  So a group of 8 heads wastes nothing, and P^T, which wants tokens along its
-// rows, is what movmatrix makes of S.  tcgen05 products would want 64 or 128 rows and the unpacked codes in shared memory.
+// rows, is what movmatrix makes of S.  tcgen05 products would want 64 or 128 rows and the unpacked codes in shared memory:
+// 128 rows a head over 30,011 tokens twice took 105 us that way, and 99 in tiles of 16 rows here (the softmax of a thread a row, and its waits for
+// products, unpacked tiles and tensor memory, took longer than unpacking a tile 8 times).
 //
 // Each warp walks tiles of 64 tokens (32 at d = 256) by itself: bulk copies of the tile's codes and scales two tiles ahead, an mbarrier
 // for each stage.  No block-wide wait stands in the loop.  The warps' results meet in shared memory at the end, those of the parts of a
@@ -30,6 +32,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../include/kv4.cuh"
 #include "../include/omni_ptx.cuh"
@@ -797,8 +800,9 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, 
 }
 
 // The weights that the rows give a request's tokens: the scores of the staged keys once more, against the finished sums.  Reading the
-// keys twice costs as much as keeping the scores of 8 query rows would, and nothing more for more rows; 16 tokens are unpacked once for
-// all rows, whose fragments stand in shared memory.
+// keys twice costs as much as keeping the scores of 8 query rows would, and nothing more for more rows; 32 tokens (16 at d = 256) are unpacked
+// once for all rows, whose fragments stand in shared memory.  128 rows a key/value head over 30,011 tokens twice take 55 us (16 tokens at a time,
+// one product and one row after the other: 67), bound by the latencies of 12 warps an SM: issue slots are 38% full, tensor pipes 36%.
 template <int NG, int TOK>
 __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decode a, Kv4Cache c, int B, OmniStatus* st) {
   using T = Kv4Tile<NG, false, TOK>;
@@ -806,7 +810,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   __shared__ __align__(8) uint64_t bars[KV4_WARPS * KV4_STAGES];
   __shared__ int abort_flag;
   __shared__ float s_w[KV4_WARPS][TOK];
-  constexpr int ROW = 1 + NG, EACH = (TOK + 31) / 32;
+  constexpr int ROW = 1 + NG, EACH = TOK / 32, SUBS = NG == 4 ? 1 : 2;
   const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + 7) / 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
   uint8_t* stages = smem + warp * (KV4_STAGES * T::BYTES);
@@ -843,7 +847,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int t = of * TOK + i * 32 + lane;
-        place[i] = (EACH > 1 || lane < TOK) && t < stop ? a.table[(long long)b * a.table_ld + t / c.block] : -1;
+        place[i] = t < stop ? a.table[(long long)b * a.table_ld + t / c.block] : -1;
       }
     };
     look(tile);
@@ -857,8 +861,8 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
 #pragma unroll
         for (int x = 0; x < 2; ++x)
           s_q[(ch * NG * 2 + g2 * 2 + x) * 32 + lane] = make_uint4(q.b[g2][2 * x][0], q.b[g2][2 * x][1], q.b[g2][2 * x + 1][0], q.b[g2][2 * x + 1][1]);
-      if (r == 0) {                 // of the rows 2 c and 2 c + 1: their sums (below) and units, and for each group qs and base
-        s_row[(ch * ROW) * 4 + cc] = make_float4(INFINITY, INFINITY, q.unit[0], q.unit[1]);
+      if (r == 0) {                 // of the rows 2 c and 2 c + 1: minus their sums (below), their units, and for each group qs and base
+        s_row[(ch * ROW) * 4 + cc] = make_float4(-INFINITY, -INFINITY, q.unit[0], q.unit[1]);
 #pragma unroll
         for (int g2 = 0; g2 < NG; ++g2) s_row[(ch * ROW + 1 + g2) * 4 + cc] = make_float4(q.qs[g2][0], q.qs[g2][1], q.base[g2][0], q.base[g2][1]);
       }
@@ -866,7 +870,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
     __syncthreads();
     if (first) asm volatile("griddepcontrol.wait;" ::: "memory");         // the sums are there
     for (int row = threadIdx.x; row < total; row += KV4_WARPS * 32)
-      reinterpret_cast<float*>(&s_row[(row / 8 * ROW) * 4 + row % 8 / 2])[row & 1] = a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep];
+      reinterpret_cast<float*>(&s_row[(row / 8 * ROW) * 4 + row % 8 / 2])[row & 1] = -a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep];
     __syncthreads();
     for (; tile < end_tile; tile += KV4_WARPS, next += KV4_WARPS, ++uses) {
       const int st_i = uses % KV4_STAGES;
@@ -882,55 +886,85 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
       look(tile + KV4_WARPS);
       if (!__all_sync(0xffffffffu, mbar_wait(bar + st_i, (uses / KV4_STAGES) & 1, &abort_flag, st, KV4_SITE_WEIGHTS, tile))) break;
 #pragma unroll 1
-      for (int u = 0; u < TOK / 16; ++u) {
+      for (int u = 0; u < TOK / 16; u += SUBS) {
         const int t0 = tile * TOK + u * 16;
         if (t0 >= len) break;
-        const bool edge = t0 + 16 > len - a.rows + 1;
-        Kv4Keys<NG, false, TOK> k;
-        k.load(stage, u);
-        uint32_t f[NG][4][4];
+        uint32_t f[SUBS][NG][4][4];
+        f32x2 step[SUBS][2][NG], low[SUBS][2][NG], sum[SUBS][2];
 #pragma unroll
-        for (int g2 = 0; g2 < NG; ++g2)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) k.fragment(g2, x, f[g2][x]);
-        float sum[2] = {0.f, 0.f};
-#pragma unroll 1
-        for (int ch = 0; ch < chunks; ++ch) {
-          const float4 row = s_row[ch * ROW * 4 + cc];
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < SUBS; ++x) {
+          Kv4Keys<NG, false, TOK> k;
+          k.load(stage, u + x);
 #pragma unroll
           for (int g2 = 0; g2 < NG; ++g2) {
-            const float4 sums = s_row[(ch * ROW + 1 + g2) * 4 + cc];
-            float acc[4] = {sums.z, sums.w, sums.z, sums.w};
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint4 v = s_q[(ch * NG * 2 + g2 * 2 + x) * 32 + lane];
-              const uint32_t b0[2] = {v.x, v.y}, b1[2] = {v.z, v.w};
-              kv4_mma(acc, f[g2][2 * x], b0);
-              kv4_mma(acc, f[g2][2 * x + 1], b1);
-            }
-            const float qs[2] = {sums.x, sums.y};
-            const uint32_t word[2] = {k.sc[0][g2], k.sc[1][g2]};
-            kv4_score(s, acc, word, qs);
-          }
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
+            for (int y = 0; y < 4; ++y) k.fragment(g2, y, f[x][g2][y]);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float p = ex2_fast(fmaf(s[2 * e + x], x ? row.w : row.z, -(x ? row.y : row.x)));
-              if (edge || (ch + 1) * 8 > total) {                         // rows beyond the last, tokens that the row does not see
-                const int i = ch * 8 + cc * 2 + x;
-                if (i >= total || t0 + r + 8 * e >= len - a.rows + 1 + i / rep) p = 0.f;
-              }
-              sum[e] += p;
+              step[x][e][g2] = pack_f32x2(kv4_step(k.sc[e][g2]), kv4_step(k.sc[e][g2]));
+              low[x][e][g2] = pack_f32x2(kv4_low(k.sc[e][g2]), kv4_low(k.sc[e][g2]));
             }
+          }
+          sum[x][0] = sum[x][1] = 0ull;
         }
+        // EDGE: some row does not see all of these tokens.  Rows beyond the last have a weight of 0 by their sums.
+        auto rows = [&](auto edge) {
+#pragma unroll 1
+          for (int ch = 0; ch < chunks; ++ch) {
+            const float4 row = s_row[ch * ROW * 4 + cc];
+            f32x2 s[SUBS][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
-          sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
-          if (cc == 0) s_w[warp][u * 16 + r + 8 * e] = sum[e];
-        }
+            for (int g2 = 0; g2 < NG; ++g2) {
+              const float4 sums = s_row[(ch * ROW + 1 + g2) * 4 + cc];
+              const float base[4] = {sums.z, sums.w, sums.z, sums.w};
+              const f32x2 qs = pack_f32x2(sums.x, sums.y);
+              const uint4 v0 = s_q[(ch * NG * 2 + g2 * 2) * 32 + lane], v1 = s_q[(ch * NG * 2 + g2 * 2 + 1) * 32 + lane];
+              const uint32_t bq[4][2] = {{v0.x, v0.y}, {v0.z, v0.w}, {v1.x, v1.y}, {v1.z, v1.w}};
+              float acc[SUBS][4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int x = 0; x < SUBS; ++x) {
+                  if (y == 0) kv4_mma_from(acc[x], f[x][g2][y], bq[y], base);
+                  else kv4_mma(acc[x], f[x][g2][y], bq[y]);
+                }
+#pragma unroll
+              for (int x = 0; x < SUBS; ++x)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  s[x][e] = fma_f32x2(step[x][e][g2], pack_f32x2(acc[x][2 * e], acc[x][2 * e + 1]), fma_f32x2(low[x][e][g2], qs, g2 == 0 ? 0ull : s[x][e]));
+            }
+#pragma unroll
+            for (int x = 0; x < SUBS; ++x)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float p[2];
+                unpack_f32x2(fma_f32x2(s[x][e], pack_f32x2(row.z, row.w), pack_f32x2(row.x, row.y)), p[0], p[1]);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  p[y] = ex2_fast(p[y]);
+                  if (decltype(edge)::value) {
+                    const int i = ch * 8 + cc * 2 + y;
+                    if (i >= total || t0 + x * 16 + r + 8 * e >= len - a.rows + 1 + i / rep) p[y] = 0.f;
+                  }
+                }
+                sum[x][e] = add_f32x2(sum[x][e], pack_f32x2(p[0], p[1]));
+              }
+          }
+        };
+        if (t0 + SUBS * 16 > len - a.rows + 1) rows(std::true_type{});
+        else rows(std::false_type{});
+#pragma unroll
+        for (int x = 0; x < SUBS; ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float p0, p1;
+            unpack_f32x2(sum[x][e], p0, p1);
+            p0 += p1;
+            p0 += __shfl_xor_sync(0xffffffffu, p0, 1);
+            p0 += __shfl_xor_sync(0xffffffffu, p0, 2);
+            if (cc == 0) s_w[warp][(u + x) * 16 + r + 8 * e] = p0;
+          }
       }
       __syncwarp();
 #pragma unroll
@@ -1055,11 +1089,8 @@ extern "C" int omni_kv4_decode(const Kv4DecodeArgs* p, void* status, cudaStream_
                   : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, n, st, stream) : kv4_launch<2, 1>(a, c, B, n, st, stream)
                              : kv4_launch<4, 1>(a, c, B, n, st, stream);
   if (e != cudaSuccess || p->weights == nullptr) return (int)e;
-  // Many rows make a tile long: shorter ones are shared out more evenly (16 rows of 8 heads over 30,011 tokens twice: 160 us in all, 167
-  // with 64 tokens a tile).
-  const bool fine = p->rows * rep > 32;
-  e = d == 64    ? fine ? kv4_launch_weights<1, 16>(a, c, B, p->max_len, st, stream) : kv4_launch_weights<1, 64>(a, c, B, p->max_len, st, stream)
-      : d == 128 ? fine ? kv4_launch_weights<2, 16>(a, c, B, p->max_len, st, stream) : kv4_launch_weights<2, 64>(a, c, B, p->max_len, st, stream)
-                 : fine ? kv4_launch_weights<4, 16>(a, c, B, p->max_len, st, stream) : kv4_launch_weights<4, 32>(a, c, B, p->max_len, st, stream);
+  e = d == 64    ? kv4_launch_weights<1, 64>(a, c, B, p->max_len, st, stream)
+      : d == 128 ? kv4_launch_weights<2, 64>(a, c, B, p->max_len, st, stream)
+                 : kv4_launch_weights<4, 32>(a, c, B, p->max_len, st, stream);
   return (int)e;
 }
