@@ -26,7 +26,8 @@
 //
 // Each warp walks tiles of 64 tokens (32 at d = 256) by itself: bulk copies of the tile's codes and scales two tiles ahead, an mbarrier
 // for each stage.  No block-wide wait stands in the loop.  The warps' results meet in shared memory at the end, those of the parts of a
-// long request in a second kernel, the weights come from a third, each started while the one ahead of it ends.
+// long request in a second kernel, the weights come from a third, each started while the one ahead of it ends: from scores that the first
+// kept, or, where those would take too much memory, from the keys once more.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -58,6 +59,8 @@ struct Kv4Decode {
   int min_tiles;                    // fewest tiles of a block's share; 0: a block takes one item, whole
   float* o_part;                    // [blocks, 2, 8 NT, d]: what a block has of the item that it starts with, and of the one it ends with
   float* lse_part;                  // [blocks, 2, 8 NT]
+  float* scores;                    // [B, Hkv, chunks, score_places, 8 NT] in units of log 2, or null
+  int score_places;                 // table_w blocks up to a multiple of 64
   int2* shared;                     // [B, Hkv, chunks]: where the parts of an item start (2 block + which), and how many there are
 };
 
@@ -419,9 +422,9 @@ struct Kv4Sums {
       }
   }
 
-  // 32 tokens from `t0` on, from sub `sub0` of the stage.  EDGE: some row does not see all of them.
-  template <bool EDGE>
-  __device__ __forceinline__ void add(const uint8_t* stage, int sub0, int t0, int end, const int (&sees)[NT][2], const Kv4Query<NG> (&q)[NT]) {
+  // 32 tokens from `t0` on, from sub `sub0` of the stage.  EDGE: some row does not see all of them.  KEEP: scores go to memory as well.
+  template <bool EDGE, bool KEEP>
+  __device__ __forceinline__ void add(const uint8_t* stage, int sub0, int t0, int end, const int (&sees)[NT][2], const Kv4Query<NG> (&q)[NT], float* scores) {
     const int lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
     float s[SUBS][NT][4], top[NT][2], steps = 0.f;
     uint32_t vs[SUBS][2][NG];
@@ -472,6 +475,16 @@ struct Kv4Sums {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int x = 0; x < 2; ++x) top[n][x] = fmaxf(top[n][x], fmaxf(s[u][n][x], s[u][n][2 + x]));
+    }
+    if (KEEP) {
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float2*>(scores + (long long)(t0 + u * 16 + r + 8 * e) * (8 * NT) + n * 8 + cc * 2) =
+                make_float2(s[u][n][2 * e] * q[n].unit[0], s[u][n][2 * e + 1] * q[n].unit[1]);
     }
     // The maximum is followed only when a score exceeds it by 2^8: weights in fp32, and in fp16 after to_one, bear that.
     bool more = steps > most;
@@ -570,7 +583,7 @@ struct Kv4Sums {
   }
 };
 
-template <int NG, int NT>
+template <int NG, int NT, bool KEEP>
 __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decode_kernel(Kv4Decode a, Kv4Cache c, int B, OmniStatus* st) {
   using T = Kv4Tile<NG, true>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -631,6 +644,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
 #pragma unroll
       for (int x = 0; x < 2; ++x) sees[n][x] = len - a.rows + 1 + min(row0 + n * 8 + cc * 2 + x, total - 1) / rep;
     }
+    float* scores = KEEP ? a.scores + ((long long)b * items + w.item) * a.score_places * NQ : nullptr;
     Kv4Sums<NG, NT> sum;
     sum.clear();
     for (; tile < stop_tile; tile += KV4_WARPS, next += KV4_WARPS, ++uses) {
@@ -640,8 +654,8 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
 #pragma unroll 1
       for (int sub = 0; sub < T::TOKENS / 16; sub += 2) {
         const int t0 = tile * T::TOKENS + sub * 16;
-        if (t0 + 32 <= first_sees) sum.template add<false>(stage, sub, t0, end, sees, q);
-        else if (t0 < end) sum.template add<true>(stage, sub, t0, end, sees, q);
+        if (t0 + 32 <= first_sees) sum.template add<false, KEEP>(stage, sub, t0, end, sees, q, scores);
+        else if (t0 < end) sum.template add<true, KEEP>(stage, sub, t0, end, sees, q, scores);
       }
       __syncwarp();                                                        // every lane has read the stage
       if (next < stop_tile) feed.start(a, c, min(T::TOKENS, (end - next * T::TOKENS + 15) & ~15), stop, stage, bar + i, st);
@@ -799,8 +813,61 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, 
   if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = sum == 0.f ? -INFINITY : mm + __log2f(sum);
 }
 
-// The weights that the rows give a request's tokens: the scores of the staged keys once more, against the finished sums.  Reading the
-// keys twice costs as much as keeping the scores of 8 query rows would, and nothing more for more rows; 32 tokens (16 at d = 256) are unpacked
+// The weights that the rows give a request's tokens by kept scores and the finished sums.  With one tile of 8 rows a lane takes a token (32 requests of
+// up to 4099 tokens: 9 us, by two lanes a token 12), with tiles of 16 rows 4 of them, so that a warp reads 512 bytes in a row (128 rows, 30,011
+// tokens twice: 36 us, by a lane a token 39).
+template <int NQ>
+__global__ void __launch_bounds__(256) kv4_add_kernel(Kv4Decode a, Kv4Cache c) {
+  constexpr int LANES = NQ == 8 ? 1 : NQ / 4, TOKENS = 256 / LANES, EACH = NQ / LANES / 4;
+  __shared__ __align__(16) float s_lse[256 + NQ];
+  const int rep = a.hq / c.hkv, total = a.rows * rep, chunks = (total + NQ - 1) / NQ;
+  const int h = blockIdx.y, b = blockIdx.z, part = threadIdx.x % LANES;
+  const int len = min(max(a.seq_lens[b], 0), a.table_w * c.block);          // longer ones are reported by the kernel ahead
+  int t = blockIdx.x * TOKENS + threadIdx.x / LANES;
+  float *to, old;
+  auto look = [&] {
+    const int blk = t < len ? a.table[(long long)b * a.table_ld + t / c.block] : -1;
+    to = blk >= 0 && blk < c.blocks ? a.weights + ((long long)blk * c.hkv + h) * c.block + t % c.block : nullptr;
+    old = to != nullptr && a.decay != 0.f ? *to : 0.f;
+  };
+  look();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (blockIdx.x * TOKENS >= len) return;
+  for (int row = threadIdx.x; row < chunks * NQ; row += 256)                // rows beyond the last have a weight of 0
+    s_lse[row] = row < total ? a.lse[((long long)b * a.hq + h * rep + row % rep) * a.rows + row / rep] : INFINITY;
+  __syncthreads();
+  const int all_see = len - a.rows + 1;                                     // tokens that every row sees
+  const float* scores = a.scores + ((long long)b * c.hkv + h) * chunks * a.score_places * NQ + part * (EACH * 4);
+  for (; t - (int)threadIdx.x / LANES < len; t += gridDim.x * TOKENS, look()) {
+    float sum = 0.f;
+    if (t < len) {
+#pragma unroll 4
+      for (int ch = 0; ch < chunks; ++ch) {
+        const float4* from = reinterpret_cast<const float4*>(scores + ((long long)ch * a.score_places + t) * NQ);
+        float4 v[EACH];
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) v[j] = from[j];
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+          const int row = ch * NQ + (part * EACH + j) * 4;
+          const float4 l = *reinterpret_cast<const float4*>(s_lse + row);
+          float p[4] = {ex2_fast(v[j].x - l.x), ex2_fast(v[j].y - l.y), ex2_fast(v[j].z - l.z), ex2_fast(v[j].w - l.w)};
+          if (t >= all_see) {                                               // scores that are not there are dropped as well
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (row + x >= total || t >= all_see + (row + x) / rep) p[x] = 0.f;
+          }
+          sum += (p[0] + p[1]) + (p[2] + p[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (part == 0 && to != nullptr) *to = a.decay == 0.f ? sum : fmaf(a.decay, old, sum);
+  }
+}
+
+// The same without kept scores: those of the staged keys once more, against the finished sums.  32 tokens (16 at d = 256) are unpacked
 // once for all rows, whose fragments stand in shared memory.  128 rows a key/value head over 30,011 tokens twice take 55 us (16 tokens at a time,
 // one product and one row after the other: 67), bound by the latencies of 12 warps an SM: issue slots are 38% full, tensor pipes 36%.
 template <int NG, int TOK>
@@ -1022,20 +1089,27 @@ static cudaError_t kv4_follow(void (*kernel)(Args...), dim3 grid, int threads, i
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
-template <int NG, int NT>
-static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int blocks, OmniStatus* st, cudaStream_t stream) {
+template <int NG, int NT, bool KEEP>
+static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int blocks, int max_len, OmniStatus* st, cudaStream_t stream) {
   using T = Kv4Tile<NG, true>;
   constexpr int merge = KV4_WARPS * 8 * NT * (NG * 64 + 2) * 4, stages = KV4_WARPS * KV4_STAGES * T::BYTES, bytes = merge > stages ? merge : stages;
   const int total = a.rows * (a.hq / c.hkv), chunks = (total + 8 * NT - 1) / (8 * NT);
   const long long grid = a.min_tiles == 0 ? (long long)B * c.hkv * chunks : blocks;
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   static int most[64] = {0};
-  cudaError_t e = kv4_smem((const void*)kv4_decode_kernel<NG, NT>, bytes, most);
+  cudaError_t e = kv4_smem((const void*)kv4_decode_kernel<NG, NT, KEEP>, bytes, most);
   if (e != cudaSuccess) return e;
-  kv4_decode_kernel<NG, NT><<<(unsigned)grid, KV4_WARPS * 32, bytes, stream>>>(a, c, B, st);
+  kv4_decode_kernel<NG, NT, KEEP><<<(unsigned)grid, KV4_WARPS * 32, bytes, stream>>>(a, c, B, st);
   e = cudaGetLastError();
-  if (e != cudaSuccess || a.min_tiles == 0) return e;
-  return kv4_follow(kv4_join_kernel<NT>, dim3(c.hkv * total, B), c.d, blocks * 4, stream, a, c, blocks);
+  if (e == cudaSuccess && a.min_tiles > 0) e = kv4_follow(kv4_join_kernel<NT>, dim3(c.hkv * total, B), c.d, blocks * 4, stream, a, c, blocks);
+  if (e != cudaSuccess || !KEEP) return e;
+  // as many blocks as the longest request has tokens for, while that is no more than two rounds of them
+  const int tokens = NT == 1 ? 256 : 64, want = (max_len + tokens - 1) / tokens, most_x = 148 * 16 / (c.hkv * B), x = want < most_x ? want : most_x;
+  return kv4_follow(kv4_add_kernel<8 * NT>, dim3(x < 1 ? 1 : x, c.hkv, B), 256, 0, stream, a, c);
+}
+template <int NG, int NT>
+static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int blocks, int max_len, OmniStatus* st, cudaStream_t stream) {
+  return a.scores != nullptr ? kv4_launch<NG, NT, true>(a, c, B, blocks, max_len, st, stream) : kv4_launch<NG, NT, false>(a, c, B, blocks, max_len, st, stream);
 }
 
 template <int NG, int TOK>
@@ -1064,6 +1138,7 @@ struct Kv4DecodeArgs {
   void* out;
   float *o_part, *lse_part, *lse, *weights;
   void* shared;                     // int32 [batch, hkv, row tiles, 2]
+  float* scores;                    // [batch, hkv, row tiles, table_w blocks up to a multiple of 64, row_tile]; null: scores are made twice
   long long q_row, blocks;
   int q_head, block, hkv, d, table_ld, table_w, batch, rows, hq, max_len, row_tile, blocks_at_once, min_tiles;
   float scale, decay;
@@ -1081,14 +1156,14 @@ extern "C" int omni_kv4_decode(const Kv4DecodeArgs* p, void* status, cudaStream_
   const int wide_q = (uintptr_t)p->q % 16 == 0 && p->q_row % 8 == 0 && p->q_head % 8 == 0;
   const Kv4Decode a = {(const __nv_bfloat16*)p->q, p->q_row, p->q_head, wide_q, p->table, p->seq_lens, p->table_ld, p->table_w, p->rows, p->hq,
                        p->scale * 1.4426950408889634f, (__nv_bfloat16*)p->out, p->lse, p->weights, p->decay,
-                       p->block % 64 == 0 ? 64 : p->block % 32 == 0 ? 32 : 16, p->min_tiles, p->o_part, p->lse_part, (int2*)p->shared};
+                       p->block % 64 == 0 ? 64 : p->block % 32 == 0 ? 32 : 16, p->min_tiles, p->o_part, p->lse_part, p->weights != nullptr ? p->scores : nullptr, (p->table_w * p->block + 63) / 64 * 64, (int2*)p->shared};
   OmniStatus* st = (OmniStatus*)status;
   const bool wide = p->row_tile == 16;
   const int n = p->blocks_at_once;
-  cudaError_t e = d == 64    ? wide ? kv4_launch<1, 2>(a, c, B, n, st, stream) : kv4_launch<1, 1>(a, c, B, n, st, stream)
-                  : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, n, st, stream) : kv4_launch<2, 1>(a, c, B, n, st, stream)
-                             : kv4_launch<4, 1>(a, c, B, n, st, stream);
-  if (e != cudaSuccess || p->weights == nullptr) return (int)e;
+  cudaError_t e = d == 64    ? wide ? kv4_launch<1, 2>(a, c, B, n, p->max_len, st, stream) : kv4_launch<1, 1>(a, c, B, n, p->max_len, st, stream)
+                  : d == 128 ? wide ? kv4_launch<2, 2>(a, c, B, n, p->max_len, st, stream) : kv4_launch<2, 1>(a, c, B, n, p->max_len, st, stream)
+                             : kv4_launch<4, 1>(a, c, B, n, p->max_len, st, stream);
+  if (e != cudaSuccess || p->weights == nullptr || p->scores != nullptr) return (int)e;
   e = d == 64    ? kv4_launch_weights<1, 64>(a, c, B, p->max_len, st, stream)
       : d == 128 ? kv4_launch_weights<2, 64>(a, c, B, p->max_len, st, stream)
                  : kv4_launch_weights<4, 32>(a, c, B, p->max_len, st, stream);

@@ -174,7 +174,7 @@ _ARGS = {
     "omni_kv4_read": struct.Struct("5Q2q4i"),
     "omni_kv4_keep": struct.Struct("8Q1q10i"),
     "omni_kv4_move": struct.Struct("6Q1q8i"),
-    "omni_kv4_decode": struct.Struct("11Q2q13i2fi"),
+    "omni_kv4_decode": struct.Struct("12Q2q13i2fi"),
 }
 _bound = {}
 
@@ -284,6 +284,12 @@ def kv4_read(k_cache, v_cache, slots):
     return k, v
 
 
+# Bytes up to which the scores of a call are kept for its weights (a number for each row that a tile of them has, key/value head and place of
+# the block table); beyond they are made from the keys once more.  Kept, 32 requests of up to 4099 tokens and 8 rows a key/value head take
+# 38 us and not 46, 64 of 16,384 199 and not 260, two of 131,072 with 128 rows 557 and not 573: it is the memory that sets the bound.
+KEPT_SCORES = 256 << 20
+
+
 def _blocks(items, tiles, resident):
     """(blocks, fewest tiles of one) for ``items`` passes over up to ``tiles`` tiles each, with ``resident`` blocks on each of the 148
     SMs; 0 tiles: a block takes a pass, whole."""
@@ -300,7 +306,8 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
     ``weights`` [blocks, Hkv, block] fp32: of every place below seq_lens[b] becomes decay * weights + the softmax weights that the
     rows and the query heads of its key/value head give it (decay 0: whatever was there is dropped).  Requests that share a block
     would write the same numbers: give ``weights`` only where blocks belong to one request.  At most 256 rows times query
-    heads of a key/value head then.  ``max_seq_len`` (a bound of
+    heads of a key/value head then.  Up to 256 MiB go to scores meanwhile: 32 bytes (8 rows) to 1 KiB (256) for each place of the table
+    and key/value head, so a table no wider than needed saves memory.  ``max_seq_len`` (a bound of
     ``seq_lens``) shapes the launch; without it the width of the block table does."""
     blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
     _check_rows("q", q, None, d, device)
@@ -322,6 +329,10 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
         items = B * hkv * -(-total // tile)
         blocks_at_once, min_tiles = _blocks(items, -(-longest // (32 if d == 256 else 64)), 3 if tile * d <= 1024 else 2)
         lse = torch.empty(T * hq, dtype=torch.float32, device=device) if weights is not None else None
+        places = -(-width * block // 64) * 64
+        scores = None
+        if weights is not None and items * tile * places * 4 <= KEPT_SCORES:
+            scores = torch.empty(items * tile * places, dtype=torch.float32, device=device)
         o_part = lse_part = shared = 0
         if min_tiles:                                        # partial results, their sums, where the parts of an item are
             n = blocks_at_once * 2 * tile
@@ -329,7 +340,7 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
             o_part = scratch.data_ptr()
             lse_part, shared = o_part + 4 * n * d, o_part + 4 * n * (d + 1)
         _call("omni_kv4_decode", device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(),
-              o_part, lse_part, _p(lse), _p(weights), shared, q.stride(0), blocks, q.stride(1), block, hkv, d, block_table.stride(0), width, B, T // B, hq, longest, tile,
+              o_part, lse_part, _p(lse), _p(weights), shared, _p(scores), q.stride(0), blocks, q.stride(1), block, hkv, d, block_table.stride(0), width, B, T // B, hq, longest, tile,
               blocks_at_once, min_tiles, scale, decay, 0)
     return out
 

@@ -5,6 +5,7 @@ import torch
 import kv4_oracle as O
 from omni_infer_b200 import ops
 from omni_infer_b200.ops import _native as nat
+from omni_infer_b200.ops import kv4
 
 GPU = pytest.param("cuda", marks=pytest.mark.gpu)
 BOTH = pytest.mark.parametrize("dev", ["cpu", GPU])
@@ -421,6 +422,39 @@ def test_move(dev, d, block, hkv):
     got = [x.cpu() for x in ops.kv4_read(f.k_cache, f.v_cache, everything)] + [wd.cpu(), pd.cpu()]
     for a, b in zip(got, want):
         assert torch.equal(a.float().nan_to_num(nan=1e9), b.float().nan_to_num(nan=1e9))
+
+
+# ----------------------------------------------------------------------------- without room for scores
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["set", "add"])
+@pytest.mark.parametrize("lens,rows,hq,hkv,d,block", SHAPES)
+def test_weights_of_scores_that_are_not_kept(monkeypatch, lens, rows, hq, hkv, d, block, mode):
+    monkeypatch.setattr(kv4, "KEPT_SCORES", 0)
+    test_attention("cuda", lens, rows, hq, hkv, d, block, mode)
+
+
+@pytest.mark.gpu
+def test_long_and_extreme_scores_that_are_not_kept(monkeypatch):
+    monkeypatch.setattr(kv4, "KEPT_SCORES", 0)
+    for bound in (None, 1, 700):
+        test_attention_is_split_over_long_caches(bound, 2, 9001, 2, 5)
+    for rows in (1, 5):
+        test_rising_scores("cuda", rows)
+        test_attention_of_any_magnitude("cuda", 40.0, 1.0, 1.0, 0.09, rows)
+        test_attention_of_any_magnitude("cuda", 1.0, 1.0, 1.0, -0.3, rows)
+
+
+@pytest.mark.gpu
+def test_weights_of_a_wide_table():
+    """A table far wider than the requests: nothing of it counts but what they have."""
+    f = Filled(3, [130, 64, 1], 2, 128, 64, "cuda")
+    wide = torch.full((3, 2000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :f.table_dev.shape[1]] = f.table_dev
+    q = torch.randn(3, 6, 128, generator=_gen(2)).bfloat16().cuda()
+    for bound in (None, 130):
+        w = torch.ones(f.k_cache.shape[:3], device="cuda")
+        out = ops.kv4_decode(q, f.k_cache, f.v_cache, wide, f.lens_dev, 0.1, max_seq_len=bound, weights=w, decay=0.5)
+        _check_decode(f, q, 1, 0.1, out, w, torch.ones(f.k_cache.shape[:3]), 0.5)
 
 
 # ----------------------------------------------------------------------------- together
