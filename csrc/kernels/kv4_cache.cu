@@ -14,6 +14,7 @@
 
 #include "../include/kv4.cuh"
 #include "../include/omni_ptx.cuh"
+#include "../include/score_mod.cuh"
 
 namespace omni {
 
@@ -55,15 +56,24 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Cache& c, long long slot,
   return {-1, 0};
 }
 
-// round(x / step), ties to even, for 0 <= x <= 15 step.  The product with the inverse is a whole number at most one off after 1.5 2^23 has
-// rounded it into the lowest bits; code * step is exact (4 and 8 bits) and x - code * step as well (no bit of it lies below those of x and of
-// the step), so that comparing it with half a step settles the code.
-__device__ __forceinline__ uint32_t kv4_nearest(float x, float step, float inverse) {
-  const float up = __fadd_rn(__fmul_rn(x, inverse), 12582912.f);
-  const float off = __fmaf_rn(-__fsub_rn(up, 12582912.f), step, x), twice = 2.f * fabsf(off);
-  uint32_t code = __float_as_uint(up);
-  if (twice > step || (twice == step && (code & 1u))) code += off > 0.f ? 1u : ~0u;
-  return code & 15u;
+// Word of the codes round((x - low) / step), ties to even, of 8 columns, all times `lift` (a power of two that leaves step and inverse normal).
+// The inverse is at most 2^-20 of it too small, never too large, so that code = floor((x - low) inverse) is the quotient's floor or one less, which
+// an addition that rounds down leaves in the lowest bits.  The remainder off = x - low - code step is exact (code step has 12 bits, and no bit
+// of the rest lies below those of x - low and of step); it is not negative and one more is right where it is more than half a step, or
+// half a step and the code odd: a comparison of their bits as whole numbers.
+__device__ __forceinline__ uint32_t kv4_word(const __nv_bfloat162 (&x)[4], float low, float step, float lift) {
+  const float unit = step * lift, inverse = rcp_fast(unit) * (1.f - 0x1p-21f);
+  const int half = __float_as_int(0.5f * unit);
+  uint32_t word = 0, over = 0;      // over: the sums' exponents, shifted along with the codes
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    const float v = __fsub_rn(i & 1 ? __high2float(x[i / 2]) : __low2float(x[i / 2]), low) * lift;
+    const float sum = __fmaf_rd(v, inverse, 12582912.f), off = __fmaf_rn(12582912.f - sum, unit, v);
+    const uint32_t code = __float_as_uint(sum);
+    word = word * 16u + code + ((uint32_t)(half - __float_as_int(off) - (int)(code & 1u)) >> 31);
+    over = over * 16u + 0x4b400000u;
+  }
+  return word - over;
 }
 
 template <int D>
@@ -90,13 +100,13 @@ __device__ __forceinline__ long long kv4_unit(const Kv4Rows& a, const Kv4Cache& 
   return tok;
 }
 
-// The 8 lanes of a group find its range with three shuffles.  Reads 2 d bytes and writes 9 d / 16 a row; bound by its
-// instructions.
+// The 8 lanes of a group find its range, as the smallest of x and of -x, with three shuffles.  Reads 2 d bytes and writes 9 d / 16 a row; bound
+// by its instructions: 4099 tokens of 8 heads in 12 us, 30,000 in 58 (2.5 TB/s).  32 registers a thread (8 blocks an SM) beat 48 and 56.
 template <int D, bool VEC>
-__global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows a, Kv4Cache c, OmniStatus* st) {
+__global__ void __launch_bounds__(256, 8) kv4_write_kernel(Kv4Rows a, Kv4Cache c, OmniStatus* st) {
   using L = Kv4Lane<D>;
   const L lane;
-  const long long warps = (long long)gridDim.x * 8;
+  const long long warps = (long long)gridDim.x * 8, head_bytes = c.piece() * L::HEADS;
   for (long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); unit < a.n * a.parts; unit += warps) {
     int from, to;
     const long long tok = kv4_unit(a, c, unit, from, to);
@@ -105,15 +115,15 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows a, Kv4Cache c, O
 #pragma unroll
     for (int side = 0; side < L::SIDES; ++side) {
       const bool values = L::SIDES == 2 ? side == 1 : lane.values;
-      const __nv_bfloat16* rows = (values ? a.v + tok * a.v_row : a.k + tok * a.k_row) + lane.u * 8;
-      const int head_step = values ? a.v_head : a.k_head;
+      const int h = from + lane.head;
+      const long long head_step = (long long)(values ? a.v_head : a.k_head);
+      const __nv_bfloat16* src = (values ? a.v + tok * a.v_row : a.k + tok * a.k_row) + lane.u * 8 + h * head_step;
       uint8_t* cache = values ? c.v : c.k;
+      uint8_t *codes = cache + lane.word(c, p, values, h), *scales = cache + lane.scale(c, p, h);
+      int left = to - h;                                                    // heads of this lane that there are to write
       for (int h0 = from; h0 < to; h0 += L::HEADS) {
-        const int h = h0 + lane.head;
-        const bool in = h < to;
-        const __nv_bfloat16* src = rows + (long long)h * head_step;
         __nv_bfloat162 x[4];
-        if (!in) {
+        if (left <= 0) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[j] = __float2bfloat162_rn(0.f);
         } else if (VEC) {
@@ -124,40 +134,37 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows a, Kv4Cache c, O
         }
         const __nv_bfloat162 lo2 = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3]));
         const __nv_bfloat162 hi2 = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
-        __nv_bfloat16 lo = __hmin_nan(__low2bfloat16(lo2), __high2bfloat16(lo2)), hi = __hmax_nan(__low2bfloat16(hi2), __high2bfloat16(hi2));
+        auto least = [](uint32_t p, uint32_t q) {
+          const __nv_bfloat162 m = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&p), *reinterpret_cast<__nv_bfloat162*>(&q));
+          return *reinterpret_cast<const uint32_t*>(&m);
+        };
+        const uint32_t lo = *reinterpret_cast<const uint32_t*>(&lo2), hi = *reinterpret_cast<const uint32_t*>(&hi2) ^ 0x80008000u;
+        uint32_t ends = least(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));      // smallest, minus the largest
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-          lo = __hmin_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-          hi = __hmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
-        const float low = __bfloat162float(lo), range = __fsub_rn(__bfloat162float(hi), low);
+        for (int o = 4; o > 0; o >>= 1) ends = least(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+        const float low = __uint_as_float(ends << 16), range = __fsub_rn(__uint_as_float((ends & 0xffff0000u) ^ 0x80000000u), low);
         float step = __uint_as_float((__float_as_uint(__fdiv_rn(range, 15.f)) + 0xffffu) & 0xffff0000u);
         if (!(range < INFINITY)) step = __uint_as_float(0x7fc00000u);                                     // NaN or infinite
         uint32_t word = 0;
-        if (step > 0.f) {
-          const float lift = step < 0x1p-100f ? 0x1p60f : 1.f, unit = step * lift, inverse = __frcp_rn(unit);      // an inverse that is finite
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = __bfloat1622float2(x[j]);
-            word |= (kv4_nearest(__fsub_rn(f.x, low) * lift, unit, inverse) | kv4_nearest(__fsub_rn(f.y, low) * lift, unit, inverse) << 4) << (8 * j);
-          }
+        if (step >= 0x1p-100f) word = kv4_word(x, low, step, 1.f);
+        else if (step > 0.f) word = kv4_word(x, low, step, 0x1p60f);
+        if (left > 0) {
+          *reinterpret_cast<uint32_t*>(codes) = word;
+          if ((lane.u & 7) == 0) *reinterpret_cast<uint32_t*>(scales) = (__float_as_uint(step) >> 16) | ends << 16;
+          if (lane.u == 0 && !values && a.weights != nullptr) a.weights[(p.blk * c.hkv + h0 + lane.head) * c.block + p.t] = 0.f;
+          if (lane.u == 0 && !values && a.positions != nullptr) a.positions[(p.blk * c.hkv + h0 + lane.head) * c.block + p.t] = (int)a.token_positions[tok];
         }
-        if (!in) continue;
-        *reinterpret_cast<uint32_t*>(cache + lane.word(c, p, values, h)) = word;
-        if ((lane.u & 7) == 0)
-          *reinterpret_cast<uint32_t*>(cache + lane.scale(c, p, h)) = (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
-        if (lane.u == 0 && !values) {
-          const long long at = (p.blk * c.hkv + h) * c.block + p.t;
-          if (a.weights != nullptr) a.weights[at] = 0.f;
-          if (a.positions != nullptr) a.positions[at] = (int)a.token_positions[tok];
-        }
+        codes += head_bytes;
+        scales += head_bytes;
+        src += L::HEADS * head_step;
+        left -= L::HEADS;
       }
     }
   }
 }
 
 // The inverse: a word of codes and its group's word to 8 bf16 values, four words a lane under way.  Reads 9 d / 16 bytes and writes 2 d a row:
-// 40,003 tokens of 8 heads in 37 us, 5.6 TB/s; 32 registers a thread (8 blocks an SM) beat 42 and 57 of them.
+// 40,003 tokens of 8 heads in 39 us, 5.4 TB/s; 32 registers a thread (8 blocks an SM) beat 42 and 57 of them.
 template <int D>
 __global__ void __launch_bounds__(256, 8) kv4_read_kernel(Kv4Rows a, Kv4Cache c, OmniStatus* st) {
   using L = Kv4Lane<D>;
@@ -208,8 +215,8 @@ __global__ void __launch_bounds__(256, 8) kv4_read_kernel(Kv4Rows a, Kv4Cache c,
   }
 }
 // Blocks of 8 warps, as many as fit the card four times over at most.  A token's heads are shared out to several warps while there are fewer
-// warps than `want`: 64 tokens of 4 heads are written and read back in 7 us, by a warp a token in 14; 4099 tokens of 8 heads written take
-// 18 us, by a warp a head 21, by a warp a token 26.
+// warps than `want`: 64 tokens of 4 heads are written and read back in 7 us, by a warp a token in 14; 1000 tokens of 8 heads written take
+// 5.6 us, by a warp a token 8.2; 4099 take 12, by a warp a head 16.
 static unsigned kv4_row_blocks(Kv4Rows& a, const Kv4Cache& c, long long want) {
   const int heads = c.d == 64 ? 2 : 1, steps = (c.hkv + heads - 1) / heads;
   const long long share = (want + a.n - 1) / a.n;
@@ -603,7 +610,7 @@ extern "C" int omni_kv4_write(const Kv4WriteArgs* p, void* status, cudaStream_t 
   a.weights = p->weights;
   a.positions = p->positions;
   a.token_positions = p->token_positions;
-  const unsigned grid = kv4_row_blocks(a, c, 148 * 128);
+  const unsigned grid = kv4_row_blocks(a, c, 148 * 32);
   const bool vec = ((uintptr_t)p->k | (uintptr_t)p->v) % 16 == 0 && (p->k_row | p->v_row) % 8 == 0 && (p->k_head | p->v_head) % 8 == 0;
   const auto kernel = p->d == 64    ? vec ? kv4_write_kernel<64, true> : kv4_write_kernel<64, false>
                       : p->d == 128 ? vec ? kv4_write_kernel<128, true> : kv4_write_kernel<128, false>
