@@ -94,7 +94,8 @@ def _values_ref(cache, blk, t, values, head=None):
     blk, head = blk[..., None], head[..., None]
     codes = (flat[blk, head, byte] >> shift & 15).float().unflatten(-1, (-1, GROUP))
     scales = flat[blk, head, sc].contiguous().view(torch.bfloat16).float().unflatten(-1, (-1, 2))
-    return (codes * scales[..., :1] + scales[..., 1:]).flatten(-2)
+    # 15 steps may be beyond fp32 where 15 steps and the lowest value are not
+    return (codes.double() * scales[..., :1] + scales[..., 1:]).float().flatten(-2)
 
 
 def kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights=None, decay=1.0):
@@ -302,6 +303,7 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
     """Attention of the last tokens of every request over its cached ones: q [B n, Hq, d] bf16 (any row and head pitch), the ``n``
     rows of a request one after the other; row i sees the first ``seq_lens[b] - n + 1 + i`` of the request's places (none: zeros).
     ``block_table`` [B, blocks of a request] int32, ``seq_lens`` [B] int32, with the rows' own tokens.  Returns [B n, Hq, d].
+    On a GPU the largest number of a query row is brought to 2^13 .. 2^14: keys beyond 2^98 may leave the range of the fp32 sums.
 
     ``weights`` [blocks, Hkv, block] fp32: of every place below seq_lens[b] becomes decay * weights + the softmax weights that the
     rows and the query heads of its key/value head give it (decay 0: whatever was there is dropped).  Requests that share a block

@@ -118,6 +118,30 @@ def test_groups_at_the_edges_of_the_format(dev):
 
 
 @BOTH
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_groups_of_all_exponents(dev, d):
+    """Columns of every size within a group, ties between codes, the smallest steps, and ranges just below the largest fp32 number, where
+    15 steps are beyond it and 15 steps and the lowest value are not."""
+    g, T, hkv, block = _gen(d), 96, 2, 16
+    x = torch.randn(T, hkv, d, generator=g)
+    sign = torch.sign(x)
+    x[0:16] = torch.randint(-8, 9, (16, hkv, d), generator=g).float() / 2                      # ties
+    x[16:32] = torch.exp2(torch.randint(-133, 127, (16, hkv, d), generator=g).float()) * sign[16:32]
+    x[32:48] *= torch.exp2(torch.randint(-133, 120, (16, hkv, 1), generator=g).float())
+    x[48:64] = torch.randint(0, 16, (16, hkv, d), generator=g) * 2.0 ** -133 - 2.0 ** -130      # the smallest bf16 numbers
+    x[64:80] = torch.randint(0, 31, (16, hkv, d), generator=g) * 2.0 ** torch.randint(-20, 20, (16, hkv, 1), generator=g)
+    x[80:96, :, 0::64], x[80:96, :, 1::64] = 2.5e38, torch.linspace(-8.6e37, -9.1e37, 16)[:, None, None].expand(16, hkv, d // 64)
+    x = x.bfloat16()
+    slots = torch.randperm(T, generator=g)
+    kc, vc = ops.kv4_cache(T // block, block, hkv, d, dev)
+    ops.kv4_write(x.to(dev), x.flip(0).contiguous().to(dev), slots.to(dev), kc, vc)
+    want = O.stored(x)[0].float().bfloat16()
+    for got, w in zip(ops.kv4_read(kc, vc, slots.to(dev)), (want, want.flip(0))):
+        assert torch.equal(got.cpu().isnan(), w.isnan())
+        assert torch.equal(got.cpu()[~w.isnan()], w[~w.isnan()])
+
+
+@BOTH
 def test_no_rows(dev):
     kc, vc = ops.kv4_cache(1, 16, 2, 64, dev)
     none = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=dev)
