@@ -232,9 +232,10 @@ def _check_per_place(name, x, shape, device, dtype=torch.float32):
     assert x.dtype is dtype and x.device == device and x.is_contiguous() and x.shape == shape, f"{name}: contiguous {dtype} {list(shape)} on {device}"
 
 
-def _check_table(table, device, B):
+def _check_table(table, device, B, block):
     assert table.dtype is torch.int32 and table.device == device and table.dim() == 2 and table.shape[0] >= B and table.stride(1) == 1, \
         f"block_table: int32 on {device}, a row without gaps for each of the {B} requests"
+    assert table.shape[1] * block < 1 << 30, f"block_table: fewer than 2^30 places for a request: {table.shape[1]} blocks of {block}"
 
 
 def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token_positions=None):
@@ -317,7 +318,7 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
     T, hq, B = q.shape[0], q.shape[1], seq_lens.shape[0]
     assert hq > 0 and hq % hkv == 0, f"{hq} query heads do not divide over {hkv} key/value heads"
     assert T == 0 if B == 0 else T > 0 and T % B == 0, f"{T} rows are not the same number for each of {B} requests"
-    _check_table(block_table, device, B)
+    _check_table(block_table, device, B, block)
     if weights is not None:
         _check_per_place("weights", weights, (blocks, hkv, block), device)
     if not q.is_cuda:
@@ -364,7 +365,7 @@ def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first
     _check_numbers("seq_lens", seq_lens, None, device)
     B = seq_lens.shape[0]
     _check_numbers("seen", seen, B, device)
-    _check_table(block_table, device, B)
+    _check_table(block_table, device, B, block)
     assert budget >= 1 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, \
         f"a budget of {budget} tokens holds at least the {keep_first} first and {keep_last} last ones"
     if not weights.is_cuda:
@@ -389,7 +390,7 @@ def kv4_move(k_cache, v_cache, block_table, keep, weights=None, positions=None):
     assert keep.dim() == 3 and keep.shape[1] == hkv and keep.is_contiguous() and keep.dtype is torch.int32 and keep.device == device, \
         f"keep: contiguous int32 [B, {hkv}, budget] on {device}"
     B, _, budget = keep.shape
-    _check_table(block_table, device, B)
+    _check_table(block_table, device, B, block)
     if weights is not None:
         _check_per_place("weights", weights, (blocks, hkv, block), device)
     if positions is not None:

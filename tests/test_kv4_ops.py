@@ -646,6 +646,7 @@ REFUSED = {
     "table rows": lambda a: ops.kv4_decode(a["q"], a["kc"], a["vc"], a["table"][:1], a["lens"], 1.0),
     "lengths type": lambda a: ops.kv4_decode(a["q"], a["kc"], a["vc"], a["table"], a["lens"].long(), 1.0),
     "decode weights type": lambda a: ops.kv4_decode(a["q"], a["kc"], a["vc"], a["table"], a["lens"], 1.0, weights=a["w"].double()),
+    "table too wide": lambda a: ops.kv4_decode(a["q"], a["kc"], a["vc"], torch.empty(1 << 26, dtype=torch.int32).expand(len(a["lens"]), -1), a["lens"], 0.1),
     "budget too small": lambda a: ops.kv4_keep(a["w"], a["pos"], a["table"], a["lens"], a["lens"], 4, keep_first=3, keep_last=2),
     "no budget": lambda a: ops.kv4_keep(a["w"], a["pos"], a["table"], a["lens"], a["lens"], 0),
     "positions type": lambda a: ops.kv4_keep(a["w"], a["pos"].long(), a["table"], a["lens"], a["lens"], 4),
