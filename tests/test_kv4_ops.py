@@ -468,6 +468,24 @@ def test_long_and_extreme_scores_that_are_not_kept(monkeypatch):
         test_attention_of_any_magnitude("cuda", 1.0, 1.0, 1.0, -0.3, rows)
 
 
+@BOTH
+@pytest.mark.parametrize("room", [0, 1 << 28])
+def test_weights_of_a_nan(monkeypatch, dev, room):
+    """A key that is not finite makes the weights of its head's whole request NaN, and no others."""
+    monkeypatch.setattr(kv4, "KEPT_SCORES", room)
+    lens = [100, 900]
+    f = Filled(21, lens, 2, 128, 16, dev)
+    f.k[1][20, 0, 0] = float("inf")
+    ops.kv4_write(f.k[1].to(dev), f.v[1].to(dev), f.slots[1].to(dev), f.k_cache, f.v_cache)
+    q = torch.randn(2, 6, 128, generator=_gen(1)).bfloat16().to(dev)
+    w = torch.full(f.k_cache.shape[:3], 0.5, device=dev)
+    ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.1, weights=w, decay=0.5)
+    nan = torch.zeros(w.shape, dtype=torch.bool)
+    for i in range(lens[1]):
+        nan[f.table[1, i // 16], 0, i % 16] = True
+    assert torch.equal(w.isnan().cpu(), nan)
+
+
 @pytest.mark.gpu
 def test_weights_of_a_wide_table():
     """A table far wider than the requests: nothing of it counts but what they have."""
