@@ -278,14 +278,14 @@ constexpr int KV4_BINS = 2048, KV4_MOST_BLOCKS = 8, KV4_MOST_KEYS = 40000;
 __host__ __device__ constexpr int kv4_keep_run(int n, int size) { return ((n + size - 1) / size + 3) & ~3; }      // places of a block
 struct Kv4KeepShared {
   int hist[2][KV4_BINS];            // highest keys first
-  int run[3][32];                                                 // of the warps' runs: equal keys, places to fill, tokens that fill some
+  int run[3][32];                   // of the warps' runs: equal keys, places to fill, tokens that fill some
   int count[2];                     // of this block: places to fill, tokens that fill some
   int equal;                        // keys equal to the last that stays in the blocks ahead
   uint32_t prefix;
   int left, all;
 };
-// ALL: the keys of a run find room in shared memory.  VEC: places that are read at once, 4 where blocks and addresses allow (a run is 15 keys a
-// thread of two blocks an SM: it is instructions that count, not bytes).
+// ALL: the keys of a run find room in shared memory.  VEC: places that are read at once, 4 where blocks and addresses allow (15 keys a thread and
+// 32 warps an SM are bound by instructions, not bytes).
 template <bool ALL, int VEC, int N>
 __device__ __forceinline__ void kv4_keep_body(const Kv4Keep& a, int n, int cap, uint32_t* s_keys, Kv4KeepShared& sh, OmniStatus* st) {
   namespace cg = cooperative_groups;

@@ -217,14 +217,19 @@ def _check_caches(k_cache, v_cache):
 
 
 def _check_rows(name, x, hkv, d, device):
-    assert x.dtype is torch.bfloat16 and x.device == device and x.dim() == 3 and x.stride(2) == 1 and x.shape[2] == d and (hkv is None or x.shape[1] == hkv), \
+    """(shape, stride) of rows; each is asked for once, since asking costs as much as a check."""
+    shape, stride = x.shape, x.stride()
+    assert x.dtype is torch.bfloat16 and x.device == device and len(shape) == 3 and stride[2] == 1 and shape[2] == d and (hkv is None or shape[1] == hkv), \
         f"{name}: bf16 [rows, {'heads' if hkv is None else hkv}, {d}] on {device}, columns without gaps"
+    return shape, stride
 
 
 def _check_numbers(name, x, n, device, dtype=torch.int32):
-    """One number for each of n requests or tokens (any number of them: n None)."""
-    assert x.dtype is dtype and x.device == device and x.dim() == 1 and x.is_contiguous() and (n is None or x.shape[0] == n), \
+    """How many there are of one number for each of n requests or tokens (any number of them: n None)."""
+    shape = x.shape
+    assert x.dtype is dtype and x.device == device and len(shape) == 1 and x.is_contiguous() and (n is None or shape[0] == n), \
         f"{name}: contiguous {dtype} [{'n' if n is None else n}] on {device}"
+    return shape[0]
 
 
 def _check_per_place(name, x, shape, device, dtype=torch.float32):
@@ -233,9 +238,12 @@ def _check_per_place(name, x, shape, device, dtype=torch.float32):
 
 
 def _check_table(table, device, B, block):
-    assert table.dtype is torch.int32 and table.device == device and table.dim() == 2 and table.shape[0] >= B and table.stride(1) == 1, \
+    """(blocks of a request, row pitch)"""
+    shape, stride = table.shape, table.stride()
+    assert table.dtype is torch.int32 and table.device == device and len(shape) == 2 and shape[0] >= B and stride[1] == 1, \
         f"block_table: int32 on {device}, a row without gaps for each of the {B} requests"
-    assert table.shape[1] * block < 1 << 30, f"block_table: fewer than 2^30 places for a request: {table.shape[1]} blocks of {block}"
+    assert shape[1] * block < 1 << 30, f"block_table: fewer than 2^30 places for a request: {shape[1]} blocks of {block}"
+    return shape[1], stride[0]
 
 
 def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token_positions=None):
@@ -243,10 +251,9 @@ def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token
     block; negative: not stored).  The slots of a call differ.  ``weights`` / ``positions`` [blocks, Hkv, block], where given, are
     set to 0 and to ``token_positions`` [T] int64 in those slots."""
     blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
-    _check_rows("k", k, hkv, d, device)
-    _check_rows("v", v, hkv, d, device)
-    T = k.shape[0]
-    assert v.shape[0] == T, "a row of v for every row of k"
+    (T, *_), (k_row, k_head, _) = _check_rows("k", k, hkv, d, device)
+    (v_rows, *_), (v_row, v_head, _) = _check_rows("v", v, hkv, d, device)
+    assert v_rows == T, "a row of v for every row of k"
     _check_numbers("slots", slots, T, device, torch.int64)
     assert (positions is None) == (token_positions is None), "positions and token_positions come together"
     if weights is not None:
@@ -267,14 +274,13 @@ def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token
     if T == 0:
         return
     _call("omni_kv4_write", device, k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(weights), _p(positions), _p(token_positions),
-          k.stride(0), v.stride(0), T, blocks, k.stride(1), v.stride(1), block, hkv, d, 0)
+          k_row, v_row, T, blocks, k_head, v_head, block, hkv, d, 0)
 
 
 def kv4_read(k_cache, v_cache, slots):
     """(k, v) [T, Hkv, d] bf16 of the slots ``slots`` [T] int64; zeros for negative ones.  A slot may be named more than once."""
     blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
-    _check_numbers("slots", slots, None, device, torch.int64)
-    T = slots.shape[0]
+    T = _check_numbers("slots", slots, None, device, torch.int64)
     if not k_cache.is_cuda:
         s = slots.clamp_min(0)
         ok = (slots >= 0)[:, None, None]
@@ -313,19 +319,18 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
     and key/value head, so a table no wider than needed saves memory.  ``max_seq_len`` (a bound of
     ``seq_lens``) shapes the launch; without it the width of the block table does."""
     blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
-    _check_rows("q", q, None, d, device)
-    _check_numbers("seq_lens", seq_lens, None, device)
-    T, hq, B = q.shape[0], q.shape[1], seq_lens.shape[0]
+    (T, hq, _), (q_row, q_head, _) = _check_rows("q", q, None, d, device)
+    B = _check_numbers("seq_lens", seq_lens, None, device)
     assert hq > 0 and hq % hkv == 0, f"{hq} query heads do not divide over {hkv} key/value heads"
     assert T == 0 if B == 0 else T > 0 and T % B == 0, f"{T} rows are not the same number for each of {B} requests"
-    _check_table(block_table, device, B, block)
+    width, table_ld = _check_table(block_table, device, B, block)
     if weights is not None:
         _check_per_place("weights", weights, (blocks, hkv, block), device)
     if not q.is_cuda:
         return kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights, decay)
     out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=device)
     if T:
-        width, total = block_table.shape[1], T // B * (hq // hkv)
+        total = T // B * (hq // hkv)
         assert weights is None or total <= 256, f"weights of at most 256 query rows a key/value head at once: {total}"
         longest = width * block if max_seq_len is None else max(0, min(max_seq_len, width * block))
         tile = 16 if d <= 128 and total > 8 else 8
@@ -343,7 +348,7 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
             o_part = scratch.data_ptr()
             lse_part, shared = o_part + 4 * n * d, o_part + 4 * n * (d + 1)
         _call("omni_kv4_decode", device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(),
-              o_part, lse_part, _p(lse), _p(weights), shared, _p(scores), q.stride(0), blocks, q.stride(1), block, hkv, d, block_table.stride(0), width, B, T // B, hq, longest, tile,
+              o_part, lse_part, _p(lse), _p(weights), shared, _p(scores), q_row, blocks, q_head, block, hkv, d, table_ld, width, B, T // B, hq, longest, tile,
               blocks_at_once, min_tiles, scale, decay, 0)
     return out
 
@@ -362,10 +367,9 @@ def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first
     blocks, hkv, block = shape
     _check_per_place("weights", weights, shape, device)
     _check_per_place("positions", positions, shape, device, torch.int32)
-    _check_numbers("seq_lens", seq_lens, None, device)
-    B = seq_lens.shape[0]
+    B = _check_numbers("seq_lens", seq_lens, None, device)
     _check_numbers("seen", seen, B, device)
-    _check_table(block_table, device, B, block)
+    width, table_ld = _check_table(block_table, device, B, block)
     assert budget >= 1 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, \
         f"a budget of {budget} tokens holds at least the {keep_first} first and {keep_last} last ones"
     if not weights.is_cuda:
@@ -373,12 +377,11 @@ def kv4_keep(weights, positions, block_table, seq_lens, seen, budget, keep_first
     keep = torch.empty((B, hkv, budget), dtype=torch.int32, device=device)
     lens = torch.empty(B, dtype=torch.int32, device=device)
     if B:
-        width = block_table.shape[1]
         scratch = torch.empty((B, hkv, budget), dtype=torch.int32, device=device) if width * block > 4096 else None
         longest = width * block if max_seq_len is None else max(0, min(max_seq_len, width * block))
         _call("omni_kv4_keep", device, weights.data_ptr(), positions.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), seen.data_ptr(),
               keep.data_ptr(), lens.data_ptr(), _p(scratch), blocks,
-              block, hkv, block_table.stride(0), width, B, budget, keep_first, keep_last, longest, 0)
+              block, hkv, table_ld, width, B, budget, keep_first, keep_last, longest, 0)
     return keep, lens
 
 
@@ -390,7 +393,7 @@ def kv4_move(k_cache, v_cache, block_table, keep, weights=None, positions=None):
     assert keep.dim() == 3 and keep.shape[1] == hkv and keep.is_contiguous() and keep.dtype is torch.int32 and keep.device == device, \
         f"keep: contiguous int32 [B, {hkv}, budget] on {device}"
     B, _, budget = keep.shape
-    _check_table(block_table, device, B, block)
+    width, table_ld = _check_table(block_table, device, B, block)
     if weights is not None:
         _check_per_place("weights", weights, (blocks, hkv, block), device)
     if positions is not None:
@@ -399,4 +402,4 @@ def kv4_move(k_cache, v_cache, block_table, keep, weights=None, positions=None):
         _move_ref(k_cache, v_cache, block_table, keep, weights, positions)
     elif B and budget:
         _call("omni_kv4_move", device, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), keep.data_ptr(), _p(weights), _p(positions), blocks, block, hkv, d,
-              block_table.stride(0), block_table.shape[1], B, budget, 0)
+              table_ld, width, B, budget, 0)
