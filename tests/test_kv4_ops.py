@@ -468,6 +468,19 @@ def test_long_and_extreme_scores_that_are_not_kept(monkeypatch):
         test_attention_of_any_magnitude("cuda", 1.0, 1.0, 1.0, -0.3, rows)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [0, 1 << 28])
+@pytest.mark.parametrize("d,rows,hq,hkv", [(64, 16, 32, 2), (128, 256, 1, 1), (256, 32, 8, 1), (128, 51, 5, 1)])
+def test_weights_of_the_most_rows(monkeypatch, d, rows, hq, hkv, room):
+    monkeypatch.setattr(kv4, "KEPT_SCORES", room)
+    lens = [290, 17, 0]
+    f = Filled(d, lens, hkv, d, 32, "cuda")
+    q = torch.randn(len(lens) * rows, hq, d, generator=_gen(5)).bfloat16().cuda()
+    w = torch.ones(f.k_cache.shape[:3], device="cuda")
+    out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, d ** -0.5, weights=w, decay=0.25)
+    _check_decode(f, q, rows, d ** -0.5, out, w, torch.ones(f.k_cache.shape[:3]), 0.25)
+
+
 @BOTH
 @pytest.mark.parametrize("room", [0, 1 << 28])
 def test_weights_of_a_nan(monkeypatch, dev, room):
