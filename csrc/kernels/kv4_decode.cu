@@ -330,7 +330,7 @@ struct Kv4Query {
     // exponent of the factor: 13 - that of the largest, within what a factor and its inverse can be
     const int e = min(max(13 - ((int)(__float_as_uint(most) >> 23) - 127), -120), 120);
     const float up = copysignf(__uint_as_float((uint32_t)(127 + e) << 23), scale_log2);
-    const float un = fmaxf(fabsf(scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23), 0x1p-120f);
+    const float exact = fabsf(scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23), un = exact < 0x1p-120f ? 0x1p-120f : exact;      // a NaN stays one
     unit[0] = __shfl_sync(0xffffffffu, un, c * 8);
     unit[1] = __shfl_sync(0xffffffffu, un, c * 8 + 4);
 #pragma unroll
@@ -500,6 +500,10 @@ struct Kv4Sums {
           const float sub = EDGE && m[n][x] == -INFINITY ? 0.f : m[n][x] * q[n].unit[x];
           s[u][n][x] = ex2_fast(fmaf(s[u][n][x], q[n].unit[x], -sub));
           s[u][n][2 + x] = ex2_fast(fmaf(s[u][n][2 + x], q[n].unit[x], -sub));
+          if (EDGE) {                                                      // whatever the scale is
+            if (t0 + u * 16 + r >= sees[n][x]) s[u][n][x] = 0.f;
+            if (t0 + u * 16 + r + 8 >= sees[n][x]) s[u][n][2 + x] = 0.f;
+          }
           l[n][x] += s[u][n][x] + s[u][n][2 + x];
         }
 #pragma unroll
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
       for (int x = 0; x < 2; ++x) {
         const int i = warp * NQ + n * 8 + cc * 2 + x;
         if (r == 0) {
-          s_m[i] = sum.m[n][x] * q[n].unit[x];
+          s_m[i] = sum.m[n][x] == -INFINITY ? -INFINITY : sum.m[n][x] * q[n].unit[x];
           s_l[i] = sum.l[n][x];
         }
 #pragma unroll
