@@ -113,7 +113,7 @@ def kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights=No
         s = torch.einsum("rhd,hnd->rhn", q[b * rows:(b + 1) * rows].float(), k) * scale
         sees = n - rows + 1 + torch.arange(rows, device=q.device)
         s = s.masked_fill(t >= sees[:, None, None], float("-inf"))
-        p = torch.where(sees[:, None, None] > 0, torch.softmax(s, -1), torch.zeros_like(s))
+        p = torch.where(t < sees[:, None, None], torch.softmax(s, -1), torch.zeros_like(s))      # a NaN is of what its row sees
         for i in range(rows):
             m = max(0, int(sees[i]))
             out[b * rows + i] = torch.einsum("hn,hnd->hd", p[i, :, :m], v[:, :m])

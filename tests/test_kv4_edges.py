@@ -35,3 +35,20 @@ def test_scales_that_are_not_finite(monkeypatch, dev, lens, scale, room):
         blk, t = _places(f, b)
         want[blk, :, t] = float("nan")
     assert torch.equal(w.cpu().nan_to_num(nan=-1.0), want.nan_to_num(nan=-1.0))
+
+
+@BOTH
+@pytest.mark.parametrize("room", [0, 1 << 28])
+def test_a_query_that_is_not_finite(monkeypatch, dev, room):
+    """The first of three rows: NaN for itself and for the weights of what it sees.  The last two tokens are seen by the other rows
+    alone, and their weights are numbers."""
+    monkeypatch.setattr(kv4, "KEPT_SCORES", room)
+    n, rows, d = 50, 3, 64
+    f = Filled(4, [n], 1, d, 16, dev)
+    q = torch.randn(rows, 2, d, generator=_gen(1)).bfloat16()
+    q[0, 1, 7] = float("nan")
+    w = torch.zeros(f.k_cache.shape[:3], device=dev)
+    out = ops.kv4_decode(q.to(dev), f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.125, weights=w).cpu()
+    assert out[0, 1].isnan().all() and out.isnan().sum() == d
+    blk, t = _places(f, 0)
+    assert torch.equal(w.cpu()[blk, 0, t].isnan(), torch.arange(n) < n - rows + 1)
