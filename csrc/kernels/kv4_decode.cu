@@ -527,10 +527,11 @@ struct Kv4Sums {
               const float p0 = s[u][n][2 * e], p1 = s[u][n][2 * e + 1];
               float f0 = p0 * up, f1 = p1 * up;
               if (EDGE) {                                                  // an unseen token adds nothing, whatever its value
-                f0 = p0 == 0.f ? 0.f : f0;
-                f1 = p1 == 0.f ? 0.f : f1;
-                z[n][g][0] += p0 == 0.f ? 0.f : p0 * mid;
-                z[n][g][1] += p1 == 0.f ? 0.f : p1 * mid;
+                const int t = t0 + u * 16 + r + 8 * e;
+                f0 = t < sees[n][0] ? f0 : 0.f;
+                f1 = t < sees[n][1] ? f1 : 0.f;
+                z[n][g][0] += t < sees[n][0] ? p0 * mid : 0.f;
+                z[n][g][1] += t < sees[n][1] ? p1 * mid : 0.f;
               } else {
                 z[n][g][0] = fmaf(p0, mid, z[n][g][0]);
                 z[n][g][1] = fmaf(p1, mid, z[n][g][1]);
@@ -804,15 +805,12 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Decode a, Kv4Cache c, 
   }
   sum = warp_sum(sum);
   __syncthreads();
-  float acc = 0.f;
+  float acc = 0.f;                                                         // a part that sees nothing is 0; 0 times a NaN that is seen is NaN
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s)
-    if (s < parts && s_f[s] != 0.f) acc = fmaf(s_f[s], v[s], acc);
+    if (s < parts) acc = fmaf(s_f[s], v[s], acc);
 #pragma unroll 8
-  for (int s = AHEAD; s < parts; ++s) {
-    const float f = s_f[s], x = a.o_part[slot(s) * c.d + d];
-    acc += f == 0.f ? 0.f : f * x;
-  }
+  for (int s = AHEAD; s < parts; ++s) acc = fmaf(s_f[s], a.o_part[slot(s) * c.d + d], acc);
   a.out[(((long long)b * a.rows + tok) * a.hq + head) * c.d + d] = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
   if (d == 0 && a.lse != nullptr) a.lse[((long long)b * a.hq + head) * a.rows + tok] = sum == 0.f ? -INFINITY : mm + __log2f(sum);
 }

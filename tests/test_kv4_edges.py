@@ -7,6 +7,14 @@ from omni_infer_b200 import ops
 from omni_infer_b200.ops import kv4
 from test_kv4_ops import BOTH, Filled, _gen
 
+cuda = [pytest.mark.gpu]
+
+
+def _on_both(*sizes):
+    """Sizes for both devices, and behind a None those for a GPU alone: writing long caches takes the CPU too long."""
+    at = sizes.index(None) if None in sizes else len(sizes)
+    return [("cpu", *s) for s in sizes[:at]] + [pytest.param("cuda", *s, marks=cuda) for s in sizes if s is not None]
+
 
 def _places(f, b):
     t = torch.arange(f.lens[b])
@@ -52,3 +60,23 @@ def test_a_query_that_is_not_finite(monkeypatch, dev, room):
     assert out[0, 1].isnan().all() and out.isnan().sum() == d
     blk, t = _places(f, 0)
     assert torch.equal(w.cpu()[blk, 0, t].isnan(), torch.arange(n) < n - rows + 1)
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("dev,n", _on_both((100,), None, (3000,)))
+def test_a_nan_value_whose_weight_is_zero(dev, n, rows):
+    """0 NaN is NaN: whether a row gives a NaN goes by what it sees, not by where a token lies or by how small its weight has become.
+    The token's score is 25,600 below the others'."""
+    d = 128
+    for j in sorted({5, 40, n // 2, n - 3, n - 1}):
+        f = Filled(n, [n], 1, d, 16, dev)
+        f.k[0] *= 0.1
+        f.k[0][j] = -200.0
+        f.v[0][j, 0, 3] = float("nan")
+        ops.kv4_write(f.k[0].to(dev), f.v[0].to(dev), f.slots[0].to(dev), f.k_cache, f.v_cache)
+        q = torch.ones(rows, 8, d, dtype=torch.bfloat16, device=dev)
+        out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 1.0).cpu()
+        nan = torch.zeros(rows, 8, d, dtype=torch.bool)
+        for r in range(rows):
+            nan[r, :, :64] = j < n - rows + 1 + r
+        assert torch.equal(out.isnan(), nan), f"token {j}"
