@@ -9,7 +9,8 @@
 //   out   = sum over groups  sum_t (step_t p_t) (code - 8)  +  sum_t p_t (lowest_t + 8 step_t)
 // so keys and values are never rounded.  Behind the exponent of 1024 a code is an fp16 number with an offset (kv4_code below).  Queries become fp16
 // numbers without loss (a power of two for each row); the weights of the second product, step p_t, are rounded to fp16 once, after a
-// power of two that follows the largest step: 11 bits against the 8 of the result.  Values go in around 0: their offset would cost the
+// factor for each row and group that follows the largest of them: 11 bits against the 8 of the result, whatever the sizes of other groups and
+// tokens are.  Of the error against 64 bits, 1.66e-3 of a result, that makes under 1%.  Values go in around 0: their offset would cost the
 // fp32 sums over a long cache the bits that they need.
 //
 // A token takes 144 bytes of keys and values at d = 128 and a tile of 16 tokens serves 8 query rows per product.  Unpacking bounds the
@@ -191,6 +192,10 @@ __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t kv4_pack(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t kv4_max2(uint32_t x, uint32_t y) {             // of fp16 pairs; a NaN gives way to a number
+  const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ void kv4_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -402,11 +407,13 @@ struct Kv4Sums {
   using T = Kv4Tile<NG, true>;
   static constexpr int HALF = 32, SUBS = HALF / 16;
   float m[NT][2], l[NT][2], o[NT][NG][4][4], z[NT][NG][2];                 // m in the scores' own units
-  float most, to_one;               // power of two not below the value steps so far, and 128 over it
+  // o is in units of 1 / c: the largest of a row's weights times a group's steps becomes an fp16 number of 2^7 .. 2^15, whatever other rows, groups
+  // and tokens without weight have.  One factor for all, by the largest step, is 4% faster (2 x 131,067 tokens: 80.5 us against 84), but takes the
+  // codes from a group beside one 2^24 times as large, and from all tokens behind one that is and has no weight.
+  float c[NT][2][NG];
+  static constexpr float C_MOST = 0x1p118f;                                // times a weight still finite
 
   __device__ __forceinline__ void clear() {
-    most = 0.f;
-    to_one = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -416,6 +423,7 @@ struct Kv4Sums {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           z[n][g][x] = 0.f;
+          c[n][x][g] = C_MOST;                                             // what the first tokens have lowers it
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[n][g][j][x] = o[n][g][j][x + 2] = 0.f;
         }
@@ -426,7 +434,7 @@ struct Kv4Sums {
   template <bool EDGE, bool KEEP>
   __device__ __forceinline__ void add(const uint8_t* stage, int sub0, int t0, int end, const int (&sees)[NT][2], const Kv4Query<NG> (&q)[NT], float* scores) {
     const int lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
-    float s[SUBS][NT][4], top[NT][2], steps = 0.f;
+    float s[SUBS][NT][4], top[NT][2];
     uint32_t vs[SUBS][2][NG];
 #pragma unroll
     for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
@@ -468,8 +476,6 @@ struct Kv4Sums {
             for (int x = 0; x < 2; ++x)
               if (t >= sees[n][x]) s[u][n][2 * e + x] = -INFINITY;
         }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) steps = fmaxf(steps, kv4_step(vs[u][e][g]));
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -486,11 +492,11 @@ struct Kv4Sums {
             *reinterpret_cast<float2*>(scores + (long long)(t0 + u * 16 + r + 8 * e) * (8 * NT) + n * 8 + cc * 2) =
                 make_float2(s[u][n][2 * e] * q[n].unit[0], s[u][n][2 * e + 1] * q[n].unit[1]);
     }
-    // The maximum is followed only when a score exceeds it by 2^8: weights in fp32, and in fp16 after to_one, bear that.
-    bool more = steps > most;
+    // The maximum is followed only when a score exceeds it by 2^8: weights in fp32 bear that.
+    bool more = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) more |= (top[n][0] - m[n][0]) * q[n].unit[0] > 8.f || (top[n][1] - m[n][1]) * q[n].unit[1] > 8.f;
-    if (__any_sync(0xffffffffu, more)) rescale(top, steps, q);
+    if (__any_sync(0xffffffffu, more)) rescale(top, q);
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
 #pragma unroll
@@ -506,6 +512,45 @@ struct Kv4Sums {
           }
           l[n][x] += s[u][n][x] + s[u][n][2 + x];
         }
+    }
+    uint32_t pt[SUBS][NG][NT][2], most = 0u;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float step = kv4_step(vs[u][e][g]), mid = fmaf(step, 8.f, kv4_low(vs[u][e][g]));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float p0 = s[u][n][2 * e], p1 = s[u][n][2 * e + 1];
+            if (EDGE) {                                                    // an unseen token adds nothing, whatever its value
+              const int t = t0 + u * 16 + r + 8 * e;
+              z[n][g][0] += t < sees[n][0] ? p0 * mid : 0.f;
+              z[n][g][1] += t < sees[n][1] ? p1 * mid : 0.f;
+            } else {
+              z[n][g][0] = fmaf(p0, mid, z[n][g][0]);
+              z[n][g][1] = fmaf(p1, mid, z[n][g][1]);
+            }
+            pt[u][g][n][e] = product<EDGE>(p0, p1, step, n, g, t0 + u * 16 + r + 8 * e, sees);
+            most = kv4_max2(most, pt[u][g][n][e]);
+          }
+        }
+    // One of 2^15 or more.  Weights and products ahead of a single vote for maxima and factors were slower (more registers, or scores made again).
+    if (__any_sync(0xffffffffu, ((most + 0x08000800u) & 0x80008000u) != 0u)) {
+      lower(s, vs);
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              pt[u][g][n][e] = product<EDGE>(s[u][n][2 * e], s[u][n][2 * e + 1], kv4_step(vs[u][e][g]), n, g, t0 + u * 16 + r + 8 * e, sees);
+    }
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
 #pragma unroll
       for (int p = 0; p < T::PLANES; ++p) {
         uint32_t w[2][2 * T::PER];                                         // pairs of tokens c and c + 4: even (groups), odd (groups)
@@ -518,27 +563,11 @@ struct Kv4Sums {
 #pragma unroll
         for (int gp = 0; gp < T::PER; ++gp) {
           const int g = p * T::PER + gp;
-          uint32_t pt[NT][2];
+          uint32_t b[NT][2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float step = kv4_step(vs[u][e][g]), mid = fmaf(step, 8.f, kv4_low(vs[u][e][g])), up = step * to_one;
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float p0 = s[u][n][2 * e], p1 = s[u][n][2 * e + 1];
-              float f0 = p0 * up, f1 = p1 * up;
-              if (EDGE) {                                                  // an unseen token adds nothing, whatever its value
-                const int t = t0 + u * 16 + r + 8 * e;
-                f0 = t < sees[n][0] ? f0 : 0.f;
-                f1 = t < sees[n][1] ? f1 : 0.f;
-                z[n][g][0] += t < sees[n][0] ? p0 * mid : 0.f;
-                z[n][g][1] += t < sees[n][1] ? p1 * mid : 0.f;
-              } else {
-                z[n][g][0] = fmaf(p0, mid, z[n][g][0]);
-                z[n][g][1] = fmaf(p1, mid, z[n][g][1]);
-              }
-              pt[n][e] = kv4_transpose(kv4_pack(f0, f1));
-            }
-          }
+            for (int e = 0; e < 2; ++e) b[n][e] = kv4_transpose(pt[u][g][n][e]);
           const uint32_t x0 = __byte_perm(w[0][gp], w[0][T::PER + gp], 0x5410), y0 = __byte_perm(w[0][gp], w[0][T::PER + gp], 0x7632);
           const uint32_t x1 = __byte_perm(w[1][gp], w[1][T::PER + gp], 0x5410), y1 = __byte_perm(w[1][gp], w[1][T::PER + gp], 0x7632);
 #pragma unroll
@@ -547,23 +576,50 @@ struct Kv4Sums {
             const uint32_t f[4] = {j & 1 ? kv4_code<2>(v0) : kv4_code<0>(v0), j & 1 ? kv4_code<3>(v0) : kv4_code<1>(v0),
                                    j & 1 ? kv4_code<2>(v1) : kv4_code<0>(v1), j & 1 ? kv4_code<3>(v1) : kv4_code<1>(v1)};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) kv4_mma(o[n][g][j], f, pt[n]);
+            for (int n = 0; n < NT; ++n) kv4_mma(o[n][g][j], f, b[n]);
           }
         }
       }
     }
   }
 
-  __device__ __forceinline__ void rescale(const float (&top)[NT][2], float steps, const Kv4Query<NG> (&q)[NT]) {
-    steps = warp_max(steps);
-    float by = 1.f;
-    if (steps > most) {
-      const float next = fmaxf(__uint_as_float((__float_as_uint(steps) + 0x007fffffu) & 0x7f800000u), 0x1p-110f);
-      const float next_to_one = __uint_as_float(0x7f000000u - __float_as_uint(next)) * 128.f;
-      by = most * next_to_one * 0.0078125f;
-      most = next;
-      to_one = next_to_one;
+  // step p of rows 2 c and 2 c + 1, a token that is not seen has 0 whatever its value
+  template <bool EDGE>
+  __device__ __forceinline__ uint32_t product(float p0, float p1, float step, int n, int g, int t, const int (&sees)[NT][2]) const {
+    float f0 = p0 * c[n][0][g] * step, f1 = p1 * c[n][1][g] * step;
+    if (EDGE) {
+      f0 = t < sees[n][0] ? f0 : 0.f;
+      f1 = t < sees[n][1] ? f1 : 0.f;
     }
+    return kv4_pack(f0, f1);
+  }
+  // Where 32 tokens have products of 2^14 or more, the largest of them becomes 2^7 .. 2^8
+  __device__ __forceinline__ void lower(const float (&p)[SUBS][NT][4], const uint32_t (&vs)[SUBS][2][NG]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float v = 0.f;
+#pragma unroll
+          for (int u = 0; u < SUBS; ++u) v = fmaxf(v, fmaxf(p[u][n][x] * kv4_step(vs[u][0][g]), p[u][n][2 + x] * kv4_step(vs[u][1][g])));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+          if (v * c[n][x][g] >= 0x1p14f) {
+            const float next = __uint_as_float((261u - (__float_as_uint(v) >> 23)) << 23), by = next * rcp_fast(c[n][x][g]);
+            c[n][x][g] = next;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[n][g][j][x] *= by;
+              o[n][g][j][x + 2] *= by;
+            }
+          }
+        }
+  }
+
+  // New maxima.  o stays as it is while c can grow by what the weights lose.
+  __device__ __forceinline__ void rescale(const float (&top)[NT][2], const Kv4Query<NG> (&q)[NT]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -572,16 +628,23 @@ struct Kv4Sums {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
         v = fmaxf(v, m[n][x]);
-        const float f = v == -INFINITY ? 1.f : ex2_fast((m[n][x] - v) * q[n].unit[x]);
+        const float f = v == -INFINITY ? 1.f : ex2_fast((m[n][x] - v) * q[n].unit[x]), up = v == -INFINITY ? 1.f : ex2_fast((v - m[n][x]) * q[n].unit[x]);
         m[n][x] = v;
         l[n][x] *= f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           z[n][g][x] *= f;
+          const float next = c[n][x][g] * up;
+          if (next < C_MOST) {
+            c[n][x][g] = next;
+          } else {
+            const float by = f * C_MOST * rcp_fast(c[n][x][g]);
+            c[n][x][g] = C_MOST;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            o[n][g][j][x] *= f * by;
-            o[n][g][j][x + 2] *= f * by;
+            for (int j = 0; j < 4; ++j) {
+              o[n][g][j][x] *= by;
+              o[n][g][j][x + 2] *= by;
+            }
           }
         }
       }
@@ -688,7 +751,6 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
       }
       return;
     }
-    const float unit = sum.most * 0.0078125f;
     float* s_o = reinterpret_cast<float*>(smem);                           // [warps][NQ][D]
     float* s_m = s_o + KV4_WARPS * NQ * D;                                 // [warps][NQ], and the sums likewise
     float* s_l = s_m + KV4_WARPS * NQ;
@@ -702,11 +764,13 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, NT * NG > 2 ? 2 : 3) kv4_decod
           s_l[i] = sum.l[n][x];
         }
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int g = 0; g < NG; ++g) {
+          const float unit = 1.f / sum.c[n][x][g];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             *reinterpret_cast<float2*>(s_o + (size_t)i * D + g * 64 + r * 8 + j * 2) =
                 make_float2(fmaf(sum.o[n][g][j][x], unit, sum.z[n][g][x]), fmaf(sum.o[n][g][j][x + 2], unit, sum.z[n][g][x]));
+        }
       }
     __syncthreads();
     const bool whole = tile0 == 0 && end_tile == n_tiles;

@@ -3,6 +3,7 @@ different size, work cut through many requests, and what a cache's bytes are on 
 import pytest
 import torch
 
+import kv4_oracle as O
 from omni_infer_b200 import ops
 from omni_infer_b200.ops import kv4
 from test_kv4_ops import BOTH, Filled, _gen
@@ -80,3 +81,89 @@ def test_a_nan_value_whose_weight_is_zero(dev, n, rows):
         for r in range(rows):
             nan[r, :, :64] = j < n - rows + 1 + r
         assert torch.equal(out.isnan(), nan), f"token {j}"
+
+
+# ----------------------------------------------------------------------------- sizes
+def _bound(q, keys, values, h, m, scale):
+    """One row's heads [rep, d] of key/value head h that see m stored tokens -> result, weights, relative error of the weights, and what the result may
+    be off by.  Weights and sums as the oracle has them.  A product step p is rounded to fp16 after a power of two for each row and
+    group that brings the largest such product so far to 2^7 at least: it is off by 2^-11 of itself, or below fp16's normal numbers by 2^-25, which
+    (code - 8) <= 8 multiplies: 2^-29 of the row's largest step p for each of the m tokens at most."""
+    k, k_step, k_low = (x[:m, h] for x in keys)
+    v, v_step, v_low = (x[:m, h] for x in values)
+    o, p, rel, mass, _ = O.attention(q, k, v, scale, k_step, k_low, v_step, v_low)
+    mid = (v_low + 8 * v_step).repeat_interleave(64, -1)
+    far = (v - mid).abs()
+    top = (p[:, :, None] * v_step[None]).amax(1).repeat_interleave(64, -1)
+    carried = 2.0 ** -11 * (p @ far) + (m + 16) * 2.0 ** -24 * (p @ (far + mid.abs())) + m * 2.0 ** -29 * top
+    return o, p, rel, 2.0 ** -8 * o.abs() + (1 + 2.0 ** -8) * (rel * mass + carried) + 1e-38
+
+
+def _check(f, q, rows, scale, out, weights=None, most_rel=0.05):
+    """Against the formula; weights are those of a call with decay 0.  The bounds must be tight enough to notice a mistake: weights are
+    known to a twentieth at least."""
+    rep = q.shape[1] // f.hkv
+    q, out = q.cpu(), out.cpu().double()
+    for b, n in enumerate(f.lens):
+        keys, values = O.stored(f.k[b]), O.stored(f.v[b])
+        for h in range(f.hkv):
+            sums, tol = torch.zeros(n, dtype=torch.float64), torch.zeros(n, dtype=torch.float64)
+            for r in range(rows):
+                m, got = n - rows + 1 + r, out[b * rows + r, h * rep:(h + 1) * rep]
+                if m <= 0:
+                    assert (got == 0).all()
+                    continue
+                o, p, rel, bound = _bound(q[b * rows + r, h * rep:(h + 1) * rep], keys, values, h, m, scale)
+                assert rel.max() < most_rel, f"the bound says nothing: {rel.max():.3g}"
+                assert ((got - o).abs() <= bound).all(), f"request {b}, row {r}, head {h}: {((got - o).abs() / bound).max():.3g} bounds off"
+                sums[:m] += p.sum(0)
+                tol[:m] += (p * rel).sum(0)
+            if weights is not None and n:
+                blk, t = _places(f, b)
+                w = weights.cpu().double()[blk, h, t]
+                assert ((w - sums).abs() <= tol + 2.0 ** -21 * sums + rows * rep * 2.0 ** -126).all(), f"weights of request {b}, head {h}"
+
+
+def _few_columns(g, n, hq, d, size=1.0, columns=4):
+    """Queries of a few columns: their scores, and what a worst case makes of fp32 sums, stay small against keys of any step."""
+    q = torch.zeros(n, hq, d)
+    q[:, :, torch.randperm(d, generator=g)[:columns]] = size * torch.randn(n, hq, columns, generator=g)
+    return q.bfloat16()
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("dev,d,n", _on_both((128, 60), None, (128, 300), (64, 300), (256, 700), (128, 4000)))
+def test_value_groups_of_very_different_size(dev, d, n, rows):
+    """A group of a head is as exact beside one that is 2^60 times as large as it is alone."""
+    for down in (12, 20, 24, 32, 60):
+        f = Filled(down, [n], 2, d, 16, dev)
+        f.v[0][:, 0, :64] *= 2.0 ** -down
+        f.v[0][:, 1, -64:] *= 2.0 ** down
+        ops.kv4_write(f.k[0].to(dev), f.v[0].to(dev), f.slots[0].to(dev), f.k_cache, f.v_cache)
+        q = _few_columns(_gen(n), rows, 8, d, 3.0).to(dev)
+        out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, d ** -0.5)
+        _check(f, q, rows, d ** -0.5, out)
+
+
+@pytest.mark.parametrize("up", [20, 30, 60])
+@pytest.mark.parametrize("weight", [-18, -27, -60, 2])
+@pytest.mark.parametrize("dev,n,rows", _on_both((110, 2), None, (300, 1), (300, 3), (4000, 1)))
+def test_tokens_of_very_large_values_and_small_weight(dev, n, rows, weight, up):
+    """Values 2^up times the others', of tokens with scores that half the heads put at 2^weight of the others' and the other half nowhere in
+    particular: what a row gets of the others has to keep its bits."""
+    d = 64
+    g = _gen(n + up - weight)
+    for where in (slice(0, 1), slice(90, 91), slice(n - 3, n), slice(96, 128), slice(40, n)):
+        f = Filled(up, [n], 1, d, 16, dev)
+        f.k[0] = (f.k[0] * 0.25).bfloat16()
+        f.k[0][:, :, :32] = 0
+        f.k[0][where] = 0
+        f.k[0][where, :, :32] = 1.0
+        f.v[0][where] = (f.v[0][where].float() * 2.0 ** up).bfloat16()
+        ops.kv4_write(f.k[0].to(dev), f.v[0].to(dev), f.slots[0].to(dev), f.k_cache, f.v_cache)
+        q = torch.zeros(rows, 8, d)
+        q[:, :, 40:44] = torch.randn(rows, 8, 4, generator=g)
+        q[:, ::2, 0] = weight * 0.6931471805599453
+        q = q.bfloat16().to(dev)
+        out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 1.0)
+        _check(f, q, rows, 1.0, out)
