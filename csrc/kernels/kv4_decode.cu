@@ -39,11 +39,13 @@
 #include "../include/kv4.cuh"
 #include "../include/omni_ptx.cuh"
 #include "../include/score_mod.cuh"
+#include "../include/tma_host.h"
 
 namespace omni {
 
 constexpr int KV4_SITE_DECODE = 84, KV4_SITE_TILE = 85, KV4_SITE_WEIGHTS = 86;
 constexpr int KV4_WARPS = 4, KV4_STAGES = 2, KV4_MAX_BLOCKS = 4096;
+constexpr int KV4_WEIGHTS_ROWS = 256;       // most query rows a key/value head of a call that yields weights
 
 struct Kv4Decode {
   const __nv_bfloat16* q;
@@ -1129,16 +1131,6 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 3) kv4_weights_kernel(Kv4Decod
   }
 }
 
-// Shared memory beyond 48 KB is asked for once a device and kernel; `most` remembers how much.
-static cudaError_t kv4_smem(const void* kernel, int bytes, int (&most)[64]) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || (dev < 64 && most[dev] >= bytes)) return e;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) most[dev] = bytes;
-  return e;
-}
-
 // A launch that may begin while the kernel ahead of it ends; it waits for that one's results itself.
 template <typename... Args>
 static cudaError_t kv4_follow(void (*kernel)(Args...), dim3 grid, int threads, int bytes, cudaStream_t stream, Args... args) {
@@ -1162,8 +1154,8 @@ static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int 
   const int total = a.rows * (a.hq / c.hkv), chunks = (total + 8 * NT - 1) / (8 * NT);
   const long long grid = a.min_tiles == 0 ? (long long)B * c.hkv * chunks : blocks;
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  static int most[64] = {0};
-  cudaError_t e = kv4_smem((const void*)kv4_decode_kernel<NG, NT, KEEP>, bytes, most);
+  static bool asked[64] = {false};
+  cudaError_t e = (cudaError_t)ensure_dyn_smem((const void*)kv4_decode_kernel<NG, NT, KEEP>, bytes, asked);
   if (e != cudaSuccess) return e;
   kv4_decode_kernel<NG, NT, KEEP><<<(unsigned)grid, KV4_WARPS * 32, bytes, stream>>>(a, c, B, st);
   e = cudaGetLastError();
@@ -1181,9 +1173,11 @@ static cudaError_t kv4_launch(const Kv4Decode& a, const Kv4Cache& c, int B, int 
 template <int NG, int TOK>
 static cudaError_t kv4_launch_weights(const Kv4Decode& a, const Kv4Cache& c, int B, int max_len, OmniStatus* st, cudaStream_t stream) {
   const int total = a.rows * (a.hq / c.hkv), chunks = (total + 7) / 8;
-  const int bytes = KV4_WARPS * KV4_STAGES * Kv4Tile<NG, false, TOK>::BYTES + chunks * (NG * 64 * 16 + (1 + NG) * 4 * 16);
-  static int most[64] = {0};
-  cudaError_t e = kv4_smem((const void*)kv4_weights_kernel<NG, TOK>, bytes, most);
+  constexpr int stages = KV4_WARPS * KV4_STAGES * Kv4Tile<NG, false, TOK>::BYTES, each = NG * 64 * 16 + (1 + NG) * 4 * 16;
+  const int bytes = stages + chunks * each;
+  // the most that any call needs: threads whose calls have different rows set the same limit
+  static bool asked[64] = {false};
+  cudaError_t e = (cudaError_t)ensure_dyn_smem((const void*)kv4_weights_kernel<NG, TOK>, stages + KV4_WEIGHTS_ROWS / 8 * each, asked);
   if (e != cudaSuccess) return e;
   const long long shares = ((long long)B * c.hkv * ((max_len + TOK - 1) / TOK) + KV4_WARPS - 1) / KV4_WARPS, resident = 148 * 3;
   const unsigned grid = (unsigned)(shares < 1 ? 1 : shares < resident ? shares : resident);
@@ -1216,7 +1210,7 @@ extern "C" int omni_kv4_decode(const Kv4DecodeArgs* p, void* status, cudaStream_
   if (!kv4_shape_ok(c) || p->hq < 1 || p->hq % p->hkv != 0 || p->rows < 1 || p->hkv > 65535 || B > 65535 || p->min_tiles < 0 ||
       (p->row_tile != 8 && (p->row_tile != 16 || d > 128)))
     return -1;
-  if (p->weights != nullptr && (p->lse == nullptr || p->rows * rep > 256)) return -2;
+  if (p->weights != nullptr && (p->lse == nullptr || p->rows * rep > KV4_WEIGHTS_ROWS)) return -2;
   if (p->min_tiles > 0 && (p->o_part == nullptr || p->lse_part == nullptr || p->shared == nullptr || p->blocks_at_once < 1 || p->blocks_at_once > KV4_MAX_BLOCKS)) return -3;
   if (B <= 0) return 0;
   const int wide_q = (uintptr_t)p->q % 16 == 0 && p->q_row % 8 == 0 && p->q_head % 8 == 0;

@@ -1,0 +1,39 @@
+"""The 4-bit paged cache on the ways through its kernels that small calls do not take, and what it refuses on either device."""
+import threading
+
+import pytest
+import torch
+
+from omni_infer_b200 import ops
+from omni_infer_b200.ops import kv4
+from test_kv4_ops import Filled, _gen
+
+
+# ----------------------------------------------------------------------------- calls at once, and their count
+@pytest.mark.gpu
+def test_threads_with_calls_of_different_rows(monkeypatch):
+    """Calls from several host threads at once, each with another number of rows and so with another need of shared memory."""
+    monkeypatch.setattr(kv4, "KEPT_SCORES", 0)
+    f = Filled(14, [300, 80], 1, 64, 16, "cuda")
+    each = [1, 256, 9, 130, 2, 64, 255, 33]
+    qs = [torch.randn(2 * r, 1, 64, generator=_gen(r)).bfloat16().cuda() for r in each]
+    torch.cuda.synchronize()
+    got, ready = [None] * len(each), threading.Barrier(len(each))
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ready.wait()
+            for _ in range(5):
+                w = torch.zeros(f.k_cache.shape[:3], device="cuda")
+                got[i] = (ops.kv4_decode(qs[i], f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.125, weights=w), w)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(each))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for r, q, out in zip(each, qs, got):
+        assert out is not None, f"the call with {r} rows failed"
+        w = torch.zeros(f.k_cache.shape[:3], device="cuda")
+        assert torch.equal(out[0], ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.125, weights=w)) and torch.equal(out[1], w)
