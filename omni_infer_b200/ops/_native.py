@@ -40,7 +40,7 @@ def use_library(path) -> None:
     _LIB_PATH = Path(path)
 
 
-# kernels launched by one call of each entry point (entry points not listed launch one)
+# kernels launched by one call of each entry point (entry points not listed launch one; where it depends on the call, the caller adds the others)
 _KERNELS_PER_CALL = {"omni_moe_align": 2, "omni_ssd_chunks": 2}
 
 

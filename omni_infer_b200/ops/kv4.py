@@ -350,6 +350,7 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
         _call("omni_kv4_decode", device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(),
               o_part, lse_part, _p(lse), _p(weights), shared, _p(scores), q_row, blocks, q_head, block, hkv, d, table_ld, width, B, T // B, hq, longest, tile,
               blocks_at_once, min_tiles, scale, decay, 0)
+        nat.add_launches((min_tiles > 0) + (weights is not None))          # the kernels that join parts and make weights
     return out
 
 

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from omni_infer_b200 import ops
+from omni_infer_b200.ops import _native as nat
 from omni_infer_b200.ops import kv4
 from test_kv4_ops import Filled, _gen
 
@@ -37,3 +38,15 @@ def test_threads_with_calls_of_different_rows(monkeypatch):
         assert out is not None, f"the call with {r} rows failed"
         w = torch.zeros(f.k_cache.shape[:3], device="cuda")
         assert torch.equal(out[0], ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.125, weights=w)) and torch.equal(out[1], w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [0, 1 << 28])
+@pytest.mark.parametrize("n,weighted,launches", [(100, False, 1), (100, True, 2), (2000, False, 2), (2000, True, 3)])
+def test_launches_are_counted(monkeypatch, n, weighted, launches, room):
+    monkeypatch.setattr(kv4, "KEPT_SCORES", room)
+    f = Filled(1, [n], 1, 64, 16, "cuda")
+    w = torch.zeros(f.k_cache.shape[:3], device="cuda") if weighted else None
+    before = nat.launch_count()
+    ops.kv4_decode(torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda"), f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 1.0, weights=w)
+    assert nat.launch_count() - before == launches
