@@ -242,6 +242,7 @@ def _check_table(table, device, B, block):
     shape, stride = table.shape, table.stride()
     assert table.dtype is torch.int32 and table.device == device and len(shape) == 2 and shape[0] >= B and stride[1] == 1, \
         f"block_table: int32 on {device}, a row without gaps for each of the {B} requests"
+    assert B < 1 << 16, f"block_table: at most 65,535 requests: {B}"
     assert shape[1] * block < 1 << 30, f"block_table: fewer than 2^30 places for a request: {shape[1]} blocks of {block}"
     return shape[1], stride[0]
 
@@ -309,7 +310,7 @@ def _blocks(items, tiles, resident):
 def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=None, weights=None, decay=1.0):
     """Attention of the last tokens of every request over its cached ones: q [B n, Hq, d] bf16 (any row and head pitch), the ``n``
     rows of a request one after the other; row i sees the first ``seq_lens[b] - n + 1 + i`` of the request's places (none: zeros).
-    ``block_table`` [B, blocks of a request] int32, ``seq_lens`` [B] int32, with the rows' own tokens.  Returns [B n, Hq, d].
+    ``block_table`` [B, blocks of a request] int32 (B at most 65,535), ``seq_lens`` [B] int32, with the rows' own tokens.  Returns [B n, Hq, d].
     On a GPU the largest number of a query row is brought to 2^13 .. 2^14: keys beyond 2^98 may leave the range of the fp32 sums.
 
     ``weights`` [blocks, Hkv, block] fp32: of every place below seq_lens[b] becomes decay * weights + the softmax weights that the
@@ -326,12 +327,12 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
     width, table_ld = _check_table(block_table, device, B, block)
     if weights is not None:
         _check_per_place("weights", weights, (blocks, hkv, block), device)
+        assert T == 0 or T // B * (hq // hkv) <= 256, f"weights of at most 256 query rows a key/value head at once: {T // B * (hq // hkv)}"
     if not q.is_cuda:
         return kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights, decay)
     out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=device)
     if T:
         total = T // B * (hq // hkv)
-        assert weights is None or total <= 256, f"weights of at most 256 query rows a key/value head at once: {total}"
         longest = width * block if max_seq_len is None else max(0, min(max_seq_len, width * block))
         tile = 16 if d <= 128 and total > 8 else 8
         items = B * hkv * -(-total // tile)

@@ -7,7 +7,7 @@ import torch
 from omni_infer_b200 import ops
 from omni_infer_b200.ops import _native as nat
 from omni_infer_b200.ops import kv4
-from test_kv4_ops import Filled, _gen
+from test_kv4_ops import BOTH, Filled, _args, _gen
 
 
 # ----------------------------------------------------------------------------- calls at once, and their count
@@ -50,3 +50,24 @@ def test_launches_are_counted(monkeypatch, n, weighted, launches, room):
     before = nat.launch_count()
     ops.kv4_decode(torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda"), f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 1.0, weights=w)
     assert nat.launch_count() - before == launches
+
+
+# ----------------------------------------------------------------------------- refusals, the same on both devices
+def _many(a, n):
+    return torch.zeros(n, 2, dtype=torch.int32, device=a["lens"].device), torch.zeros(n, dtype=torch.int32, device=a["lens"].device)
+
+
+REFUSED = {
+    "weights of too many rows": lambda a: ops.kv4_decode(torch.zeros(2 * 129, 4, 64, dtype=torch.bfloat16, device=a["q"].device), a["kc"], a["vc"], a["table"], a["lens"],
+                                                         1.0, weights=a["w"]),
+    "too many requests to decode": lambda a: ops.kv4_decode(torch.zeros(1 << 16, 2, 64, dtype=torch.bfloat16, device=a["q"].device), a["kc"], a["vc"], *_many(a, 1 << 16), 1.0),
+    "too many requests to keep": lambda a: ops.kv4_keep(a["w"], a["pos"], *_many(a, 1 << 16), _many(a, 1 << 16)[1], 4),
+    "too many requests to move": lambda a: ops.kv4_move(a["kc"], a["vc"], _many(a, 1 << 16)[0], torch.full((1 << 16, 2, 1), -1, dtype=torch.int32, device=a["q"].device)),
+}
+
+
+@BOTH
+@pytest.mark.parametrize("what", list(REFUSED))
+def test_refusals_on_both_devices(dev, what):
+    with pytest.raises(AssertionError):
+        REFUSED[what](_args(dev))
