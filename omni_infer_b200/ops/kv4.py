@@ -12,7 +12,8 @@ every head, its own choice for each, in the places below the budget; ``positions
 
 Calls write to no memory but their outputs and what the allocator gives them for the call: they may run on several streams, and
 captured, as their arguments allow.  Block ids and slots outside the cache are reported by ``ops._native.check_status``: rows there
-are neither written nor read, and the attention of a request with such a block is not to be used."""
+are neither written nor read, and the attention of a request with such a block is not to be used.  The same goes for requests longer than
+their block table and for sources of a move below the budget.  On the CPU they are an IndexError, and nothing is changed."""
 from __future__ import annotations
 
 import ctypes
@@ -57,6 +58,26 @@ def kv4_quantise_ref(x):
     code = torch.round((v - lo[..., None]) / step[..., None]).clamp(0, 15)
     code = torch.where(step[..., None] > 0, code, torch.zeros_like(code))
     return code.to(torch.uint8).flatten(-2), step.bfloat16(), lo.bfloat16()
+
+
+def _inside(what, index, n):
+    """On the CPU a call stops at what a GPU skips and reports."""
+    if index.numel() and (int(index.min()) < 0 or int(index.max()) >= n):
+        raise IndexError(f"{what} outside 0 .. {n - 1}: {int(index.min())} .. {int(index.max())}")
+
+
+def _fits(block_table, b, n, block):
+    if n > block_table.shape[1] * block:
+        raise IndexError(f"request {b} of {n} tokens, and a block table for {block_table.shape[1] * block}")
+
+
+def _request_places(block_table, b, n, block, blocks):
+    """(block, place in it) of the first n places of request b"""
+    _fits(block_table, b, n, block)
+    t = torch.arange(n, device=block_table.device)
+    blk = block_table[b].long()[t // block]
+    _inside(f"blocks of request {b}", blk, blocks)
+    return blk, t % block
 
 
 def _pieces(cache):
@@ -104,12 +125,13 @@ def kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights=No
     B = seq_lens.shape[0]
     rows, rep = T // B if B else 0, hq // hkv
     out = torch.zeros(T, hq, d, dtype=torch.float32, device=q.device)
-    for b, n in enumerate(seq_lens.tolist()):
-        if n <= 0:
+    lens = [max(n, 0) for n in seq_lens.tolist()]
+    places = [_request_places(block_table, b, n, block, k_cache.shape[0]) for b, n in enumerate(lens)]
+    for b, (n, (blk, place)) in enumerate(zip(lens, places)):
+        if n == 0:
             continue
         t = torch.arange(n, device=q.device)
-        blk = block_table[b].long()[t // block]
-        k, v = (_values_ref(c, blk, t % block, x).transpose(0, 1).repeat_interleave(rep, 0) for c, x in ((k_cache, False), (v_cache, True)))
+        k, v = (_values_ref(c, blk, place, x).transpose(0, 1).repeat_interleave(rep, 0) for c, x in ((k_cache, False), (v_cache, True)))
         s = torch.einsum("rhd,hnd->rhn", q[b * rows:(b + 1) * rows].float(), k) * scale
         sees = n - rows + 1 + torch.arange(rows, device=q.device)
         s = s.masked_fill(t >= sees[:, None, None], float("-inf"))
@@ -119,8 +141,7 @@ def kv4_decode_ref(q, k_cache, v_cache, block_table, seq_lens, scale, weights=No
             out[b * rows + i] = torch.einsum("hn,hnd->hd", p[i, :, :m], v[:, :m])
         if weights is not None:
             step = p.sum(0).view(hkv, rep, n).sum(1).transpose(0, 1)                  # [n, Hkv]
-            old = weights[blk, :, t % block]
-            weights[blk, :, t % block] = step if decay == 0 else old * decay + step
+            weights[blk, :, place] = step if decay == 0 else weights[blk, :, place] * decay + step
     return out.to(q.dtype)
 
 
@@ -130,12 +151,13 @@ def kv4_keep_ref(weights, positions, block_table, seq_lens, seen, budget, keep_f
     keep = torch.full((B, hkv, budget), -1, dtype=torch.int32)
     lens = seq_lens.clamp(0, budget).to(torch.int32)
     for b, n in enumerate(seq_lens.tolist()):
-        t = torch.arange(max(n, 0))
-        blk = block_table[b].long()[t // block]
+        _fits(block_table, b, n, block)
+        if n > budget:                                        # else no block is looked at
+            blk, at = _request_places(block_table, b, n, block, weights.shape[0])
         for h in range(hkv):
             place = list(range(min(n, budget)))
             if n > budget:
-                w, pos = weights[blk, h, t % block].tolist(), positions[blk, h, t % block].tolist()
+                w, pos = weights[blk, h, at].tolist(), positions[blk, h, at].tolist()
                 rank = []
                 for j in range(n):
                     safe = pos[j] < keep_first or pos[j] >= int(seen[b]) - keep_last
@@ -149,9 +171,11 @@ def kv4_keep_ref(weights, positions, block_table, seq_lens, seen, budget, keep_f
 
 def _move_ref(k_cache, v_cache, block_table, keep, weights, positions):
     block = k_cache.shape[2]
-    to = torch.arange(keep.shape[2])
-    b, h, j = ((keep >= 0) & (keep != to)).nonzero(as_tuple=True)
+    budget = keep.shape[2]
+    b, h, j = ((keep >= 0) & (keep != torch.arange(budget))).nonzero(as_tuple=True)
     s = keep[b, h, j].long()
+    _inside("places from the budget on that tokens come from", s - budget, block_table.shape[1] * block - budget)
+    _inside("blocks of the tokens and of their places", block_table[torch.cat([b, b]), torch.cat([s, j]) // block], k_cache.shape[0])
     fb, ft, tb, tt = block_table[b, s // block].long(), s % block, block_table[b, j // block].long(), j % block
     for cache, values in ((k_cache, False), (v_cache, True)):
         flat, _, d = _pieces(cache)
@@ -263,6 +287,7 @@ def kv4_write(k, v, slots, k_cache, v_cache, weights=None, positions=None, token
         _check_per_place("positions", positions, (blocks, hkv, block), device, torch.int32)
         _check_numbers("token_positions", token_positions, T, device, torch.int64)
     if not k.is_cuda:
+        _inside("slots", slots.clamp_min(0), blocks * block)
         _write_ref(k, slots, k_cache, False)
         _write_ref(v, slots, v_cache, True)
         ok = slots >= 0
@@ -284,6 +309,7 @@ def kv4_read(k_cache, v_cache, slots):
     T = _check_numbers("slots", slots, None, device, torch.int64)
     if not k_cache.is_cuda:
         s = slots.clamp_min(0)
+        _inside("slots", s, blocks * block)
         ok = (slots >= 0)[:, None, None]
         return tuple(torch.where(ok, _values_ref(c, s // block, s % block, x), torch.zeros(())).bfloat16() for c, x in ((k_cache, False), (v_cache, True)))
     k = torch.empty((T, hkv, d), dtype=torch.bfloat16, device=device)

@@ -71,3 +71,27 @@ REFUSED = {
 def test_refusals_on_both_devices(dev, what):
     with pytest.raises(AssertionError):
         REFUSED[what](_args(dev))
+
+
+def test_blocks_and_slots_outside_the_cache_on_the_cpu():
+    """What a GPU skips and reports later is an error at once on the CPU, ahead of any change."""
+    a = _args()
+    lens, bad = torch.tensor([20, 20], dtype=torch.int32), torch.tensor([[0, 3], [-1, 1]], dtype=torch.int32)
+    before = [a[x].clone() for x in ("kc", "vc", "w", "pos")]
+    own, far = a["keep"].clone(), a["keep"].clone()
+    own[0, 0, 3] = 5                                         # place 5 is itself filled
+    far[0, 1, 2] = 40                                        # behind the table
+    for call in (lambda: ops.kv4_write(a["k"] + 1, a["k"] + 1, torch.tensor([0, 48, 1, 5]), a["kc"], a["vc"], weights=a["w"]),
+                 lambda: ops.kv4_read(a["kc"], a["vc"], torch.tensor([0, 48])),
+                 lambda: ops.kv4_decode(a["q"], a["kc"], a["vc"], bad, lens, 1.0, weights=a["w"]),
+                 lambda: ops.kv4_decode(a["q"], a["kc"], a["vc"], bad[1:].expand(2, -1), lens, 1.0, weights=a["w"]),
+                 lambda: ops.kv4_decode(a["q"], a["kc"], a["vc"], a["table"], lens + 13, 1.0),
+                 lambda: ops.kv4_keep(a["w"], a["pos"], bad[1:].expand(2, -1), lens, lens, 8),
+                 lambda: ops.kv4_keep(a["w"], a["pos"], a["table"], lens + 13, lens, 8),
+                 lambda: ops.kv4_keep(a["w"], a["pos"], a["table"], lens + 13, lens, 40),
+                 lambda: ops.kv4_move(a["kc"], a["vc"], bad[1:].expand(2, -1), torch.full((2, 2, 8), 20, dtype=torch.int32)),
+                 lambda: ops.kv4_move(a["kc"], a["vc"], a["table"], own, weights=a["w"]),
+                 lambda: ops.kv4_move(a["kc"], a["vc"], a["table"], far)):
+        with pytest.raises(IndexError):
+            call()
+    assert all(torch.equal(a[x], b) for x, b in zip(("kc", "vc", "w", "pos"), before))
