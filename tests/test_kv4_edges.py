@@ -167,3 +167,41 @@ def test_tokens_of_very_large_values_and_small_weight(dev, n, rows, weight, up):
         q = q.bfloat16().to(dev)
         out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 1.0)
         _check(f, q, rows, 1.0, out)
+
+
+@BOTH
+@pytest.mark.parametrize("room", [0, 1 << 28])
+@pytest.mark.parametrize("rows", [1, 5])
+@pytest.mark.parametrize("shape", ["up", "down", "peak", "waves"])
+def test_scores_that_move_far_within_known_bounds(monkeypatch, dev, shape, rows, room):
+    """The running maximum, with the sums that it rescales, follows scores over 600 and more.  The columns 64 and up of a key are alike, so that
+    their step is 0 and scores of any size have a small error, and the results' bounds are small against them: a result or weight
+    that is a tenth too large does not pass."""
+    monkeypatch.setattr(kv4, "KEPT_SCORES", room)
+    d, n = 128, 960
+    f = Filled(9, [n], 1, d, 64, dev)
+    t = torch.arange(n).float()
+    lift = {"up": t / 3, "down": (n - t) / 3, "peak": 250.0 * (t == 321), "waves": 160 + 160 * torch.sin(t / 40) * t / n}[shape]
+    f.k[0][:, 0, 64:] = torch.round(lift).clamp(0, 256)[:, None].bfloat16()
+    ops.kv4_write(f.k[0].to(dev), f.v[0].to(dev), f.slots[0].to(dev), f.k_cache, f.v_cache)
+    q = torch.zeros(rows, 8, d)
+    q[:, :, 3:7] = torch.randn(rows, 8, 4, generator=_gen(1)) * 0.5
+    q[:, :, 70] = torch.tensor([5.0, 1.0, 0.25, 0.0, -1.0, -5.0, 3.0, 2.0])
+    q = q.bfloat16().to(dev)
+    w = torch.full(f.k_cache.shape[:3], 0.25, device=dev)
+    out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, 0.5, weights=w, decay=0.0)
+    _check(f, q, rows, 0.5, out, w)
+    for wrong in (lambda: _check(f, q, rows, 0.5, out * 1.1), lambda: _check(f, q, rows, 0.5, out * 0), lambda: _check(f, q, rows, 0.5, out, w * 1.1)):
+        with pytest.raises(AssertionError, match="bounds off|weights of"):
+            wrong()
+
+
+@BOTH
+@pytest.mark.parametrize("q_size,scale", [(10.0, 0.09), (0.01, 0.09), (3e4, 1e-4), (2.0, -0.3), (1e-30, 1e29)])
+def test_queries_of_any_size_within_known_bounds(dev, q_size, scale):
+    for rows, d in ((1, 128), (5, 64), (2, 256)):
+        f = Filled(5, [333, 64], 2, d, 16, dev)
+        q = _few_columns(_gen(d), 2 * rows, 16, d, q_size, 3).to(dev)
+        w = torch.zeros(f.k_cache.shape[:3], device=dev)
+        out = ops.kv4_decode(q, f.k_cache, f.v_cache, f.table_dev, f.lens_dev, scale, weights=w, decay=0.0)
+        _check(f, q, rows, scale, out, w)
