@@ -13,16 +13,17 @@
 // tokens are.  Of the error against 64 bits, 1.66e-3 of a result, that makes under 1%.  Values go in around 0: their offset would cost the
 // fp32 sums over a long cache the bits that they need.
 //
-// A token takes 144 bytes of keys and values at d = 128 and a tile of 16 tokens serves 8 query rows per product.  Unpacking bounds the
-// kernel: integer and packed fp16 instructions issue every other cycle each and hardly overlap; some 145 + 48 of them a tile of 16 tokens
-// and 8 rows, 70 fp32 ones and 16 products make 550 cycles of an SM quarter against the 387 in which the tile's bytes arrive.  Two and
-// three blocks an SM run equally fast.  Of the memory's 6.46 TB/s a long cache gets 5.4 once the first tiles are there.
-// Products in e4m3, in which a code needs no offset, are slower: they are carried out as four times as many fp16 ones (130 us against 82).
+// A token takes 144 bytes of keys and values at d = 128 and a tile of 16 tokens serves 8 query rows per product.  Instructions bound the
+// kernel, though none of its units is full: 344 of them a tile of 16 tokens and 8 rows (some 150 integer, 48 packed fp16, 90 fp32, 16 products).  2 x 131,067
+// tokens of 8 heads in 80 us fill 58% of the issue slots, integer pipes to 50%, tensor pipes to 22%, and read at 59% of a copy's rate.  Of the 4.5
+// cycles that a warp takes an instruction, 1 issues it, 1 waits out a fixed latency, 0.9 wait for a busy pipe, 0.75 for other warps and 0.5 for
+// data; an SM quarter has 3 warps for that.  Two and three blocks an SM run equally fast.
+// Products in e4m3, in which a code needs no offset, are slower: they are carried out as four times as many fp16 ones (130 us when fp16 took 82).
 //
 // The query rows of a key/value head (rows x heads of its group, in tiles of 8) are the columns of the products (mma.sync m16n8k16), tokens and
 // then columns of the head their rows: S = K Q^T, O^T = V^T P^T.  So a group of 8 heads wastes nothing, and P^T, which wants tokens along its
 // rows, is what movmatrix makes of S.  tcgen05 products would want 64 or 128 rows and the unpacked codes in shared memory:
-// 128 rows a head over 30,011 tokens twice took 105 us that way, and 99 in tiles of 16 rows here (the softmax of a thread a row, and its waits for
+// 128 rows a head over 30,011 tokens twice took 105 us that way when they took 99 in tiles of 16 rows here (the softmax of a thread a row, and its waits for
 // products, unpacked tiles and tensor memory, took longer than unpacking a tile 8 times).
 //
 // Each warp walks tiles of 64 tokens (32 at d = 256) by itself: bulk copies of the tile's codes and scales two tiles ahead, an mbarrier
@@ -127,7 +128,7 @@ __device__ __forceinline__ bool kv4_work(const Kv4Decode& a, int block, int toke
   all *= items;
   const long long some = (long long)busy * items, blocks = gridDim.x;
   long long ahead;
-  if (some * 2 <= blocks) {                 // up to 218 uneven items of 444 blocks: 14 us against 17, 48 against 51; above, waste
+  if (some * 2 <= blocks) {                 // of 444 blocks, 32 uneven items take 14 us against 17 and 124 48 against 51; above half, waste
     w.share = max((long long)least, kv4_ceil(all, blocks - some));
     w.b = kv4_find(B, blockIdx.x, [&](int b) { return items * kv4_ceil(kv4_tiles(a, block, tokens, b), w.share); }, ahead);
     if (w.b < 0) return false;
@@ -291,7 +292,7 @@ struct Kv4Feed {
 };
 
 // Fragments of 8 query rows (row r: query token r / rep, head h rep + r % rep) as fp16 numbers, each row times a power of two that
-// brings its largest number to 2^13 .. 2^14: bf16 numbers keep all their bits down to 2^-28 of the largest.  qs are the sums of the
+// brings its largest number to 2^13 .. 2^14: bf16 numbers keep all their bits down to 2^-26 of the largest.  qs are the sums of the
 // groups, unit what brings scores to units of log 2 (its sign is that of the query), for the rows 2 c and 2 c + 1.
 // Key codes of odd columns are left as 16 (64 + code): their queries are a 16th.  The products start from `base`, which takes off what
 // the codes have too much: 64 for the odd columns, and too little: 8 for the even ones.

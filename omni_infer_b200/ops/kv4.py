@@ -320,8 +320,8 @@ def kv4_read(k_cache, v_cache, slots):
 
 
 # Bytes up to which the scores of a call are kept for its weights (a number for each row that a tile of them has, key/value head and place of
-# the block table); beyond they are made from the keys once more.  Kept, 32 requests of up to 4099 tokens and 8 rows a key/value head take
-# 38 us and not 46, 64 of 16,384 199 and not 260, two of 131,072 with 128 rows 557 and not 573: it is the memory that sets the bound.
+# the block table); beyond they are made from the keys once more.  Kept, 32 requests of 4099 tokens and 8 rows a key/value head take
+# 44 us and not 56, 64 of 16,384 197 and not 259, two of 131,072 with 128 rows 558 and not 578: it is the memory that sets the bound.
 KEPT_SCORES = 256 << 20
 
 
@@ -337,13 +337,15 @@ def kv4_decode(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len=No
     """Attention of the last tokens of every request over its cached ones: q [B n, Hq, d] bf16 (any row and head pitch), the ``n``
     rows of a request one after the other; row i sees the first ``seq_lens[b] - n + 1 + i`` of the request's places (none: zeros).
     ``block_table`` [B, blocks of a request] int32 (B at most 65,535), ``seq_lens`` [B] int32, with the rows' own tokens.  Returns [B n, Hq, d].
-    On a GPU the largest number of a query row is brought to 2^13 .. 2^14: keys beyond 2^98 may leave the range of the fp32 sums.
+    On a GPU the largest number of a query row is brought to 2^13 .. 2^14: keys beyond 2^98 may leave the range of the fp32 sums, and numbers below
+    2^-26 of the row's largest lose bits.
 
     ``weights`` [blocks, Hkv, block] fp32: of every place below seq_lens[b] becomes decay * weights + the softmax weights that the
     rows and the query heads of its key/value head give it (decay 0: whatever was there is dropped).  Requests that share a block
     would write the same numbers: give ``weights`` only where blocks belong to one request.  At most 256 rows times query
     heads of a key/value head then.  Up to 256 MiB go to scores meanwhile: 32 bytes (8 rows) to 1 KiB (256) for each place of the table
-    and key/value head, so a table no wider than needed saves memory.  ``max_seq_len`` (a bound of
+    and key/value head, so a table no wider than needed saves memory; ``ops.kv4.KEPT_SCORES`` is how many bytes they may take, and with fewer they
+    are made twice.  A captured graph keeps them.  ``max_seq_len`` (a bound of
     ``seq_lens``) shapes the launch; without it the width of the block table does."""
     blocks, hkv, block, d, device = _check_caches(k_cache, v_cache)
     (T, hq, _), (q_row, q_head, _) = _check_rows("q", q, None, d, device)
