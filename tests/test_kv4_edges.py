@@ -1,5 +1,5 @@
-"""The 4-bit paged cache where arithmetic and launches change their way: numbers that are not finite, groups and tokens of very
-different size, work cut through many requests, and what a cache's bytes are on either device."""
+"""Attention over the 4-bit paged cache where arithmetic is hardest: numbers that are not finite, groups and tokens of very different
+size, and scores that move far, within bounds that notice a tenth."""
 import pytest
 import torch
 
